@@ -39,7 +39,7 @@
 extern "C" {
 #endif
 
-#define NM_ABI_VERSION 11
+#define NM_ABI_VERSION 12
 #define NM_MAX_K 32
 
 typedef struct nm_grid_s* nm_grid_t;    /* spatial index over the mesh vertices */
@@ -391,6 +391,49 @@ int nm_train_composite_backward(const float* sdf, const float* s, const float* d
                                 const float* weights, const float* transmittance, const float* acc, const float* depth,
                                 const float* g_rgb, const float* g_depth, const float* g_acc, const float* g_normals,
                                 float* g_sdf, float* g_radiance, float* g_nablas, float* g_s, nm_stream_t stream);
+
+/* ----------------------------------------------------------------------------- dense layers
+ * y = act(x W^T + b) + r and its gradient, for rows of any width: x [M,K] (row stride ldx), W [N,K] (ldw), b [N], r [M,N] (ldr), y [M,N] (ldy), all
+ * of one element type (the bias: that type or fp32), last axis contiguous, any element alignment.  K, N <= 2^20; zero sizes are allowed
+ * (K = 0: y = act(b) + r).  Products accumulate in fp32 and are rounded once, at the end.
+ * act: softplus is log(1 + exp(beta z)) / beta (beta > 0; other activations ignore it), GELU in its tanh form.
+ * deriv [M,N] contiguous (fp16 beside 16-bit rows, fp32 beside fp32 rows): act'(z), what the backward pass needs; NULL = not wanted.  With
+ * NM_ACT_NONE nothing is written and the backward pass takes NULL.
+ * nm_dense_backward: g [M,N] cotangent of y -> dx [M,K] (lddx), dweight [N,K] contiguous, dbias [N] (NULL = not wanted; overwritten, not added to).  The
+ * gradient of r is g itself.  The result does not change from run to run.  fp32: a non-finite operand makes the outputs it enters
+ * NaN where IEEE arithmetic may give an infinity.
+ * workspace: nm_dense_workspace_bytes(.., backward) bytes, 16-byte aligned, of this call until its stream work is done. */
+enum { NM_F32 = 0, NM_F16 = 1, NM_BF16 = 2 };                 /* element types */
+enum { NM_ACT_NONE = 0, NM_ACT_RELU = 1, NM_ACT_SOFTPLUS = 2, NM_ACT_SIGMOID = 3, NM_ACT_SILU = 4, NM_ACT_GELU_TANH = 5 };
+int64_t nm_dense_workspace_bytes(int64_t M, int64_t K, int64_t N, int dtype, int backward);
+int nm_dense_forward(const void* x, int64_t ldx, const void* weight, int64_t ldw, const void* bias, int bias_dtype, const void* residual, int64_t ldr,
+                     int64_t M, int64_t K, int64_t N, int dtype, int act, float beta, void* y, int64_t ldy, void* deriv,
+                     void* workspace, int64_t workspace_bytes, nm_stream_t stream);
+int nm_dense_backward(const void* g, int64_t ldg, const void* deriv, const void* x, int64_t ldx, const void* weight, int64_t ldw, int64_t M, int64_t K,
+                      int64_t N, int dtype, void* dx, int64_t lddx, void* dweight, void* dbias, int bias_dtype,
+                      void* workspace, int64_t workspace_bytes, nm_stream_t stream);
+
+/* ----------------------------------------------------------------------------- gated linear recurrence
+ * Along S sequences of rows, in row order or (reverse) from the last row to the first, for every channel:
+ *   plain: h_i = gate_i h_{i-1} + x_i        blend: h_i = (1 - gate_i) h_{i-1} + gate_i x_i     (alpha compositing: gate = opacity, reverse = far to near)
+ * x, states [L,D] and gate [L,D] (shared_gate: [L], one for all channels), contiguous, any element alignment; the gate is of x's element type or fp32.
+ * |gate| <= 1 (blend: 0 <= gate <= 1) is expected: products of the factors over a sequence must stay finite.
+ * cu_seqlens == NULL: S sequences of L / S rows.  Otherwise DEVICE int32 [S+1], ascending: sequence s is rows cu[s] .. cu[s+1]-1; rows
+ * outside belong to none (their states and gradients are 0).  What an ill-formed cu_seqlens gives is unspecified but stays within the buffers.
+ * h0 [S,D] fp32 (NULL = 0): the state before a sequence.  states (NULL = not wanted): rounded once to x's type; last [S,D] fp32: the state
+ * behind a sequence's last step (an empty sequence's is its h0).
+ * keep (NULL = no backward pass will follow): nm_scan_keep_elems() floats that nm_scan_backward reads back.
+ * nm_scan_backward: cotangents g_states [L,D] of x's type and g_last [S,D] fp32 (NULL = 0) -> dgate, dx, dh0 in the types and shapes of gate, x, h0
+ * (NULL = not wanted; overwritten).  The results do not change from run to run.
+ * workspace: nm_scan_workspace_bytes(.., packed = cu_seqlens != NULL, backward) bytes, 16-byte aligned, of this call until its stream work is done. */
+int64_t nm_scan_workspace_bytes(int64_t L, int64_t S, int64_t D, int dtype, int packed, int backward);
+int64_t nm_scan_keep_elems(int64_t L, int64_t S, int64_t D, int dtype, int packed);
+int nm_scan_forward(const void* gate, int gate_dtype, int shared_gate, const void* x, int dtype, const float* h0, const int32_t* cu_seqlens,
+                    int64_t L, int64_t S, int64_t D, int reverse, int blend, void* states, float* last, float* keep,
+                    void* workspace, int64_t workspace_bytes, nm_stream_t stream);
+int nm_scan_backward(const void* gate, int gate_dtype, int shared_gate, const void* x, int dtype, const float* h0, const int32_t* cu_seqlens,
+                     int64_t L, int64_t S, int64_t D, int reverse, int blend, const float* keep, const void* g_states, const float* g_last,
+                     void* dgate, void* dx, float* dh0, void* workspace, int64_t workspace_bytes, nm_stream_t stream);
 
 /* ----------------------------------------------------------------------------- image assembly
  * What render.py:219-249 does on the host with the three outputs of a frame, per pixel, on the device

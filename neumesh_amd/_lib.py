@@ -11,8 +11,12 @@ import os
 
 from . import build as _build
 
-ABI_VERSION = 11
+ABI_VERSION = 12
 MAX_K = 32
+
+
+# element types of the free-standing operators (include/neumesh_hip.h: NM_F32, ...)
+DTYPE_F32, DTYPE_F16, DTYPE_BF16 = 0, 1, 2
 
 
 class GridInfo(C.Structure):
@@ -121,6 +125,16 @@ SIGNATURES = {
                                               _P, _P, _P, _P, _P, _P, _P, _P, _P]),
     "nm_surface_workspace_bytes": (C.c_int64, [_P, C.c_int64]),
     "nm_surface_hits": (C.c_int, [_P, _P, C.POINTER(FieldTables), _P, _P, C.c_int64, _P, C.POINTER(SurfaceCfg), _P, _P, _P, _P, _P, _P]),
+    "nm_dense_workspace_bytes": (C.c_int64, [C.c_int64, C.c_int64, C.c_int64, C.c_int, C.c_int]),
+    "nm_dense_forward": (C.c_int, [_P, C.c_int64, _P, C.c_int64, _P, C.c_int, _P, C.c_int64, C.c_int64, C.c_int64, C.c_int64, C.c_int, C.c_int, C.c_float,
+                                   _P, C.c_int64, _P, _P, C.c_int64, _P]),
+    "nm_dense_backward": (C.c_int, [_P, C.c_int64, _P, _P, C.c_int64, _P, C.c_int64, C.c_int64, C.c_int64, C.c_int64, C.c_int, _P, C.c_int64, _P, _P, C.c_int,
+                                    _P, C.c_int64, _P]),
+    "nm_scan_workspace_bytes": (C.c_int64, [C.c_int64, C.c_int64, C.c_int64, C.c_int, C.c_int, C.c_int]),
+    "nm_scan_keep_elems": (C.c_int64, [C.c_int64, C.c_int64, C.c_int64, C.c_int, C.c_int]),
+    "nm_scan_forward": (C.c_int, [_P, C.c_int, C.c_int, _P, C.c_int, _P, _P, C.c_int64, C.c_int64, C.c_int64, C.c_int, C.c_int, _P, _P, _P, _P, C.c_int64, _P]),
+    "nm_scan_backward": (C.c_int, [_P, C.c_int, C.c_int, _P, C.c_int, _P, _P, C.c_int64, C.c_int64, C.c_int64, C.c_int, C.c_int, _P, _P, _P, _P, _P, _P,
+                                   _P, C.c_int64, _P]),
     "nm_assemble_frame": (C.c_int, [_P, _P, _P, C.c_int64, C.c_int, _P, _P, _P, _P, _P]),
     "nm_profile_enable": (C.c_int, [C.c_int]),
     "nm_profile_read": (C.c_int, [C.c_int, C.POINTER(C.c_double), C.POINTER(C.c_int64), C.POINTER(C.c_int64)]),

@@ -8,13 +8,14 @@ from __future__ import annotations
 import os
 import shutil
 import subprocess
+import tempfile
 
 CSRC = os.path.join(os.path.dirname(os.path.abspath(__file__)), "csrc")
 LIB_PATH = os.path.join(CSRC, "libneumesh_hip.so")
 # the same sources with -DNM_TESTING: the product's exports + test hooks (host octree build, octree export, scalar-ALU self-check
 # of the MFMA tile code, phase stamps).  Loaded by a few tests and by the measurement tools only -- never by the package.
 TESTING_LIB_PATH = os.path.join(os.path.dirname(os.path.dirname(CSRC)), "tests", "_build", "libneumesh_hip_testing.so")
-SOURCES = ["nm_api.hip"]
+SOURCES = ["nm_api.hip", "nm_dense.hip", "nm_scan.hip"]   # one translation unit each, compiled in parallel
 HEADERS = sorted(f for f in os.listdir(CSRC) if f.endswith((".h", ".inc"))) + [os.path.join("..", "..", "include", "neumesh_hip.h")]
 FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-ffp-contract=off", "-fPIC", "-shared",
          "-Wno-unused-value",
@@ -35,10 +36,19 @@ def _compile(path: str, extra, verbose: bool) -> str:
     if not os.path.exists(hipcc):
         raise RuntimeError("hipcc not found: cannot build " + os.path.basename(path))
     os.makedirs(os.path.dirname(path), exist_ok=True)
-    cmd = [hipcc, *FLAGS, *extra, *[os.path.join(CSRC, s) for s in SOURCES], "-o", path + ".tmp"]
-    if verbose:
-        print(" ".join(cmd))
-    subprocess.check_call(cmd, cwd=CSRC)
+    with tempfile.TemporaryDirectory() as tmp:
+        objects = [os.path.join(tmp, os.path.splitext(s)[0] + ".o") for s in SOURCES]
+        flags = [f for f in FLAGS if f != "-shared"]
+        cmds = [[hipcc, *flags, *extra, "-c", os.path.join(CSRC, s), "-o", o] for s, o in zip(SOURCES, objects)]
+        link = [hipcc, "--offload-arch=gfx950", "-shared", "-fPIC", *objects, "-o", path + ".tmp"]
+        if verbose:
+            print("\n".join(" ".join(c) for c in cmds + [link]))
+        procs = [subprocess.Popen(c, cwd=CSRC) for c in cmds]
+        codes = [p.wait() for p in procs]
+        for c, code in zip(cmds, codes):
+            if code != 0:
+                raise subprocess.CalledProcessError(code, c)
+        subprocess.check_call(link, cwd=CSRC)
     os.replace(path + ".tmp", path)
     return path
 

@@ -16,6 +16,7 @@
 #include <vector>
 
 #include "../../include/neumesh_hip.h"
+#include "nm_error.h"
 #include "nm_grid_build.h"
 #include "nm_grid_build_dev.h"
 #include "nm_kernels.h"
@@ -31,7 +32,7 @@
 
 // ------------------------------------------------------------------------------ error state
 static thread_local std::string g_err;
-static int nm_fail(const char* fmt, ...) {
+int nm_fail(const char* fmt, ...) {
     char buf[512];
     va_list ap;
     va_start(ap, fmt);
@@ -40,16 +41,6 @@ static int nm_fail(const char* fmt, ...) {
     g_err = buf;
     return 1;
 }
-#define NM_HIP(call)                                                                          \
-    do {                                                                                      \
-        hipError_t e_ = (call);                                                               \
-        if (e_ != hipSuccess) return nm_fail("%s failed: %s", #call, hipGetErrorString(e_));  \
-    } while (0)
-#define NM_LAUNCH_CHECK()                                                                      \
-    do {                                                                                       \
-        hipError_t e_ = hipGetLastError();                                                     \
-        if (e_ != hipSuccess) return nm_fail("kernel launch failed: %s", hipGetErrorString(e_)); \
-    } while (0)
 
 // ------------------------------------------------------------------- in-stream kernel timing
 // When enabled (nm_profile_enable), every launch of the four hot kernels is bracketed by a pair

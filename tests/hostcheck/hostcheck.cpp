@@ -10,6 +10,7 @@
 
 #include "nm_grid_build.h"
 #include "nm_rays.h"
+#include "nm_scan_index.h"
 
 struct HostGridHandle {
     NmHostGrid g;
@@ -292,4 +293,12 @@ void hc_ray_composite(const float* sdf, const float* d, int64_t R, int N, float 
                          white, rgb + 3 * r, depth + r, acc + r, normals ? normals + 3 * r : nullptr, w);
     }
 }
+// packed recurrences: sequence of every row; first / last step of the reductions of a range (of the sequences of its last / first step)
+void hc_scan_sequences(const int* cu, int64_t S, int64_t L, int* out) {
+    for (int64_t r = 0; r < L; ++r) out[r] = nm_scan_sequence(cu, S, r);
+}
+int64_t hc_scan_reduce(const int* cu, int q, int reverse, int64_t L, int64_t c0, int64_t c1, int to) {
+    return to ? nm_scan_reduce_to(cu, q, reverse, L, c0, c1) : nm_scan_reduce_from(cu, q, reverse, L, c0, c1);
+}
+
 }

@@ -20,7 +20,7 @@ f32p, i64p = C.POINTER(C.c_float), C.POINTER(C.c_int64)
 
 def build(force=False):
     srcs = [os.path.join(_HERE, "hostcheck.cpp")] + [os.path.join(_CSRC, h) for h in
-                                                      ("nm_grid.h", "nm_grid_build.h", "nm_distance.h", "nm_rays.h")]
+                                                      ("nm_grid.h", "nm_grid_build.h", "nm_distance.h", "nm_rays.h", "nm_scan_index.h")]
     if force or not os.path.exists(_SO) or any(os.path.getmtime(s) > os.path.getmtime(_SO) for s in srcs):
         subprocess.check_call(["g++", "-O2", "-std=c++17", "-ffp-contract=off", "-fno-fast-math", "-fopenmp", "-shared",
                                "-fPIC", "-I" + _CSRC, srcs[0], "-o", _SO])
@@ -49,6 +49,9 @@ def load():
         lib.hc_ray_upsample_u.argtypes = [f32p, f32p, C.c_int64, C.c_int, C.c_int, C.c_int, C.c_int, f32p]
         lib.hc_ray_merge.argtypes = [f32p, f32p, C.c_int64, C.c_int, C.c_int, C.c_int]
         lib.hc_ray_composite.argtypes = [f32p, f32p, C.c_int64, C.c_int, C.c_float, f32p, f32p, C.c_int, f32p, f32p, f32p, f32p]
+        lib.hc_scan_sequences.argtypes = [C.c_void_p, C.c_int64, C.c_int64, C.c_void_p]
+        lib.hc_scan_reduce.restype = C.c_int64
+        lib.hc_scan_reduce.argtypes = [C.c_void_p, C.c_int, C.c_int, C.c_int64, C.c_int64, C.c_int64, C.c_int]
         _lib = lib
     return _lib
 

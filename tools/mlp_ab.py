@@ -11,7 +11,7 @@ if stamps and "NEUMESH_HIP_LIB" not in os.environ:   # (a pre-built variant may 
     from neumesh_amd import build as nb
     out = os.path.join(ROOT, "tools", "_build", "libneumesh_hip_stamps.so")
     os.makedirs(os.path.dirname(out), exist_ok=True)
-    subprocess.check_call(["hipcc", *nb.FLAGS, "-DNM_TESTING", os.path.join(nb.CSRC, "nm_api.hip"), "-o", out])
+    subprocess.check_call(["hipcc", *nb.FLAGS, "-DNM_TESTING", *[os.path.join(nb.CSRC, s) for s in nb.SOURCES], "-o", out])
     os.environ["NEUMESH_HIP_LIB"] = out
 import torch
 import bench, common
