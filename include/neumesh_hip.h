@@ -394,10 +394,11 @@ int nm_train_composite_backward(const float* sdf, const float* s, const float* d
 
 /* ----------------------------------------------------------------------------- dense layers
  * y = act(x W^T + b) + r and its gradient, for rows of any width: x [M,K] (row stride ldx), W [N,K] (ldw), b [N], r [M,N] (ldr), y [M,N] (ldy), all
- * of one element type (the bias: that type or fp32), last axis contiguous, any element alignment.  K, N <= 2^20; zero sizes are allowed
+ * of one element type (the bias: that type or fp32), last axis contiguous, any element alignment.  K, N <= 2^20, strides <= 2^24; zero sizes are allowed
  * (K = 0: y = act(b) + r).  Products accumulate in fp32 and are rounded once, at the end.
  * act: softplus is log(1 + exp(beta z)) / beta (beta > 0; other activations ignore it), GELU in its tanh form.
- * deriv [M,N] contiguous (fp16 beside 16-bit rows, fp32 beside fp32 rows): act'(z), what the backward pass needs; NULL = not wanted.  With
+ * deriv [M,N] contiguous, 2 bytes per element beside 16-bit rows, 4 beside fp32 rows: act'(z) in a form of the library's own, what the backward
+ * pass needs; NULL = not wanted.  With
  * NM_ACT_NONE nothing is written and the backward pass takes NULL.
  * nm_dense_backward: g [M,N] cotangent of y -> dx [M,K] (lddx), dweight [N,K] contiguous, dbias [N] (NULL = not wanted; overwritten, not added to).  The
  * gradient of r is g itself.  The result does not change from run to run.  fp32: a non-finite operand makes the outputs it enters

@@ -3,33 +3,57 @@
 //   z = x W^T + b,   y = act(z) + r          x [M,K], W [N,K], b [N], r and y [M,N]
 //   dz = g * act'(z);  dx = dz W;  dW = dz^T x;  db = sum over the rows of dz;  dr = g
 //
-// Three products, two kernels:
-//   nm_dense_kernel      forward and dx: rows x a weight matrix, contraction along the rows' contiguous axis
-//   nm_dense_grad_kernel dW and db: contraction over the rows, split over workgroups; nm_dense_sum_kernel adds the partial sums in a
+// Three products:
+//   nm_dense_resident_kernel, nm_dense_stream_kernel   forward and dx: rows x a weight matrix, contraction along the rows' contiguous axis
+//   nm_dense_grad_kernel  dW and db: contraction over the rows, split over workgroups; nm_dense_sum_kernel adds the partial sums in a
 //                        fixed order (the same bits from run to run)
-// nm_dense_few_kernel serves 1 .. 8 rows (a probe, a picked point) without the layout step of the weights.
+// nm_dense_few_kernel serves 1 .. 8 rows (a probe, a picked point).
 //
 // Arithmetic.  16-bit inputs: one product per pair on the f16 / bf16 pipe, fp32 accumulation, fp32 epilogue, one rounding at the end.  The
-// forward pass keeps act'(z) for the backward pass as fp16 (of either 16-bit type: its values lie in [-0.2, 1.2], where fp16 has 11 bits
-// and bf16 8); dz = g act'(z) enters the products as TWO 16-bit pieces (value + residual): a single rounded piece put an error as
+// forward pass keeps act'(z) for the backward pass in 16 bits that are finer than the rows' own (NmFactor); dz = g act'(z) enters the products as TWO 16-bit pieces (value + residual): a single rounded piece put an error as
 // large as the output's own rounding on dx and dW.  fp32 inputs: every operand cut into three bf16 pieces (nm_gemm.h: exact), six
 // piece products, fp32 accumulation; act'(z) is kept in fp32.  An fp32 product with a non-finite operand is NaN where IEEE
 // arithmetic may give an infinity.
 #include "nm_error.h"
 #include "nm_num.h"
 
+// act'(z) in 16 bits, values in (-2, 2).  Beside bf16 rows (8 bits): fp16 (11 bits).  Beside fp16 rows: fp16 with one bit of exponent traded for one of
+// mantissa -- 4 bits of exponent, 1.0 = 2^0 at the top of the range, 12 significant bits down to 2^-14, steps of 2^-25 below; all ones is NaN --
+// so that keeping act' does not cost what rounding the result costs.
+enum { NM_ACT16 = 3 };
+template <> struct NmType<NM_ACT16> { typedef unsigned short elem; };
+template <>
+__device__ __forceinline__ float nm_to_float<NM_ACT16>(unsigned short b) {
+    const unsigned m = b & 0x7fffu;
+    const unsigned f = __float_as_uint(__uint_as_float(m << 12) * 0x1p112f) | ((unsigned)(b & 0x8000u) << 16);
+    return m == 0x7fffu ? __builtin_nanf("") : __uint_as_float(f);
+}
+template <>
+__device__ __forceinline__ unsigned short nm_from_float<NM_ACT16>(float d) {
+    const unsigned m = (__float_as_uint(fabsf(d) * 0x1p-112f) + 0x800u) >> 12;
+    return (unsigned short)(d != d ? 0x7fffu : m | ((__float_as_uint(d) >> 16) & 0x8000u));
+}
+template <int DT> struct NmFactor { static constexpr int T = DT == NM_F32 ? (int)NM_F32 : DT == NM_F16 ? (int)NM_ACT16 : (int)NM_F16; };
+
 #define NM_D_MAX_DIM (1 << 20)   // columns and contraction lengths fit 32-bit arithmetic with room
+#define NM_D_MAX_LD (1 << 24)    // 64 rows of any stride stay below 2^32 bytes
 
 // ------------------------------------------------------------------------------------------------ activations
-// F32: the accurate exponential and division (fp32 outputs); otherwise the hardware approximations (16-bit outputs: errors of 1e-6 are far below
-// their rounding)
+// Exponentials and reciprocals from the hardware's approximations; F32 (fp32 outputs) corrects them to the last place (library exponential and division:
+// 70 instructions per element, 34 us of a 65536 x 256 layer), 16-bit outputs take them as they are (errors of 1e-6 are far below their rounding).
 template <bool F32>
-__device__ __forceinline__ float nm_d_exp(float x) {
-    return F32 ? expf(x) : __builtin_amdgcn_exp2f(x * 1.44269504088896341f);
+__device__ __forceinline__ float nm_d_exp(float x) {         // x <= 0
+    const float t = x * 1.44269504088896341f;
+    if (!F32) return __builtin_amdgcn_exp2f(t);
+    // what the rounded product t leaves of x log2(e), as a first-order factor: 1 + r ln 2
+    const float r = fmaf(x, 1.92596299112661746e-8f, fmaf(x, 1.44269504088896341f, -t));
+    const float e = __builtin_amdgcn_exp2f(t);
+    return x < -104.0f ? 0.0f : fmaf(e, r * 0.693147180559945309f, e);
 }
 template <bool F32>
-__device__ __forceinline__ float nm_d_rcp(float x) {
-    return F32 ? 1.0f / x : __builtin_amdgcn_rcpf(x);
+__device__ __forceinline__ float nm_d_rcp(float x) {         // 1 <= x <= 3
+    const float r = __builtin_amdgcn_rcpf(x);
+    return F32 ? fmaf(r, fmaf(-x, r, 1.0f), r) : r;          // one Newton step
 }
 
 // log(1 + e) for e in [0, 1]: 2 atanh(e / (2 + e)), series in s^2 <= 1/9 (truncation 1.4e-8 relative)
@@ -114,24 +138,28 @@ __device__ __forceinline__ void nm_d_two8(const float (&f)[8], uint4 (&p)[2]) {
     __builtin_memcpy(&p[1], lo, 16);
 }
 
-template <int DT>
-__device__ __forceinline__ nm_v16f nm_d_mfma(const uint4& a, const uint4& b, nm_v16f c) {
+// one matrix instruction: V = nm_v16f: 32 x 32 outputs, 16 deep;  nm_v4f: 16 x 16 outputs, 32 deep
+template <int DT, typename V>
+__device__ __forceinline__ V nm_d_mfma(const uint4& a, const uint4& b, V c) {
+    constexpr bool WIDE = sizeof(V) == 64;
     if constexpr (DT == NM_F16) {
         nm_v8h x, y;
         __builtin_memcpy(&x, &a, 16);
         __builtin_memcpy(&y, &b, 16);
-        return __builtin_amdgcn_mfma_f32_32x32x16_f16(x, y, c, 0, 0, 0);
+        if constexpr (WIDE) return __builtin_amdgcn_mfma_f32_32x32x16_f16(x, y, c, 0, 0, 0);
+        else return __builtin_amdgcn_mfma_f32_16x16x32_f16(x, y, c, 0, 0, 0);
     } else {
         nm_v8b x, y;
         __builtin_memcpy(&x, &a, 16);
         __builtin_memcpy(&y, &b, 16);
-        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(x, y, c, 0, 0, 0);
+        if constexpr (WIDE) return __builtin_amdgcn_mfma_f32_32x32x16_bf16(x, y, c, 0, 0, 0);
+        else return __builtin_amdgcn_mfma_f32_16x16x32_bf16(x, y, c, 0, 0, 0);
     }
 }
 
 // all piece products of one pair of fragments, small terms first.  Planes: PA of a, PB of b.
-template <int DT, int PA, int PB>
-__device__ __forceinline__ nm_v16f nm_d_products(const uint4 (&a)[PA], const uint4 (&b)[PB], nm_v16f c) {
+template <int DT, int PA, int PB, typename V>
+__device__ __forceinline__ V nm_d_products(const uint4 (&a)[PA], const uint4 (&b)[PB], V c) {
     if constexpr (PA == 3 && PB == 3) {      // dropped: a1 b2 + a2 b1 + a2 b2 < 2^-21 |a||b|
         c = nm_d_mfma<DT>(a[1], b[1], c);
         c = nm_d_mfma<DT>(a[0], b[2], c);
@@ -150,10 +178,15 @@ __device__ __forceinline__ nm_v16f nm_d_products(const uint4 (&a)[PA], const uin
 }
 
 // ------------------------------------------------------------------------------------------------ weights in fragment order
-// Column operand of nm_dense_kernel: element (c, q), output column c, contraction q.  Fragment (step q / 16, column tile c / 32): lane (i, h) holds
-// q = 16 step + 8 h .. + 7 of column 32 tile + nm_d_col(i).  An output tile of the matrix pipe gives a lane the rows (r & 3) + 8 (r >> 2) + 4 h of
-// the first operand: with this order of the columns they are 16 consecutive ones, which the epilogue stores as whole 16-byte pieces.
-__host__ __device__ __forceinline__ int nm_d_col(int i) { return 16 * ((i >> 2) & 1) + 4 * (i >> 3) + (i & 3); }
+// Column operand of the products rows x weights: element (c, q), output column c, contraction q.  Fragment (step q / 32, tile of 16 columns): lane
+// (i, h), i = lane % 16, holds q = 32 step + 8 h .. + 7 of the column at position i.  An output tile of the matrix pipe gives lane (j, h) the positions
+// 4 h .. 4 h + 3 of row j.  16-bit outputs: a pair of tiles is 32 columns, positions ordered so that the lane's eight values of the pair are
+// columns 8 h .. 8 h + 7 -- 16 bytes, and the four lanes of a row 64 bytes on end; fp32 outputs: columns in order, the lane's four values are
+// 16 bytes.  (32 x 32 tiles leave a row to two lanes: pieces of 16 bytes 32 apart made the stores three quarters of a memory-bound layer's time.)
+template <int DT>
+__host__ __device__ __forceinline__ int nm_d_column(int tile, int i) {
+    return DT == NM_F32 ? 16 * tile + i : 32 * (tile >> 1) + 8 * (i >> 2) + 4 * (tile & 1) + (i & 3);
+}
 
 // Eight consecutive contraction elements always come as ONE whole load: the piece that would end beyond Q starts at Q - 8 instead, and what it
 // repeats is zero on the packed side (and cleared on the rows' side, where it may be an infinity).  Q < 8: element by element from 0.
@@ -162,21 +195,19 @@ __host__ __device__ __forceinline__ long long nm_d_window(long long q0, long lon
 // pieces per weight element
 template <int DT> struct NmPlanes { static constexpr int W = DT == NM_F32 ? 3 : 1; };
 
-// dst [steps][tiles][plane][lane] (zero beyond C and Q); bias -> fp32 [32 tiles]
+// The streaming kernel's weights: dst [steps][tiles][plane][lane], zero beyond C and Q
 template <int DT>
 __global__ __launch_bounds__(256) void nm_dense_pack_kernel(const typename NmType<DT>::elem* __restrict__ w, long long ldw, int trans, int C, int Q, int tiles,
-                                                            int steps, uint4* __restrict__ dst, const void* __restrict__ bias, int bias_f32,
-                                                            float* __restrict__ bias_out) {
+                                                            int steps, uint4* __restrict__ dst) {
     typedef typename NmType<DT>::elem T;
     const long long t = (long long)blockIdx.x * 256 + threadIdx.x;
-    if (bias && t < 32LL * tiles) bias_out[t] = t >= C ? 0.f : bias_f32 ? ((const float*)bias)[t] : (float)((const T*)bias)[t];
-    const int lane = (int)(t & 63), i = lane & 31, h = lane >> 5;
+    const int lane = (int)(t & 63), h = lane >> 4;
     const long long frag = t >> 6;
     const int tile = (int)(frag % tiles);
     const long long step = frag / tiles;
     if (step >= steps) return;
-    const int c = 32 * tile + nm_d_col(i);
-    const long long q0 = 16 * step + 8 * h, s0 = nm_d_window(q0, Q);
+    const int c = nm_d_column<DT>(tile, lane & 15);
+    const long long q0 = 32 * step + 8 * h, s0 = nm_d_window(q0, Q);
     T e[8];
     if (!trans) {
         NmOct<DT> o = nm_oct_zero<DT>();
@@ -209,205 +240,419 @@ __global__ __launch_bounds__(256) void nm_dense_pack_kernel(const typename NmTyp
 // ------------------------------------------------------------------------------------------------ rows x weights
 struct NmDenseArgs {
     const void* A; long long lda;        // rows [R, Q]
-    const void* D;                       // PROD: factor of every element of A, contiguous [R, Q] (fp16 beside 16-bit rows, else fp32)
-    const uint4* W; int tiles;           // packed column operand
-    const float* bias;                   // [32 tiles] or NULL
+    const void* D;                       // PROD: factor of every element of A (NmFactor), contiguous [R, Q]
+    const void* W; long long ldw;        // column operand as it is: [C, Q], or (trans) [Q, C]
+    const uint4* P; int tiles;           // ... in fragment order (streaming kernel)
+    const void* bias;                    // [C] or NULL
+    int trans, bias_f32;
     const void* res; long long ldr;      // added after the activation, [R, C] or NULL
     void* Y; long long ldy;              // [R, C]
-    void* DV;                            // act'(z), contiguous [R, C] (fp16 / fp32) or NULL
+    void* DV;                            // act'(z) (NmFactor), contiguous [R, C], or NULL
     long long R;
     int Q, C, act;
     float beta;
     unsigned col_blocks;
 };
 
-// One workgroup: 4 waves, 128 RT rows x 32 NT columns.  A wave owns 32 RT whole rows: their elements go from global memory straight into fragments
-// (a lane's 8 consecutive elements of one row ARE a fragment), so the rows need no shared memory and are read once per column block; the column
-// operand is shared by the four waves through LDS, PS steps of 16 at a time in two buffers, one barrier per panel, both sides' next
-// panel in flight in registers meanwhile.
-template <int DT, bool PROD, int RT, int NT, int PS>
-__global__ __launch_bounds__(256, 2) void nm_dense_kernel(NmDenseArgs p) {
+// a piece of a row (times its factor) -> fragments
+template <int DT, bool PROD, int PX>
+__device__ __forceinline__ void nm_d_operand(const NmOct<DT>& a, const NmOct<NmFactor<DT>::T>& d, uint4 (&x)[PX]) {
+    if constexpr (DT != NM_F32 && !PROD) {
+        x[0] = a.v[0];
+    } else {
+        float f[8];
+        nm_oct_to_float<DT>(a, f);
+        if constexpr (PROD) {
+            float g[8];
+            nm_oct_to_float<NmFactor<DT>::T>(d, g);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) f[e] *= g[e];
+        }
+        if constexpr (DT == NM_F32) nm_d_cut8(f, x);
+        else nm_d_two8<DT>(f, x);
+    }
+}
+
+// piece q .. q + 7 of a row of Q (its window, nm_d_window); rows shorter than eight: from the first lane group alone
+template <int DT>
+__device__ __forceinline__ NmOct<DT> nm_d_fetch(const typename NmType<DT>::elem* row, int q, int Q) {
+    if (Q >= 8) return nm_oct_load<DT>(row + (q + 8 <= Q ? q : Q - 8));      // (uniform)
+    return nm_oct_load_short<DT>(row, q == 0 ? Q : 0);
+}
+
+// Eight columns of one row as the matrix pipe leaves them to a lane: 16-bit: on end; fp32: two quads, 16 columns apart.
+template <int DT>
+__device__ __forceinline__ NmOct<DT> nm_d_load_cols(const typename NmType<DT>::elem* row, int c, int C) {
+    if constexpr (DT != NM_F32) {
+        return nm_oct_load_row<DT>(row, c, C);
+    } else {
+        NmOct<DT> o;
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+            const int at = c + 16 * k;
+            o.v[k] = make_uint4(0, 0, 0, 0);
+            if (at + 4 <= C) __builtin_memcpy(&o.v[k], row + at, 16);
+            else if (at < C) o.v[k] = nm_oct_load_short<DT>(row + at, C - at).v[0];
+        }
+        return o;
+    }
+}
+template <int DT>
+__device__ __forceinline__ void nm_d_store_cols(typename NmType<DT>::elem* row, const float (&f)[8], int c, int C) {
+    if constexpr (DT != NM_F32) {
+        if (c < C) nm_oct_store_n<DT>(row + c, f, C - c);
+    } else {
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+            const int at = c + 16 * k;
+            if (at + 4 <= C) __builtin_memcpy(row + at, f + 4 * k, 16);
+            else {
+#pragma unroll
+                for (int i = 0; i < 3; ++i)
+                    if (at + i < C) row[at + i] = f[4 * k + i];
+            }
+        }
+    }
+}
+
+// accumulators of 16 RT rows x 32 NP columns -> bias (in LDS), activation, residual, stores.  A load waits for every store before it: a bias read from
+// global memory here, piece by piece, cost a 131072 x 256 layer 8 of 52 us.  So the residual (RES) of eight pieces is in flight before the first store, and
+// column blocks with one that stay resident have no more than eight pieces per wave.  The scheduling barriers keep the pieces apart, and the opaque column makes its tests, biases and
+// addresses HERE: mixed together or hoisted out of a loop over row tiles they cost 100 registers and spills.
+template <int DT, bool PROD, bool RES, int RT, int NP>
+__device__ __forceinline__ void nm_d_epilogue(const NmDenseArgs& p, const nm_v4f (&acc)[RT][2 * NP], const float* bias, long long m0, int cb,
+                                              int lane) {
     typedef typename NmType<DT>::elem T;
-    constexpr int PW = NmPlanes<DT>::W, PX = DT == NM_F32 ? 3 : PROD ? 2 : 1;
-    constexpr int DD = DT == NM_F32 ? NM_F32 : NM_F16;       // type of the factor
-    constexpr int PANEL = PS * NT * PW * 64;                 // uint4
-    constexpr int WV = PANEL / 256;
+    constexpr int DD = NmFactor<DT>::T, PIECES = RT * NP, AHEAD = PIECES < 8 ? PIECES : 8;
+    const float ibeta = 1.0f / p.beta;
+    const int cw = cb * (32 * NP) + (DT == NM_F32 ? 4 : 8) * (lane >> 4);
+    NmOct<DT> rs[AHEAD];
+    auto row_of = [&](int piece) { return m0 + 16 * (piece / NP) + (lane & 15); };
+    auto fetch = [&](int piece) {
+        if (!RES || !p.res || piece >= PIECES) return;
+        long long m = row_of(piece);
+        m = m < p.R ? m : p.R - 1;
+        int c = cw + 32 * (piece % NP);
+        asm volatile("" : "+v"(c));
+        rs[piece % AHEAD] = nm_d_load_cols<DT>((const T*)p.res + m * p.ldr, c, p.C);
+    };
+#pragma unroll
+    for (int k = 0; k < AHEAD; ++k) fetch(k);
+#pragma unroll
+    for (int k = 0; k < PIECES; ++k) {
+        __builtin_amdgcn_sched_barrier(0);
+        const int r = k / NP, n = k % NP;
+        const long long m = row_of(k);
+        int c = cw + 32 * n;
+        asm volatile("" : "+v"(c));
+        float z[8], dv[8], q[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) z[i] = acc[r][2 * n + (i >> 2)][i & 3];
+        if (!PROD && p.bias) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) z[i] += bias[c - cb * (32 * NP) + (DT == NM_F32 ? 16 * (i >> 2) + (i & 3) : i)];
+        }
+        if (RES && p.res) {
+            nm_oct_to_float<DT>(rs[k % AHEAD], q);
+            fetch(k + AHEAD);
+        }
+        if constexpr (!PROD) nm_d_act<DT == NM_F32>(p.act, p.beta, ibeta, z, dv);
+        if (m >= p.R) continue;
+        if constexpr (!PROD) {
+            if (p.DV) nm_d_store_cols<DD>((typename NmType<DD>::elem*)p.DV + m * p.C, dv, c, p.C);
+            if (RES && p.res) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) z[i] += q[i];
+            }
+        }
+        nm_d_store_cols<DT>((T*)p.Y + m * p.ldy, z, c, p.C);
+    }
+}
+
+template <int DT>
+__device__ __forceinline__ float nm_d_bias(const NmDenseArgs& p, int c) {
+    return c >= p.C ? 0.f : p.bias_f32 ? ((const float*)p.bias)[c] : (float)((const typename NmType<DT>::elem*)p.bias)[c];
+}
+
+// a weight block -> LDS in fragment order, [step][tile][plane][lane], by 512 threads; zero beyond C and Q
+template <int DT, int NP>
+__device__ __forceinline__ void nm_d_load_block(const NmDenseArgs& p, int cb, int steps, uint4* lds, int t) {
+    typedef typename NmType<DT>::elem T;
+    constexpr int PW = NmPlanes<DT>::W;
+    const T* w = (const T*)p.W;
+    if (!p.trans) {                                          // a lane's eight contraction elements lie on end: one piece each
+        const int n = steps * 2 * NP * 64;
+#pragma unroll 8
+        for (int i = t; i < n; i += 512) {
+            const int lane = i & 63, tile = (i >> 6) % (2 * NP), s = (i >> 6) / (2 * NP);
+            const int c = cb * (32 * NP) + nm_d_column<DT>(tile, lane & 15), q0 = 32 * s + 8 * (lane >> 4);
+            NmOct<DT> o = nm_d_fetch<DT>(w + (long long)(c < p.C ? c : p.C - 1) * p.ldw, q0, p.Q);
+            const int sh = c >= p.C ? 8 : p.Q < 8 || q0 + 8 <= p.Q ? 0 : q0 + 8 - p.Q;
+            o = nm_oct_clear_first<DT>(o, sh);
+            uint4* d = lds + (i >> 6) * (PW * 64) + lane;
+            if constexpr (DT == NM_F32) {
+                float f[8];
+                uint4 x[3];
+                nm_oct_to_float<DT>(o, f);
+                nm_d_cut8(f, x);
+#pragma unroll
+                for (int q = 0; q < 3; ++q) d[q * 64] = x[q];
+            } else {
+                *d = o.v[0];
+            }
+        }
+        return;
+    }
+    // transposed: eight rows x eight columns per thread, columns side by side over the threads
+    const int n = steps * 4 * (4 * NP);                      // groups of eight rows x groups of eight columns
+    for (int i = t; i < n; i += 512) {
+        const int g = i % (4 * NP), qg = i / (4 * NP);
+        const int c = cb * (32 * NP) + 8 * g, q0 = 8 * qg, s0 = (int)nm_d_window(q0, p.Q);
+        NmOct<DT> v[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const int q = s0 + e;
+            v[e] = nm_oct_zero<DT>();
+            if (q >= q0 && q < p.Q) v[e] = nm_oct_load_row<DT>(w + (long long)q * p.ldw, c, p.C);
+        }
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            // tile and position of column 8 g + e of the block
+            const int tile = DT == NM_F32 ? g >> 1 : 2 * (g >> 2) + (e >> 2), pos = DT == NM_F32 ? 8 * (g & 1) + e : 4 * (g & 3) + (e & 3);
+            uint4* d = lds + ((qg >> 2) * (2 * NP) + tile) * (PW * 64) + 16 * (qg & 3) + pos;
+            if constexpr (DT == NM_F32) {
+                float f[8], a[8];
+                uint4 x[3];
+#pragma unroll
+                for (int k = 0; k < 8; ++k) {
+                    nm_oct_to_float<DT>(v[k], a);
+                    f[k] = a[e];
+                }
+                nm_d_cut8(f, x);
+#pragma unroll
+                for (int q = 0; q < 3; ++q) d[q * 64] = x[q];
+            } else {
+                const unsigned sel = (e & 1) ? 0x07060302u : 0x05040100u;
+                unsigned r[8];
+#pragma unroll
+                for (int k = 0; k < 8; ++k) r[k] = (e >> 1) == 0 ? v[k].v[0].x : (e >> 1) == 1 ? v[k].v[0].y : (e >> 1) == 2 ? v[k].v[0].z : v[k].v[0].w;
+                *d = make_uint4(__builtin_amdgcn_perm(r[1], r[0], sel), __builtin_amdgcn_perm(r[3], r[2], sel), __builtin_amdgcn_perm(r[5], r[4], sel),
+                                __builtin_amdgcn_perm(r[7], r[6], sel));
+            }
+        }
+    }
+}
+
+// Many rows against a weight block that FITS in LDS (32-deep steps x 16-column tiles x pieces <= NM_D_RESIDENT KB): one persistent workgroup per CU loads
+// it once, and its eight waves then walk over tiles of 32 rows, each for itself, without another barrier.  A wave owns whole rows: their elements
+// go from global memory straight into fragments (a lane's 8 consecutive elements of one row ARE a fragment), RING steps ahead of their use
+// and across the end of a tile: the next tile's rows are in flight while this one's results are stored.
+#define NM_D_RESIDENT 144
+
+template <int DT, bool PROD, int NP>
+__global__ __launch_bounds__(512, 2) void nm_dense_resident_kernel(NmDenseArgs p) {
+    typedef typename NmType<DT>::elem T;
+    constexpr int PW = NmPlanes<DT>::W, PX = DT == NM_F32 ? 3 : PROD ? 2 : 1, DD = NmFactor<DT>::T;
+    constexpr int RING = DT == NM_F32 || (PROD && NP == 8) ? 2 : 4;
+    __shared__ uint4 lds[NM_D_RESIDENT * 64];
+    __shared__ float bias[32 * NP];
+    const int t = threadIdx.x, lane = t & 63, li = lane & 15, h = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
+    // consecutive workgroup numbers go to the eight XCDs in turn: the column blocks of one share of the rows sit on one XCD and read them together
+    const unsigned id = blockIdx.x, turn = id >> 3;
+    const int cb = (int)(turn % p.col_blocks);
+    const long long slot = (long long)(turn / p.col_blocks) * 8 + (id & 7), slots = gridDim.x / p.col_blocks;
+    const int steps = (p.Q + 31) / 32;
+    const long long tiles = (p.R + 31) / 32;
+    const T* arow[2];
+    const typename NmType<DD>::elem* drow[2];
+    auto rows_of = [&](long long tile) {
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+            long long m = tile * 32 + 16 * r + li;
+            m = m < p.R ? m : p.R - 1;
+            arow[r] = (const T*)p.A + m * p.lda;
+            drow[r] = PROD ? (const typename NmType<DD>::elem*)p.D + m * p.Q : nullptr;
+        }
+    };
+    NmOct<DT> xa[RING][2];
+    NmOct<DD> xd[RING][2];
+    auto fetch = [&](int s, NmOct<DT> (&a)[2], NmOct<DD> (&d)[2]) {
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+            a[r] = nm_d_fetch<DT>(arow[r], 32 * s + 8 * h, p.Q);
+            if constexpr (PROD) d[r] = nm_d_fetch<DD>(drow[r], 32 * s + 8 * h, p.Q);
+        }
+    };
+    long long tile = slot * 8 + wave;
+    if (tile < tiles) {
+        rows_of(tile);
+#pragma unroll
+        for (int u = 0; u < RING; ++u)
+            if (u < steps) fetch(u, xa[u], xd[u]);
+    }
+    nm_d_load_block<DT, NP>(p, cb, steps, lds, t);
+    if (!PROD && p.bias && t < 32 * NP) bias[t] = nm_d_bias<DT>(p, cb * (32 * NP) + t);
+    __syncthreads();
+    for (; tile < tiles; tile += slots * 8) {
+        nm_v4f acc[2][2 * NP];
+#pragma unroll
+        for (int r = 0; r < 2; ++r)
+#pragma unroll
+            for (int n = 0; n < 2 * NP; ++n) acc[r][n] = nm_v4f{0.f, 0.f, 0.f, 0.f};
+        const bool more = tile + slots * 8 < tiles;
+        for (int b = 0; b < steps; b += RING) {
+#pragma unroll
+            for (int u = 0; u < RING; ++u) {
+                const int s = b + u;
+                if (s >= steps) break;                       // (uniform)
+                __builtin_amdgcn_sched_barrier(0);           // (one step's pieces at a time)
+                uint4 x[2][PX];
+#pragma unroll
+                for (int r = 0; r < 2; ++r) {
+                    NmOct<DT> a = xa[u][r];
+                    NmOct<DD> d = xd[u][r];
+                    if (32 * s + 32 > p.Q && p.Q >= 8) {     // what the last whole load repeated
+                        const int q = 32 * s + 8 * h, sh = q + 8 <= p.Q ? 0 : q + 8 - p.Q;
+                        a = nm_oct_clear_first<DT>(a, sh);
+                        if constexpr (PROD) d = nm_oct_clear_first<DD>(d, sh);
+                    }
+                    nm_d_operand<DT, PROD>(a, d, x[r]);
+                }
+                if (s + RING < steps) {
+                    fetch(s + RING, xa[u], xd[u]);
+                } else if (more) {                           // the first use of this place in the next tile
+                    if (s == (steps > RING ? steps - RING : 0)) rows_of(tile + slots * 8);
+                    fetch(u, xa[u], xd[u]);
+                }
+#pragma unroll
+                for (int n = 0; n < 2 * NP; ++n) {
+                    uint4 w[PW];
+#pragma unroll
+                    for (int q = 0; q < PW; ++q) w[q] = lds[((s * (2 * NP) + n) * PW + q) * 64 + lane];
+#pragma unroll
+                    for (int r = 0; r < 2; ++r) acc[r][n] = nm_d_products<DT>(w, x[r], acc[r][n]);
+                }
+            }
+        }
+        nm_d_epilogue<DT, PROD, !PROD && NP <= 4, 2, NP>(p, acc, bias, tile * 32, cb, lane);
+    }
+}
+
+// Otherwise: one workgroup: 4 waves, 64 RT rows x 32 NP columns, both sides streamed.  The rows as above; the column operand is shared by the four waves
+// through LDS, PS steps at a time in two buffers, one barrier per panel, both sides' next panel in flight in registers meanwhile.
+template <int DT, bool PROD, int RT, int NP, int PS>
+__global__ __launch_bounds__(256, 2) void nm_dense_stream_kernel(NmDenseArgs p) {
+    typedef typename NmType<DT>::elem T;
+    constexpr int PW = NmPlanes<DT>::W, PX = DT == NM_F32 ? 3 : PROD ? 2 : 1, DD = NmFactor<DT>::T;
+    constexpr int STEP = 2 * NP * PW * 64, PANEL = PS * STEP, WV = PANEL / 256;      // uint4
     static_assert(PANEL % 256 == 0, "a panel is whole 16-byte pieces per thread");
     __shared__ uint4 lds[2][PANEL];
-    const int t = threadIdx.x, lane = t & 63, wave = t >> 6, li = lane & 31, h = lane >> 5;
-    // consecutive workgroup numbers go to the eight XCDs in turn: the column blocks of one row block follow each other on ONE of them
-    const unsigned id = blockIdx.x, xcd = id & 7, slot = id >> 3;
-    const long long rb = (long long)(slot / p.col_blocks) * 8 + xcd;
-    const int cb = (int)(slot % p.col_blocks);
-    const long long m0 = rb * (128 * RT) + wave * (32 * RT);
-    if (rb * (128 * RT) >= p.R) return;
-    const int steps = (p.Q + 15) / 16, panels = (steps + PS - 1) / PS;
+    __shared__ float bias[32 * NP];
+    const int t = threadIdx.x, lane = t & 63, wave = t >> 6, li = lane & 15, h = lane >> 4;
+    const unsigned id = blockIdx.x, turn = id >> 3;          // (XCDs: see above)
+    const long long rb = (long long)(turn / p.col_blocks) * 8 + (id & 7);
+    const int cb = (int)(turn % p.col_blocks);
+    const long long m0 = rb * (64 * RT) + wave * (16 * RT);
+    if (rb * (64 * RT) >= p.R) return;
+    const int steps = (p.Q + 31) / 32, panels = (steps + PS - 1) / PS;
     const T* arow[RT];
     const typename NmType<DD>::elem* drow[RT];
 #pragma unroll
     for (int r = 0; r < RT; ++r) {
-        long long m = m0 + 32 * r + li;
+        long long m = m0 + 16 * r + li;
         m = m < p.R ? m : p.R - 1;
         arow[r] = (const T*)p.A + m * p.lda;
         drow[r] = PROD ? (const typename NmType<DD>::elem*)p.D + m * p.Q : nullptr;
     }
-    nm_v16f acc[RT][NT];
+    nm_v4f acc[RT][2 * NP];
 #pragma unroll
     for (int r = 0; r < RT; ++r)
 #pragma unroll
-        for (int n = 0; n < NT; ++n)
-#pragma unroll
-            for (int i = 0; i < 16; ++i) acc[r][n][i] = 0.f;
+        for (int n = 0; n < 2 * NP; ++n) acc[r][n] = nm_v4f{0.f, 0.f, 0.f, 0.f};
 
     uint4 wv[WV];
-    NmOct<DT> xa[2][RT][PS];
-    NmOct<DD> xd[2][RT][PS];
+    NmOct<DT> xa[PS][RT];
+    NmOct<DD> xd[PS][RT];
     auto load_w = [&](int panel) {
 #pragma unroll
         for (int i = 0; i < WV; ++i) {
-            const int e = i * 256 + t, s = e / (NT * PW * 64), o = e % (NT * PW * 64);
-            wv[i] = p.W[((long long)(panel * PS + s) * p.tiles + cb * NT) * (PW * 64) + o];
+            const int e = i * 256 + t;
+            wv[i] = p.P[((long long)(panel * PS + e / STEP) * p.tiles + cb * (2 * NP)) * (PW * 64) + e % STEP];
         }
     };
     auto store_w = [&](int buf) {
 #pragma unroll
         for (int i = 0; i < WV; ++i) lds[buf][i * 256 + t] = wv[i];
     };
-    auto load_x = [&](int panel, NmOct<DT> (&a)[RT][PS], NmOct<DD> (&d)[RT][PS]) {
-        if (p.Q >= 8) {
+    auto load_x = [&](int panel, NmOct<DT> (&a)[PS][RT], NmOct<DD> (&d)[PS][RT]) {
 #pragma unroll
-            for (int r = 0; r < RT; ++r)
+        for (int s = 0; s < PS; ++s)
 #pragma unroll
-                for (int s = 0; s < PS; ++s) {
-                    const int q = panel * (16 * PS) + 16 * s + 8 * h, w = q + 8 <= p.Q ? q : p.Q - 8;
-                    a[r][s] = nm_oct_load<DT>(arow[r] + w);
-                    if constexpr (PROD) d[r][s] = nm_oct_load<DD>(drow[r] + w);
-                }
-        } else {                                             // (one step; lanes of the upper half have nothing)
-#pragma unroll
-            for (int r = 0; r < RT; ++r)
-#pragma unroll
-                for (int s = 0; s < PS; ++s) {
-                    a[r][s] = nm_oct_zero<DT>();
-                    if constexpr (PROD) d[r][s] = nm_oct_zero<DD>();
-                    if (s == 0 && h == 0) {
-                        a[r][s] = nm_oct_load_short<DT>(arow[r], p.Q);
-                        if constexpr (PROD) d[r][s] = nm_oct_load_short<DD>(drow[r], p.Q);
-                    }
-                }
-        }
+            for (int r = 0; r < RT; ++r) {
+                a[s][r] = nm_d_fetch<DT>(arow[r], (panel * PS + s) * 32 + 8 * h, p.Q);
+                if constexpr (PROD) d[s][r] = nm_d_fetch<DD>(drow[r], (panel * PS + s) * 32 + 8 * h, p.Q);
+            }
     };
     // the last panel: clear what a whole load repeated or brought beyond the row
-    auto trim = [&](int panel, NmOct<DT> (&a)[RT][PS], NmOct<DD> (&d)[RT][PS]) {
-        if ((panel + 1) * (16 * PS) <= p.Q || p.Q < 8) return;
+    auto trim = [&](int panel, NmOct<DT> (&a)[PS][RT], NmOct<DD> (&d)[PS][RT]) {
+        if ((panel + 1) * (32 * PS) <= p.Q || p.Q < 8) return;
 #pragma unroll
         for (int s = 0; s < PS; ++s) {
-            const int q = panel * (16 * PS) + 16 * s + 8 * h, sh = q + 8 <= p.Q ? 0 : q + 8 - p.Q;
+            const int q = (panel * PS + s) * 32 + 8 * h, sh = q + 8 <= p.Q ? 0 : q + 8 - p.Q;
 #pragma unroll
             for (int r = 0; r < RT; ++r) {
-                a[r][s] = nm_oct_clear_first<DT>(a[r][s], sh);
-                if constexpr (PROD) d[r][s] = nm_oct_clear_first<DD>(d[r][s], sh);
+                a[s][r] = nm_oct_clear_first<DT>(a[s][r], sh);
+                if constexpr (PROD) d[s][r] = nm_oct_clear_first<DD>(d[s][r], sh);
             }
         }
     };
-    auto compute = [&](int buf, const NmOct<DT> (&a)[RT][PS], const NmOct<DD> (&d)[RT][PS]) {
+    auto compute = [&](int buf, const NmOct<DT> (&a)[PS][RT], const NmOct<DD> (&d)[PS][RT]) {
 #pragma unroll
         for (int s = 0; s < PS; ++s) {
+            __builtin_amdgcn_sched_barrier(0);               // (one step's pieces at a time)
             uint4 x[RT][PX];
 #pragma unroll
-            for (int r = 0; r < RT; ++r) {
-                if constexpr (DT != NM_F32 && !PROD) {
-                    x[r][0] = a[r][s].v[0];
-                } else {
-                    float f[8];
-                    nm_oct_to_float<DT>(a[r][s], f);
-                    if constexpr (PROD) {
-                        float g[8];
-                        nm_oct_to_float<DD>(d[r][s], g);
+            for (int r = 0; r < RT; ++r) nm_d_operand<DT, PROD>(a[s][r], d[s][r], x[r]);
 #pragma unroll
-                        for (int e = 0; e < 8; ++e) f[e] *= g[e];
-                    }
-                    if constexpr (DT == NM_F32) nm_d_cut8(f, x[r]);
-                    else nm_d_two8<DT>(f, x[r]);
-                }
-            }
-#pragma unroll
-            for (int n = 0; n < NT; ++n) {
+            for (int n = 0; n < 2 * NP; ++n) {
                 uint4 w[PW];
 #pragma unroll
-                for (int q = 0; q < PW; ++q) w[q] = lds[buf][((s * NT + n) * PW + q) * 64 + lane];
+                for (int q = 0; q < PW; ++q) w[q] = lds[buf][((s * (2 * NP) + n) * PW + q) * 64 + lane];
 #pragma unroll
                 for (int r = 0; r < RT; ++r) acc[r][n] = nm_d_products<DT>(w, x[r], acc[r][n]);
             }
         }
     };
 
+    if (!PROD && p.bias && t < 32 * NP) bias[t] = nm_d_bias<DT>(p, cb * (32 * NP) + t);
     if (panels > 0) {
         load_w(0);
-        load_x(0, xa[0], xd[0]);
+        load_x(0, xa, xd);
         store_w(0);
     }
     __syncthreads();
-    for (int k = 0; k < panels; k += 2) {
+    for (int k = 0; k < panels; ++k) {
         // (a wave that is a panel ahead fills the OTHER buffer; nobody is two panels ahead: one barrier per panel)
+        NmOct<DT> na[PS][RT];
+        NmOct<DD> nd[PS][RT];
         if (k + 1 < panels) {
             load_w(k + 1);
-            load_x(k + 1, xa[1], xd[1]);
+            load_x(k + 1, na, nd);
         }
-        trim(k, xa[0], xd[0]);
-        compute(0, xa[0], xd[0]);
-        if (k + 1 >= panels) break;
-        store_w(1);
+        trim(k, xa, xd);
+        compute(k & 1, xa, xd);
+        if (k + 1 < panels) store_w((k + 1) & 1);
         __syncthreads();
-        if (k + 2 < panels) {
-            load_w(k + 2);
-            load_x(k + 2, xa[0], xd[0]);
-        }
-        trim(k + 1, xa[1], xd[1]);
-        compute(1, xa[1], xd[1]);
-        if (k + 2 < panels) store_w(0);
-        __syncthreads();
-    }
-
-    const float ibeta = 1.0f / p.beta;
 #pragma unroll
-    for (int r = 0; r < RT; ++r) {
-        const long long m = m0 + 32 * r + li;
-        if (m >= p.R) continue;
+        for (int s = 0; s < PS; ++s)
 #pragma unroll
-        for (int n = 0; n < NT; ++n) {
-            const int c0 = (cb * NT + n) * 32 + 16 * h;
-            if (c0 >= p.C) continue;
-            float z[16], dv[16];
-#pragma unroll
-            for (int i = 0; i < 16; ++i) z[i] = acc[r][n][i];
-            if (!PROD && p.bias) {
-#pragma unroll
-                for (int i = 0; i < 16; ++i) z[i] += p.bias[c0 + i];
+            for (int r = 0; r < RT; ++r) {
+                xa[s][r] = na[s][r];
+                if constexpr (PROD) xd[s][r] = nd[s][r];
             }
-            if constexpr (!PROD) nm_d_act<DT == NM_F32>(p.act, p.beta, ibeta, z, dv);
-#pragma unroll
-            for (int o = 0; o < 16; o += 8) {
-                const long long left = p.C - c0 - o;
-                if (left <= 0) break;
-                float f[8];
-#pragma unroll
-                for (int i = 0; i < 8; ++i) f[i] = z[o + i];
-                if (!PROD && p.res) {
-                    float q[8];
-                    nm_oct_to_float<DT>(nm_oct_load_row<DT>((const T*)p.res + m * p.ldr, c0 + o, p.C), q);
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) f[i] += q[i];
-                }
-                nm_oct_store_n<DT>((T*)p.Y + m * p.ldy + c0 + o, f, left);
-                if (!PROD && p.DV) {
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) f[i] = dv[o + i];
-                    nm_oct_store_n<DD>((typename NmType<DD>::elem*)p.DV + m * p.C + c0 + o, f, left);
-                }
-            }
-        }
     }
+    nm_d_epilogue<DT, PROD, !PROD, RT, NP>(p, acc, bias, m0, cb, lane);
 }
 
 // ------------------------------------------------------------------------------------------------ a few rows
@@ -452,70 +697,117 @@ __global__ __launch_bounds__(256) void nm_dense_few_kernel(const typename NmType
     if (res) h += (float)res[sub * ldr + n];
     y[sub * ldy + n] = (T)h;
     if (dv) {
-        if (DT == NM_F32) ((float*)dv)[(long long)sub * N + n] = d[0];
-        else ((_Float16*)dv)[(long long)sub * N + n] = (_Float16)d[0];
+        ((typename NmType<NmFactor<DT>::T>::elem*)dv)[(long long)sub * N + n] = nm_from_float<NmFactor<DT>::T>(d[0]);
     }
 }
 
 // ------------------------------------------------------------------------------------------------ weight and bias gradient
-// dW = dz^T x, contraction over the rows.  One workgroup: a 128 x 128 tile of dW over a range of rows, 64 rows at a time; 4 waves of 64 x 64.
-// The contraction is the SLOW axis of both operands.  A thread loads eight rows x eight columns (16-byte pieces, whole lines per row) and
-// transposes them in its own registers (one byte permute per two elements, or on the way through the product's fp32): it then holds, for each of its columns, eight consecutive rows --
-// a fragment -- and writes it to LDS in the order in which the waves read fragments.  Tile t, position i of the matrix pipe is column
-// 8 (i % 16) + 2 t + i / 16 of the 128.  Two waves bring dz (from g and act'(z), in two pieces or three), two bring x.
-__host__ __device__ __forceinline__ int nm_d_group(int c, int n) { return n < 8 || c + 8 <= n ? c : n - 8; }   // first column of the group at c
-
+// dW = dz^T x, contraction over the rows.  One workgroup: a 128 x 128 tile of dW over a range of rows, in blocks of 64 (fp32: 32); 4 waves of 64 x 64.
+// The contraction is the SLOW axis of both operands.  A thread loads eight rows x CG columns of each (8-byte pieces, whole lines per row) and
+// transposes them in its own registers (one byte permute per two elements, or on the way through the product's fp32): it then holds, for each of its
+// columns, eight consecutive rows -- a fragment -- and writes it to LDS in the order in which the waves read fragments.  Every wave brings its share of
+// dz (from g and act'(z), in two pieces or three) AND of x: the conversions, which cost as much as the products, are spread over the four
+// SIMDs.  The next block's rows are in flight while this one is multiplied.
 struct NmDenseGradArgs {
-    const void* G; long long ldg; const void* D;   // dz = G * D (D contiguous [R, N] fp16 / fp32, or NULL)
+    const void* G; long long ldg; const void* D;   // dz = G * D (D contiguous [R, N], NmFactor, or NULL)
     const void* X; long long ldx;
     long long R;
-    int N, K, n_tiles, k_tiles;
+    int N, K, n_tiles, k_tiles, splits;
     long long rows;                      // rows per workgroup (a multiple of 64)
     float* part;                         // [splits][n_tiles * k_tiles][16384] in the order of the accumulators
     float* bias_part;                    // [splits][128 n_tiles] or NULL
 };
 
-// 16-bit elements: column e of eight rows
+template <int DT> struct NmGroup { static constexpr int C = DT == NM_F32 ? 2 : 4; };    // columns of a thread: 8 bytes
+// Position i of the matrix pipe's tile t -> the thread group (of columns) and its column.  Lanes that follow each other sit at consecutive positions: whole
+// 256 bytes per 16 lanes go into LDS.
 template <int DT>
-__device__ __forceinline__ uint4 nm_d_column16(const NmOct<DT> (&r)[8], int e) {
+__host__ __device__ __forceinline__ void nm_d_place(int t, int i, int& group, int& e) {
+    if (DT == NM_F32) { group = i + 32 * (t & 1); e = t >> 1; }
+    else { group = i; e = t; }
+}
+// first column of the group that belongs at c: a group that would end beyond the row is the row's last one (nm_dense_sum_kernel takes the columns that
+// are its own)
+template <int DT>
+__host__ __device__ __forceinline__ int nm_d_group(int c, int n) { return n < NmGroup<DT>::C ? 0 : c + NmGroup<DT>::C <= n ? c : n - NmGroup<DT>::C; }
+
+// 8 bytes of elements at any element-aligned address
+template <int DT> struct NmPiece { typename NmType<DT>::elem e[8 / sizeof(typename NmType<DT>::elem)]; };
+template <int DT>
+__device__ __forceinline__ uint2 nm_d_load8(const typename NmType<DT>::elem* p) {
+    uint2 v;
+    __builtin_memcpy(&v, p, 8);
+    return v;
+}
+// The thread's eight rows 8 rg .. of a block of `rows` <= full rows at row `base`, columns col .. (ncol: of the array).  An address is a uniform base and a
+// 32-bit offset of the lane (strides are below 2^24): 24 addresses of 64 bits per lane cost more registers than the data.  All three forms are
+// straight code without branches per lane; rows beyond the block read its last row and are cleared.
+template <int DT>
+__device__ __forceinline__ void nm_d_load_rows(const typename NmType<DT>::elem* src, long long ld, int ncol, int col, long long base, int rows, int full, int rg,
+                                               uint2 (&v)[8]) {
+    typedef typename NmType<DT>::elem T;
+    constexpr unsigned E = sizeof(T);
+    const char* at = (const char*)(src + base * ld);
+    if (ncol >= (int)(8 / E) && rows == full) {              // (uniform)
+        const unsigned off = (unsigned)(rg * 8 * (unsigned)ld + col) * E;
+#pragma unroll
+        for (int r = 0; r < 8; ++r) v[r] = nm_d_load8<DT>((const T*)(at + r * ld * E + off));
+        return;
+    }
+#pragma unroll
+    for (int r = 0; r < 8; ++r) {
+        const int m = rg * 8 + r < rows ? rg * 8 + r : rows - 1;
+        const unsigned off = ((unsigned)m * (unsigned)ld + col) * E;
+        v[r] = make_uint2(0, 0);
+        if (ncol >= (int)(8 / E)) {
+            v[r] = nm_d_load8<DT>((const T*)(at + off));
+        } else if (ncol > 0) {                               // fewer columns than a group: one by one, the last one again
+            NmPiece<DT> x;
+#pragma unroll
+            for (int e = 0; e < (int)(8 / E); ++e) x.e[e] = *(const T*)(at + off + (e < ncol ? e : ncol - 1) * E);
+            __builtin_memcpy(&v[r], &x, 8);
+        }
+        if (rg * 8 + r >= rows) v[r] = make_uint2(0, 0);
+    }
+}
+template <int DT>
+__device__ __forceinline__ float nm_d_element(const uint2& v, int e) {
+    NmPiece<DT> x;
+    __builtin_memcpy(&x, &v, 8);
+    return nm_to_float<DT>(x.e[e]);
+}
+// 16-bit elements: column e of eight rows
+__device__ __forceinline__ uint4 nm_d_column16(const uint2 (&r)[8], int e) {
     const unsigned sel = (e & 1) ? 0x07060302u : 0x05040100u;
     unsigned w[8];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) w[j] = (e >> 1) == 0 ? r[j].v[0].x : (e >> 1) == 1 ? r[j].v[0].y : (e >> 1) == 2 ? r[j].v[0].z : r[j].v[0].w;
+    for (int j = 0; j < 8; ++j) w[j] = e < 2 ? r[j].x : r[j].y;
     return make_uint4(__builtin_amdgcn_perm(w[1], w[0], sel), __builtin_amdgcn_perm(w[3], w[2], sel), __builtin_amdgcn_perm(w[5], w[4], sel),
                       __builtin_amdgcn_perm(w[7], w[6], sel));
-}
-template <int DT>
-__device__ __forceinline__ float nm_d_element(const NmOct<DT>& o, int e) {
-    float f[8];
-    nm_oct_to_float<DT>(o, f);
-    return f[e];
 }
 
 template <int DT, bool PROD>
 __global__ __launch_bounds__(256, 2) void nm_dense_grad_kernel(NmDenseGradArgs p) {
     typedef typename NmType<DT>::elem T;
-    constexpr int DD = DT == NM_F32 ? NM_F32 : NM_F16;
+    constexpr int DD = NmFactor<DT>::T, CG = NmGroup<DT>::C;
+    typedef typename NmType<DD>::elem TD;
     constexpr int PZ = DT == NM_F32 ? 3 : PROD ? 2 : 1, PX = DT == NM_F32 ? 3 : 1;
-    constexpr int STEPS = DT == NM_F32 ? 2 : 4;              // steps of 16 rows in a block
-    constexpr int ROWS = 16 * STEPS;
-    constexpr int LZ = PZ * STEPS * 256, LX = PX * STEPS * 256;   // uint4: [plane][step][tile 4][lane 64]
-    __shared__ uint4 lds[LZ + LX];
+    constexpr int LANES = 128 / CG;                          // lanes side by side
+    constexpr int ROWS = 8 * 4 * (64 / LANES), STEPS = ROWS / 16;
+    __shared__ uint4 lds[(PZ + PX) * STEPS * 256];           // [plane][step][tile 4][lane 64], dz then x
+    constexpr int LZ = PZ * STEPS * 256;
     const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
-    const unsigned tile = blockIdx.x % (p.n_tiles * p.k_tiles), split = blockIdx.x / (p.n_tiles * p.k_tiles);
+    // the tiles of one range of rows on one XCD, at the same time: they read the same rows
+    const unsigned turn = blockIdx.x >> 3, tile = turn % (p.n_tiles * p.k_tiles), split = turn / (p.n_tiles * p.k_tiles) * 8 + (blockIdx.x & 7);
+    if ((int)split >= p.splits) return;
     const int tn = (int)(tile / p.k_tiles), tk = (int)(tile % p.k_tiles);
     const long long r0 = (long long)split * p.rows, r1 = r0 + p.rows < p.R ? r0 + p.rows : p.R;
-    const bool isz = wave < 2;                               // (wave-uniform)
-    // a thread's share of a block: columns 8 cg .. + 7 of eight rows; four row groups per wave.  16-bit: two waves bring 64 rows.  fp32: a block
-    // is 32 rows (three planes of 64 would leave one workgroup per CU): one wave of the two brings them.
-    const int cg = lane & 15, rg = (lane >> 4) + 4 * (wave & 1);
-    const bool active = rg * 8 < ROWS;
-    // (a group of columns that would end beyond the row is the row's last eight: nm_dense_sum_kernel takes the columns that are its own)
-    const int ncol = isz ? p.N : p.K, col = nm_d_group((isz ? tn : tk) * 128 + cg * 8, ncol);
-    const bool want_bias = isz && p.bias_part && tk == 0;
-    float bsum[8];
+    const int cg = t % LANES, rg = t / LANES;                // group of columns, group of eight rows
+    const int coln = nm_d_group<DT>(tn * 128 + cg * CG, p.N), colk = nm_d_group<DT>(tk * 128 + cg * CG, p.K);
+    const bool want_bias = p.bias_part && tk == 0;
+    float bsum[CG];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) bsum[e] = 0.f;
+    for (int e = 0; e < CG; ++e) bsum[e] = 0.f;
     nm_v16f acc[2][2];
 #pragma unroll
     for (int i = 0; i < 2; ++i)
@@ -524,73 +816,49 @@ __global__ __launch_bounds__(256, 2) void nm_dense_grad_kernel(NmDenseGradArgs p
 #pragma unroll
             for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.f;
 
-    NmOct<DT> va[8];
-    NmOct<DD> vd[8];
+    uint2 vg[8], vd[8], vx[8];
     auto load = [&](long long base) {
-        const T* src = isz ? (const T*)p.G : (const T*)p.X;
-        const long long ld = isz ? p.ldg : p.ldx;
-        const typename NmType<DD>::elem* fac = (const typename NmType<DD>::elem*)p.D;
-        if (base + ROWS <= r1 && ncol >= 8) {                // (uniform over the wave)
-            if (active) {
-#pragma unroll
-                for (int r = 0; r < 8; ++r) {
-                    const long long m = base + rg * 8 + r;
-                    va[r] = nm_oct_load<DT>(src + m * ld + col);
-                    if constexpr (PROD)
-                        if (isz) vd[r] = nm_oct_load<DD>(fac + m * p.N + col);
-                }
-            }
-            return;
-        }
-#pragma unroll
-        for (int r = 0; r < 8; ++r) {
-            const long long m = base + rg * 8 + r;
-            va[r] = nm_oct_zero<DT>();
-            if constexpr (PROD) vd[r] = nm_oct_zero<DD>();
-            if (m < r1 && active && ncol > 0) {
-                if (ncol >= 8) {
-                    va[r] = nm_oct_load<DT>(src + m * ld + col);
-                    if constexpr (PROD)
-                        if (isz) vd[r] = nm_oct_load<DD>(fac + m * p.N + col);
-                } else if (col == 0) {
-                    va[r] = nm_oct_load_short<DT>(src + m * ld, ncol);
-                    if constexpr (PROD)
-                        if (isz) vd[r] = nm_oct_load_short<DD>(fac + m * p.N, ncol);
-                }
-            }
-        }
+        const int rows = r1 - base < ROWS ? (int)(r1 - base) : ROWS;
+        nm_d_load_rows<DT>((const T*)p.G, p.ldg, p.N, coln, base, rows, ROWS, rg, vg);
+        if constexpr (PROD) nm_d_load_rows<DD>((const TD*)p.D, p.N, p.N, coln, base, rows, ROWS, rg, vd);
+        nm_d_load_rows<DT>((const T*)p.X, p.ldx, p.K, colk, base, rows, ROWS, rg, vx);
     };
-    // a fragment of this thread -> LDS: column e of its eight is position 16 (e & 1) + cg of tile e >> 1
-    auto put = [&](uint4* base, const uint4& c, int e) { base[(rg >> 1) * 256 + (e >> 1) * 64 + (rg & 1) * 32 + (e & 1) * 16 + cg] = c; };
+    // a fragment of this thread -> LDS: its column e, rows 8 rg ..
+    auto put = [&](uint4* base, const uint4& c, int e) {
+        const int tt = DT == NM_F32 ? 2 * e + (cg >> 5) : e;
+        base[(rg >> 1) * 256 + tt * 64 + (rg & 1) * 32 + (cg & 31)] = c;
+    };
     auto stash = [&]() {
-        if (!active) return;
-        uint4* base = isz ? lds : lds + LZ;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {                        // one column: eight rows -> a fragment per plane
-            if (DT != NM_F32 && !(isz && (PROD || want_bias))) {
-                if constexpr (DT != NM_F32) put(base, nm_d_column16<DT>(va, e), e);
-                continue;
-            }
+        for (int e = 0; e < CG; ++e) {                       // one column: eight rows -> a fragment per plane
+            __builtin_amdgcn_sched_barrier(0);               // (one column's temporaries at a time)
             float f[8];
 #pragma unroll
             for (int r = 0; r < 8; ++r) {
-                f[r] = nm_d_element<DT>(va[r], e);
-                if constexpr (PROD)
-                    if (isz) f[r] *= nm_d_element<DD>(vd[r], e);
+                f[r] = nm_d_element<DT>(vg[r], e);
+                if constexpr (PROD) f[r] *= nm_d_element<DD>(vd[r], e);
                 if (want_bias) bsum[e] += f[r];
             }
             if constexpr (DT == NM_F32) {
                 uint4 c[3];
                 nm_d_cut8(f, c);
 #pragma unroll
-                for (int q = 0; q < 3; ++q) put(base + q * STEPS * 256, c[q], e);
-            } else if constexpr (PROD) {
-                uint4 c[2];
-                nm_d_two8<DT>(f, c);
-                put(base, c[0], e);
-                put(base + STEPS * 256, c[1], e);
+                for (int q = 0; q < 3; ++q) put(lds + q * STEPS * 256, c[q], e);
+#pragma unroll
+                for (int r = 0; r < 8; ++r) f[r] = nm_d_element<DT>(vx[r], e);
+                nm_d_cut8(f, c);
+#pragma unroll
+                for (int q = 0; q < 3; ++q) put(lds + LZ + q * STEPS * 256, c[q], e);
             } else {
-                put(base, nm_d_column16<DT>(va, e), e);
+                if constexpr (PROD) {
+                    uint4 c[2];
+                    nm_d_two8<DT>(f, c);
+                    put(lds, c[0], e);
+                    put(lds + STEPS * 256, c[1], e);
+                } else {
+                    put(lds, nm_d_column16(vg, e), e);
+                }
+                put(lds + LZ, nm_d_column16(vx, e), e);
             }
         }
     };
@@ -599,10 +867,11 @@ __global__ __launch_bounds__(256, 2) void nm_dense_grad_kernel(NmDenseGradArgs p
     if (r0 < r1) load(r0);
     for (long long b = r0; b < r1; b += ROWS) {
         stash();
-        __syncthreads();
         if (b + ROWS < r1) load(b + ROWS);
+        __syncthreads();
 #pragma unroll
         for (int s = 0; s < STEPS; ++s) {
+            if (s % 2 == 0) __builtin_amdgcn_sched_barrier(0);
             uint4 z[2][PZ], x[2][PX];
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
@@ -627,54 +896,69 @@ __global__ __launch_bounds__(256, 2) void nm_dense_grad_kernel(NmDenseGradArgs p
             for (int r = 0; r < 16; r += 4)
                 *reinterpret_cast<float4*>(out + ((i * 2 + j) * 4 + (r >> 2)) * 256 + lane * 4) =
                     make_float4(acc[i][j][r], acc[i][j][r + 1], acc[i][j][r + 2], acc[i][j][r + 3]);
-    if (!p.bias_part || tk != 0) return;                      // (uniform over the workgroup)
-    float* sh = reinterpret_cast<float*>(lds);
-    if (isz) {
+    if (!want_bias) return;                                  // (uniform over the workgroup)
+    float* sh = reinterpret_cast<float*>(lds);               // [row group][128]
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            bsum[e] += __shfl_xor(bsum[e], 16);
-            bsum[e] += __shfl_xor(bsum[e], 32);
-            if (lane < 16) sh[wave * 128 + cg * 8 + e] = bsum[e];
-        }
-    }
+    for (int e = 0; e < CG; ++e) sh[rg * 128 + cg * CG + e] = bsum[e];
     __syncthreads();
-    if (t < 128) p.bias_part[((long long)split * p.n_tiles + tn) * 128 + t] = sh[t] + sh[128 + t];
+    if (t < 128) {
+        float b = 0.f;
+#pragma unroll
+        for (int g = 0; g < ROWS / 8; ++g) b += sh[g * 128 + t];
+        p.bias_part[((long long)split * p.n_tiles + tn) * 128 + t] = b;
+    }
 }
 
-// partial sums -> dW [N, K], db [N], over the splits in order
+// partial sums -> dW [N, K], db [N].  Four groups of threads take the splits s, s + 4, .. of the same 64 pieces, and their sums are added in order.
 template <int DT>
 __global__ __launch_bounds__(256) void nm_dense_sum_kernel(const float* __restrict__ part, const float* __restrict__ bias_part, int splits, int N, int K, int n_tiles,
                                                            int k_tiles, typename NmType<DT>::elem* __restrict__ dw, void* __restrict__ db, int db_f32) {
     typedef typename NmType<DT>::elem T;
-    const long long t = (long long)blockIdx.x * 256 + threadIdx.x;
-    const long long tiles = (long long)n_tiles * k_tiles;
-    if (t < tiles * 4096) {
-        const int tile = (int)(t >> 12), e4 = (int)(t & 4095);
-        const int wave = e4 >> 10, sub = (e4 >> 6) & 15, lane = e4 & 63, li = lane & 31, h = lane >> 5;
-        const int i = sub >> 3, j = (sub >> 2) & 1, rq = sub & 3;
-        // position of the matrix pipe -> group of eight columns and column of the group
-        const int gk = (tile % k_tiles) * 128 + 8 * (li & 15), k = nm_d_group(gk, K) + 2 * (2 * (wave >> 1) + j) + (li >> 4);
-        if (dw && k >= gk && k < K) {
-            float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
-            const float* src = part + t * 4;
-            for (int c = 0; c < splits; ++c) {
-                const float4 v = *reinterpret_cast<const float4*>(src + (long long)c * tiles * 16384);
-                s.x += v.x; s.y += v.y; s.z += v.z; s.w += v.w;
-            }
-#pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                const int pn = q + 8 * rq + 4 * h;
-                const int gn = (tile / k_tiles) * 128 + 8 * (pn & 15), n = nm_d_group(gn, N) + 2 * (2 * (wave & 1) + i) + (pn >> 4);
-                if (n >= gn && n < N) dw[(long long)n * K + k] = (T)(q == 0 ? s.x : q == 1 ? s.y : q == 2 ? s.z : s.w);
-            }
+    constexpr int CG = NmGroup<DT>::C;
+    __shared__ float4 sh[3][64];
+    const int g = threadIdx.x >> 6;
+    const long long t = (long long)blockIdx.x * 64 + (threadIdx.x & 63), tiles = (long long)n_tiles * k_tiles;
+    const bool in = t < tiles * 4096;
+    float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (dw && in) {
+        const float* src = part + t * 4;
+#pragma unroll 4
+        for (int c = g; c < splits; c += 4) {
+            const float4 v = *reinterpret_cast<const float4*>(src + (long long)c * tiles * 16384);
+            s.x += v.x; s.y += v.y; s.z += v.z; s.w += v.w;
         }
     }
-    if (db && t < N) {
-        const int gn = (int)t & ~7, e = (int)t - nm_d_group(gn, N);
-        float s = 0.f;
-        for (int c = 0; c < splits; ++c) s += bias_part[(long long)c * n_tiles * 128 + gn + e];
-        if (db_f32) ((float*)db)[t] = s;
-        else ((T*)db)[t] = (T)s;
+    if (g > 0) sh[g - 1][threadIdx.x & 63] = s;
+    __syncthreads();
+    if (g > 0) {
+        if (g == 1 && db && t < N) {
+            const int gn = (int)t / CG * CG, e = (int)t - nm_d_group<DT>(gn, N);
+            float b = 0.f;
+#pragma unroll 4
+            for (int c = 0; c < splits; ++c) b += bias_part[(long long)c * n_tiles * 128 + gn + e];
+            if (db_f32) ((float*)db)[t] = b;
+            else ((T*)db)[t] = (T)b;
+        }
+        return;
+    }
+    if (!dw || !in) return;
+#pragma unroll
+    for (int o = 0; o < 3; ++o) {
+        const float4 v = sh[o][threadIdx.x];
+        s.x += v.x; s.y += v.y; s.z += v.z; s.w += v.w;
+    }
+    const int tile = (int)(t >> 12), e4 = (int)(t & 4095);
+    const int wave = e4 >> 10, sub = (e4 >> 6) & 15, lane = e4 & 63, li = lane & 31, h = lane >> 5;
+    const int i = sub >> 3, j = (sub >> 2) & 1, rq = sub & 3;
+    int gr, e;
+    nm_d_place<DT>(2 * (wave >> 1) + j, li, gr, e);
+    const int gk = (tile % k_tiles) * 128 + gr * CG, k = nm_d_group<DT>(gk, K) + e;
+    if (k < gk || k >= K) return;
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+        nm_d_place<DT>(2 * (wave & 1) + i, q + 8 * rq + 4 * h, gr, e);
+        const int gn = (tile / k_tiles) * 128 + gr * CG, n = nm_d_group<DT>(gn, N) + e;
+        if (n >= gn && n < N) dw[(long long)n * K + k] = (T)(q == 0 ? s.x : q == 1 ? s.y : q == 2 ? s.z : s.w);
     }
 }
 
@@ -682,20 +966,28 @@ __global__ __launch_bounds__(256) void nm_dense_sum_kernel(const float* __restri
 static inline long long nm_d_up(long long a, long long b) { return (a + b - 1) / b; }
 static inline long long nm_d_align(long long b) { return nm_d_up(b, 256) * 256; }
 
-struct NmDensePlan { int nt, ps, tiles, col_blocks; long long steps, bytes_w, bytes; };
+struct NmDensePlan { bool resident; int np, tiles, col_blocks, rt; long long steps, bytes; };
 
-// columns C, contraction Q, rows R.  Panels: PS steps x NT tiles.
-static NmDensePlan nm_d_plan(int dt, long long R, long long C, long long Q) {
+// columns C, contraction Q, rows R: which kernel, and its column blocks of 32 np columns
+static NmDensePlan nm_d_plan(int dt, bool prod, bool res, long long R, long long C, long long Q) {
     NmDensePlan p;
-    p.nt = C > 128 ? 8 : C > 64 ? 4 : C > 32 ? 2 : 1;
-    const long long rb = nm_d_up(R, 128);
-    while (p.nt > 1 && rb * nm_d_up(C, 32 * p.nt) < 256) p.nt >>= 1;     // few rows: narrower column blocks until the chip is filled
-    p.ps = dt != NM_F32 ? (p.nt == 8 ? 2 : 4) : p.nt == 8 ? 1 : p.nt == 1 ? 4 : 2;
-    p.tiles = (int)(nm_d_up(C, 32 * p.nt) * p.nt);
-    p.col_blocks = p.tiles / p.nt;
-    p.steps = nm_d_up(nm_d_up(Q, 16), p.ps) * p.ps;
-    p.bytes_w = nm_d_align(p.steps * p.tiles * (dt == NM_F32 ? 3 : 1) * 1024);
-    p.bytes = p.bytes_w + nm_d_align(32LL * p.tiles * 4);
+    const int pieces = dt == NM_F32 ? 3 : 1;
+    const long long steps = nm_d_up(Q, 32);
+    p.np = C > 128 ? 8 : C > 64 ? 4 : C > 32 ? 2 : 1;
+    int fit = pieces == 3 && p.np == 8 ? 4 : p.np;           // (three pieces of sixteen tiles leave no registers)
+    if (res && fit == 8) fit = 4;                            // (the residual of eight pieces is in flight at once)
+    while (fit > 0 && 2 * steps * pieces * fit > NM_D_RESIDENT) fit >>= 1;
+    p.resident = fit > 0 && nm_d_up(C, 32 * fit) <= 4;
+    p.np = p.resident ? fit : p.np > 4 ? 4 : p.np;
+    // few rows: narrower column blocks until every wave has a tile (streaming: every CU a workgroup)
+    while (p.np > 1 && (p.resident ? nm_d_up(R, 32) * nm_d_up(C, 32 * p.np) < 1024 : nm_d_up(R, 128) * nm_d_up(C, 32 * p.np) < 256)) p.np >>= 1;
+    // streaming many rows: 64 rows per wave, so that a read of the weights serves twice the products
+    p.rt = !p.resident && p.np == 4 && dt != NM_F32 && !prod && nm_d_up(R, 256) * nm_d_up(C, 128) >= 256 ? 4 : 2;
+    const int ps = dt != NM_F32 || p.np == 1 ? 2 : 1;
+    p.tiles = (int)(nm_d_up(C, 32 * p.np) * p.np * 2);
+    p.col_blocks = p.tiles / (2 * p.np);
+    p.steps = p.resident ? steps : nm_d_up(steps, ps) * ps;
+    p.bytes = p.resident ? 0 : nm_d_align(p.steps * p.tiles * pieces * 1024);
     return p;
 }
 
@@ -705,7 +997,7 @@ static NmDenseGradPlan nm_d_grad_plan(long long M, long long N, long long K) {
     p.n_tiles = (int)nm_d_up(N > 0 ? N : 1, 128);
     p.k_tiles = (int)nm_d_up(K > 0 ? K : 1, 128);
     const long long tiles = (long long)p.n_tiles * p.k_tiles;
-    long long splits = nm_d_up(256, tiles);
+    long long splits = nm_d_up(512, tiles);                  // two workgroups per CU
     const long long most = nm_d_up(M, 256);
     if (splits > most) splits = most < 1 ? 1 : most;
     p.rows = nm_d_up(nm_d_up(M, splits), 64) * 64;
@@ -719,25 +1011,45 @@ template <int DT, bool PROD>
 static int nm_d_launch(const NmDensePlan& pl, NmDenseArgs a, hipStream_t stream) {
     a.tiles = pl.tiles;
     a.col_blocks = (unsigned)pl.col_blocks;
-    const long long groups = nm_d_up(nm_d_up(a.R, 128), 8) * 8 * pl.col_blocks;
+    constexpr bool F = DT == NM_F32;
+    if (pl.resident) {
+        // eight waves per workgroup, one tile of 32 rows each at least; one workgroup per CU
+        long long slots = nm_d_up(nm_d_up(nm_d_up(a.R, 32), 8), 8) * 8;
+        const long long most = 256 / pl.col_blocks / 8 * 8;
+        if (slots > most) slots = most;
+        const dim3 grid((unsigned)(slots * pl.col_blocks)), block(512);
+        switch (pl.np) {
+            case 8:
+                if constexpr (!F) hipLaunchKernelGGL((nm_dense_resident_kernel<DT, PROD, 8>), grid, block, 0, stream, a);
+                break;
+            case 4: hipLaunchKernelGGL((nm_dense_resident_kernel<DT, PROD, 4>), grid, block, 0, stream, a); break;
+            case 2: hipLaunchKernelGGL((nm_dense_resident_kernel<DT, PROD, 2>), grid, block, 0, stream, a); break;
+            default: hipLaunchKernelGGL((nm_dense_resident_kernel<DT, PROD, 1>), grid, block, 0, stream, a); break;
+        }
+        NM_LAUNCH_CHECK();
+        return 0;
+    }
+    const long long groups = nm_d_up(nm_d_up(a.R, 64 * pl.rt), 8) * 8 * pl.col_blocks;
     if (groups > 0x7fffffffLL) return nm_fail("nm_dense: %lld rows x %d columns exceed one launch", a.R, a.C);
     const dim3 grid((unsigned)groups), block(256);
-    constexpr bool F = DT == NM_F32;
-    switch (pl.nt) {
-        case 8: hipLaunchKernelGGL((nm_dense_kernel<DT, PROD, 1, 8, F ? 1 : 2>), grid, block, 0, stream, a); break;
-        case 4: hipLaunchKernelGGL((nm_dense_kernel<DT, PROD, 1, 4, F ? 2 : 4>), grid, block, 0, stream, a); break;
-        case 2: hipLaunchKernelGGL((nm_dense_kernel<DT, PROD, 1, 2, F ? 2 : 4>), grid, block, 0, stream, a); break;
-        default: hipLaunchKernelGGL((nm_dense_kernel<DT, PROD, 1, 1, 4>), grid, block, 0, stream, a); break;
+    if (pl.rt == 4) {
+        if constexpr (!F && !PROD) hipLaunchKernelGGL((nm_dense_stream_kernel<DT, PROD, 4, 4, 2>), grid, block, 0, stream, a);
+    } else {
+        switch (pl.np) {
+            case 4: hipLaunchKernelGGL((nm_dense_stream_kernel<DT, PROD, 2, 4, F ? 1 : 2>), grid, block, 0, stream, a); break;
+            case 2: hipLaunchKernelGGL((nm_dense_stream_kernel<DT, PROD, 2, 2, F ? 1 : 2>), grid, block, 0, stream, a); break;
+            default: hipLaunchKernelGGL((nm_dense_stream_kernel<DT, PROD, 2, 1, 2>), grid, block, 0, stream, a); break;
+        }
     }
     NM_LAUNCH_CHECK();
     return 0;
 }
 
 template <int DT>
-static int nm_d_pack(const NmDensePlan& pl, const void* w, long long ldw, int trans, int C, int Q, const void* bias, int bias_dt, char* ws, hipStream_t stream) {
-    const long long threads = pl.steps * pl.tiles * 64 > 32LL * pl.tiles ? pl.steps * pl.tiles * 64 : 32LL * pl.tiles;
-    hipLaunchKernelGGL((nm_dense_pack_kernel<DT>), dim3((unsigned)nm_d_up(threads, 256)), dim3(256), 0, stream, (const typename NmType<DT>::elem*)w, ldw, trans, C, Q,
-                       pl.tiles, (int)pl.steps, (uint4*)ws, bias, bias_dt == NM_F32, (float*)(ws + pl.bytes_w));
+static int nm_d_pack(const NmDensePlan& pl, const NmDenseArgs& a, char* ws, hipStream_t stream) {
+    if (pl.resident || pl.steps == 0) return 0;
+    hipLaunchKernelGGL((nm_dense_pack_kernel<DT>), dim3((unsigned)nm_d_up(pl.steps * pl.tiles * 64, 256)), dim3(256), 0, stream, (const typename NmType<DT>::elem*)a.W,
+                       a.ldw, a.trans, a.C, a.Q, pl.tiles, (int)pl.steps, (uint4*)ws);
     NM_LAUNCH_CHECK();
     return 0;
 }
@@ -760,11 +1072,11 @@ static int nm_d_forward(const void* x, long long ldx, const void* w, long long l
         NM_LAUNCH_CHECK();
         return 0;
     }
-    const NmDensePlan pl = nm_d_plan(DT, M, N, K);
-    if (nm_d_pack<DT>(pl, w, ldw, 0, N, K, bias, bias_dt, ws, stream)) return 1;
+    const NmDensePlan pl = nm_d_plan(DT, false, res != nullptr, M, N, K);
     NmDenseArgs a = {};
-    a.A = x; a.lda = ldx; a.W = (const uint4*)ws; a.bias = bias ? (const float*)(ws + pl.bytes_w) : nullptr;
+    a.A = x; a.lda = ldx; a.W = w; a.ldw = ldw; a.P = (const uint4*)ws; a.bias = bias; a.bias_f32 = bias_dt == NM_F32;
     a.res = res; a.ldr = ldr; a.Y = y; a.ldy = ldy; a.DV = deriv; a.R = M; a.Q = K; a.C = N; a.act = act; a.beta = beta;
+    if (nm_d_pack<DT>(pl, a, ws, stream)) return 1;
     return nm_d_launch<DT, false>(pl, a, stream);
 }
 
@@ -773,10 +1085,10 @@ static int nm_d_backward(const void* g, long long ldg, const void* deriv, const 
                          long long lddx, void* dw, void* db, int bias_dt, char* ws, hipStream_t stream) {
     typedef typename NmType<DT>::elem T;
     if (dx) {
-        const NmDensePlan pl = nm_d_plan(DT, M, K, N);
-        if (nm_d_pack<DT>(pl, w, ldw, 1, K, N, nullptr, NM_F32, ws, stream)) return 1;
+        const NmDensePlan pl = nm_d_plan(DT, deriv != nullptr, false, M, K, N);
         NmDenseArgs a = {};
-        a.A = g; a.lda = ldg; a.D = deriv; a.W = (const uint4*)ws; a.Y = dx; a.ldy = lddx; a.R = M; a.Q = N; a.C = K; a.act = NM_ACT_NONE; a.beta = 1.f;
+        a.A = g; a.lda = ldg; a.D = deriv; a.W = w; a.ldw = ldw; a.trans = 1; a.P = (const uint4*)ws; a.Y = dx; a.ldy = lddx; a.R = M; a.Q = N; a.C = K; a.act = NM_ACT_NONE; a.beta = 1.f;
+        if (nm_d_pack<DT>(pl, a, ws, stream)) return 1;
         if (deriv ? nm_d_launch<DT, true>(pl, a, stream) : nm_d_launch<DT, false>(pl, a, stream)) return 1;
         ws += pl.bytes;
     }
@@ -786,12 +1098,14 @@ static int nm_d_backward(const void* g, long long ldg, const void* deriv, const 
     a.G = g; a.ldg = ldg; a.D = deriv; a.X = x; a.ldx = ldx; a.R = M; a.N = N; a.K = dw ? K : 0; a.n_tiles = pl.n_tiles; a.k_tiles = pl.k_tiles; a.rows = pl.rows;
     a.part = (float*)ws; a.bias_part = db ? (float*)(ws + pl.bytes_part) : nullptr;
     const long long tiles = (long long)pl.n_tiles * pl.k_tiles;
-    if (tiles * pl.splits > 0x7fffffffLL) return nm_fail("nm_dense_backward: %d x %d weights exceed one launch", N, K);
-    const dim3 grid((unsigned)(tiles * pl.splits)), block(256);
+    const long long groups = tiles * nm_d_up(pl.splits, 8) * 8;
+    a.splits = pl.splits;
+    if (groups > 0x7fffffffLL) return nm_fail("nm_dense_backward: %d x %d weights exceed one launch", N, K);
+    const dim3 grid((unsigned)groups), block(256);
     if (deriv) hipLaunchKernelGGL((nm_dense_grad_kernel<DT, true>), grid, block, 0, stream, a);
     else hipLaunchKernelGGL((nm_dense_grad_kernel<DT, false>), grid, block, 0, stream, a);
-    const long long threads = tiles * 4096 > N ? tiles * 4096 : N;
-    hipLaunchKernelGGL((nm_dense_sum_kernel<DT>), dim3((unsigned)nm_d_up(threads, 256)), dim3(256), 0, stream, a.part, a.bias_part, pl.splits, N, a.K, pl.n_tiles,
+    const long long pieces = tiles * 4096 > N ? tiles * 4096 : N;
+    hipLaunchKernelGGL((nm_dense_sum_kernel<DT>), dim3((unsigned)nm_d_up(pieces, 64)), dim3(256), 0, stream, a.part, a.bias_part, pl.splits, N, a.K, pl.n_tiles,
                        pl.k_tiles, (T*)dw, db, bias_dt == NM_F32);
     NM_LAUNCH_CHECK();
     return 0;
@@ -809,10 +1123,14 @@ extern "C" {
 
 int64_t nm_dense_workspace_bytes(int64_t M, int64_t K, int64_t N, int dtype, int backward) {
     if (nm_d_check("nm_dense_workspace_bytes", M, K, N, dtype, dtype)) return -1;
-    if (!backward) return M <= NM_D_FEW ? 0 : nm_d_plan(dtype, M, N, K).bytes;
+    if (!backward) {
+        if (M <= NM_D_FEW) return 0;
+        const long long with = nm_d_plan(dtype, false, true, M, N, K).bytes, without = nm_d_plan(dtype, false, false, M, N, K).bytes;
+        return with > without ? with : without;
+    }
     // (the bias gradient alone is a plan of its own: one block of columns, more splits)
     const long long both = nm_d_grad_plan(M, N, K).bytes, bias = nm_d_grad_plan(M, N, 1).bytes;
-    return nm_d_plan(dtype, M, K, N).bytes + (both > bias ? both : bias);
+    return nm_d_plan(dtype, false, false, M, K, N).bytes + (both > bias ? both : bias);
 }
 
 int nm_dense_forward(const void* x, int64_t ldx, const void* weight, int64_t ldw, const void* bias, int bias_dtype, const void* residual, int64_t ldr, int64_t M,
@@ -824,6 +1142,7 @@ int nm_dense_forward(const void* x, int64_t ldx, const void* weight, int64_t ldw
     if (act == NM_ACT_SOFTPLUS && !(beta > 0.f)) return nm_fail("nm_dense_forward: softplus needs beta > 0");
     if (M == 0 || N == 0) return 0;
     if ((K > 0 && (!x || !weight)) || !y) return nm_fail("nm_dense_forward: NULL argument");
+    if (ldx > NM_D_MAX_LD || ldw > NM_D_MAX_LD || ldy > NM_D_MAX_LD || ldr > NM_D_MAX_LD) return nm_fail("nm_dense_forward: row stride beyond 2^24");
     if (ldx < K || ldw < K || ldy < N || (residual && ldr < N)) return nm_fail("nm_dense_forward: row stride shorter than a row");
     if (workspace_bytes < nm_dense_workspace_bytes(M, K, N, dtype, 0)) return nm_fail("nm_dense_forward: workspace too small");
     if (workspace_bytes > 0 && !workspace) return nm_fail("nm_dense_forward: NULL workspace");
@@ -844,6 +1163,7 @@ int nm_dense_backward(const void* g, int64_t ldg, const void* deriv, const void*
     if (M == 0) dx = nullptr;
     if (!dx && !dweight && !dbias) return 0;
     if ((M > 0 && N > 0 && !g) || (dx && N > 0 && !weight) || (dweight && M > 0 && !x)) return nm_fail("nm_dense_backward: NULL argument");
+    if (ldg > NM_D_MAX_LD || ldx > NM_D_MAX_LD || ldw > NM_D_MAX_LD || lddx > NM_D_MAX_LD) return nm_fail("nm_dense_backward: row stride beyond 2^24");
     if (ldg < N || (dx && (ldw < K || lddx < K)) || (dweight && ldx < K)) return nm_fail("nm_dense_backward: row stride shorter than a row");
     if (!workspace || workspace_bytes < nm_dense_workspace_bytes(M, K, N, dtype, 1)) return nm_fail("nm_dense_backward: workspace too small");
     const int k = (int)K, n = (int)N;

@@ -7,12 +7,18 @@
 
 typedef __bf16 nm_v8b __attribute__((ext_vector_type(8)));
 typedef _Float16 nm_v8h __attribute__((ext_vector_type(8)));
+typedef float nm_v4f __attribute__((ext_vector_type(4)));
 typedef float nm_v16f __attribute__((ext_vector_type(16)));
 
 template <int DT> struct NmType;
 template <> struct NmType<NM_F32> { typedef float elem; };
 template <> struct NmType<NM_F16> { typedef _Float16 elem; };
 template <> struct NmType<NM_BF16> { typedef __bf16 elem; };
+
+template <int DT>
+__device__ __forceinline__ float nm_to_float(typename NmType<DT>::elem e) { return (float)e; }
+template <int DT>
+__device__ __forceinline__ typename NmType<DT>::elem nm_from_float(float f) { return (typename NmType<DT>::elem)f; }
 
 static inline bool nm_dtype_ok(int dt) { return dt == NM_F32 || dt == NM_F16 || dt == NM_BF16; }
 static inline int nm_dtype_size(int dt) { return dt == NM_F32 ? 4 : 2; }
@@ -108,14 +114,14 @@ __device__ __forceinline__ void nm_oct_to_float(const NmOct<DT>& o, float (&f)[8
     typename NmType<DT>::elem e[8];
     __builtin_memcpy(e, &o, sizeof(o));
 #pragma unroll
-    for (int i = 0; i < 8; ++i) f[i] = (float)e[i];
+    for (int i = 0; i < 8; ++i) f[i] = nm_to_float<DT>(e[i]);
 }
 // the first `n` of eight values, rounded once to the element type
 template <int DT>
 __device__ __forceinline__ void nm_oct_store_n(typename NmType<DT>::elem* p, const float (&f)[8], long long n) {
     typename NmType<DT>::elem e[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) e[i] = (typename NmType<DT>::elem)f[i];
+    for (int i = 0; i < 8; ++i) e[i] = nm_from_float<DT>(f[i]);
     if (n >= 8) {
         __builtin_memcpy(p, e, sizeof(e));
         return;

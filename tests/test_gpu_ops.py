@@ -69,7 +69,8 @@ def dense_reference(x, w, b, r, act, beta, g=None):
         return y, by
     g = g.double().cpu()
     dz = g * d
-    keep = 2.0 ** -24 if t == torch.float32 else half_step(torch.float16)     # act' is kept in fp32 / fp16: one rounding, 2^-11 (not 2^-12: 11 significant bits)
+    # act' is kept with 24 significant bits beside fp32 rows, 12 beside fp16 and 11 beside bf16 rows: half a step is
+    keep = {torch.float32: 2.0 ** -24, torch.float16: 2.0 ** -12, torch.bfloat16: 2.0 ** -11}[t]
     edz = g.abs() * (curve * ez + (keep + 4e-6) * d.abs() + 2.0 ** -24) + 2.0 ** -15 * dz.abs() * (t != torch.float32) + 2 * U * dz.abs() + tiny(t)
     extra = 2.0 ** -21 if t == torch.float32 else 0.0
 

@@ -49,8 +49,9 @@ def test_c_entries_refuse(dtype):
 
     def fwd(x=p, ldx=8, w=p, ldw=8, bdt=dtype, r=None, ldr=0, M=20, K=8, N=4, dt=dtype, act=0, beta=1.0, y=p, ldy=4, ws=p, n=1 << 30):
         return lib.nm_dense_forward(x, ldx, w, ldw, None, bdt, r, ldr, M, K, N, dt, act, beta, y, ldy, None, ws, n, None)
-    for bad in (dict(dt=3), dict(bdt=7), dict(act=6), dict(act=-1), dict(act=2, beta=0.0), dict(x=None), dict(w=None), dict(y=None), dict(ldx=7), dict(ldw=7), dict(ldy=3),
-                dict(r=p, ldr=3), dict(M=-1), dict(K=-1), dict(N=-1), dict(K=(1 << 20) + 1, ldx=1 << 21, ldw=1 << 21), dict(n=16), dict(n=-1), dict(ws=None)):
+    for bad in (dict(dt=3), dict(bdt=7), dict(act=6), dict(act=-1), dict(act=2, beta=0.0), dict(x=None), dict(w=None), dict(y=None), dict(ldx=7), dict(ldw=7), dict(ldy=3), dict(ldx=(1 << 24) + 1),
+                dict(r=p, ldr=3), dict(M=-1), dict(K=-1), dict(N=-1), dict(K=(1 << 20) + 1, ldx=1 << 21, ldw=1 << 21), dict(K=4096, ldx=4096, ldw=4096, N=700, ldy=700, n=16),
+                dict(K=4096, ldx=4096, ldw=4096, N=700, ldy=700, n=-1), dict(K=4096, ldx=4096, ldw=4096, N=700, ldy=700, ws=None)):
         assert fwd(**bad) == 1 and lib.nm_last_error(), bad
     assert fwd(M=0, x=None, y=None) == 0 and fwd(N=0, y=None) == 0
 
