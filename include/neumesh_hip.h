@@ -426,9 +426,9 @@ int nm_dense_backward(const void* g, int64_t ldg, const void* deriv, const void*
  * keep (NULL = no backward pass will follow): nm_scan_keep_elems() floats that nm_scan_backward reads back.
  * nm_scan_backward: cotangents g_states [L,D] of x's type and g_last [S,D] fp32 (NULL = 0) -> dgate, dx, dh0 in the types and shapes of gate, x, h0
  * (NULL = not wanted; overwritten).  The results do not change from run to run.
- * workspace: nm_scan_workspace_bytes(.., packed = cu_seqlens != NULL, backward) bytes, 16-byte aligned, of this call until its stream work is done. */
-int64_t nm_scan_workspace_bytes(int64_t L, int64_t S, int64_t D, int dtype, int packed, int backward);
-int64_t nm_scan_keep_elems(int64_t L, int64_t S, int64_t D, int dtype, int packed);
+ * workspace (either direction): nm_scan_workspace_bytes(.., packed = cu_seqlens != NULL) bytes, 16-byte aligned, of this call until its stream work is done. */
+int64_t nm_scan_workspace_bytes(int64_t L, int64_t S, int64_t D, int dtype, int shared_gate, int packed);
+int64_t nm_scan_keep_elems(int64_t L, int64_t S, int64_t D, int dtype, int shared_gate, int packed);
 int nm_scan_forward(const void* gate, int gate_dtype, int shared_gate, const void* x, int dtype, const float* h0, const int32_t* cu_seqlens,
                     int64_t L, int64_t S, int64_t D, int reverse, int blend, void* states, float* last, float* keep,
                     void* workspace, int64_t workspace_bytes, nm_stream_t stream);

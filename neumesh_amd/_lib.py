@@ -131,7 +131,7 @@ SIGNATURES = {
     "nm_dense_backward": (C.c_int, [_P, C.c_int64, _P, _P, C.c_int64, _P, C.c_int64, C.c_int64, C.c_int64, C.c_int64, C.c_int, _P, C.c_int64, _P, _P, C.c_int,
                                     _P, C.c_int64, _P]),
     "nm_scan_workspace_bytes": (C.c_int64, [C.c_int64, C.c_int64, C.c_int64, C.c_int, C.c_int, C.c_int]),
-    "nm_scan_keep_elems": (C.c_int64, [C.c_int64, C.c_int64, C.c_int64, C.c_int, C.c_int]),
+    "nm_scan_keep_elems": (C.c_int64, [C.c_int64, C.c_int64, C.c_int64, C.c_int, C.c_int, C.c_int]),
     "nm_scan_forward": (C.c_int, [_P, C.c_int, C.c_int, _P, C.c_int, _P, _P, C.c_int64, C.c_int64, C.c_int64, C.c_int, C.c_int, _P, _P, _P, _P, C.c_int64, _P]),
     "nm_scan_backward": (C.c_int, [_P, C.c_int, C.c_int, _P, C.c_int, _P, _P, C.c_int64, C.c_int64, C.c_int64, C.c_int, C.c_int, _P, _P, _P, _P, _P, _P,
                                    _P, C.c_int64, _P]),

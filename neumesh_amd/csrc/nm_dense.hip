@@ -714,8 +714,9 @@ struct NmDenseGradArgs {
     long long R;
     int N, K, n_tiles, k_tiles, splits;
     long long rows;                      // rows per workgroup (a multiple of 64)
-    float* part;                         // [splits][n_tiles * k_tiles][16384] in the order of the accumulators
-    float* bias_part;                    // [splits][128 n_tiles] or NULL
+    float* part;                         // [splits][n_tiles * k_tiles][16384] in the order of the accumulators; one split: NULL, straight to
+    void* dw; void* db; int db_f32;      // dW [N, K] (or NULL) and db [N] (or NULL)
+    float* bias_part;                    // [splits][128 n_tiles], or NULL: db is not wanted, or one split
 };
 
 template <int DT> struct NmGroup { static constexpr int C = DT == NM_F32 ? 2 : 4; };    // columns of a thread: 8 bytes
@@ -786,6 +787,22 @@ __device__ __forceinline__ uint4 nm_d_column16(const uint2 (&r)[8], int e) {
                       __builtin_amdgcn_perm(w[7], w[6], sel));
 }
 
+// four values of a lane's accumulators (rows 8 rq + 4 (lane / 32) .. of tile `ti`, position lane % 32 of tile `tj`) -> dW
+template <int DT>
+__device__ __forceinline__ void nm_d_put_grad(typename NmType<DT>::elem* dw, int N, int K, int tn, int tk, int ti, int tj, int lane, int rq, const float4& s) {
+    constexpr int CG = NmGroup<DT>::C;
+    int gr, e;
+    nm_d_place<DT>(tj, lane & 31, gr, e);
+    const int gk = tk * 128 + gr * CG, k = nm_d_group<DT>(gk, K) + e;
+    if (k < gk || k >= K) return;
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+        nm_d_place<DT>(ti, q + 8 * rq + 4 * (lane >> 5), gr, e);
+        const int gn = tn * 128 + gr * CG, n = nm_d_group<DT>(gn, N) + e;
+        if (n >= gn && n < N) dw[(long long)n * K + k] = (typename NmType<DT>::elem)(q == 0 ? s.x : q == 1 ? s.y : q == 2 ? s.z : s.w);
+    }
+}
+
 template <int DT, bool PROD>
 __global__ __launch_bounds__(256, 2) void nm_dense_grad_kernel(NmDenseGradArgs p) {
     typedef typename NmType<DT>::elem T;
@@ -804,7 +821,7 @@ __global__ __launch_bounds__(256, 2) void nm_dense_grad_kernel(NmDenseGradArgs p
     const long long r0 = (long long)split * p.rows, r1 = r0 + p.rows < p.R ? r0 + p.rows : p.R;
     const int cg = t % LANES, rg = t / LANES;                // group of columns, group of eight rows
     const int coln = nm_d_group<DT>(tn * 128 + cg * CG, p.N), colk = nm_d_group<DT>(tk * 128 + cg * CG, p.K);
-    const bool want_bias = p.bias_part && tk == 0;
+    const bool want_bias = (p.bias_part || p.db) && tk == 0;
     float bsum[CG];
 #pragma unroll
     for (int e = 0; e < CG; ++e) bsum[e] = 0.f;
@@ -887,15 +904,26 @@ __global__ __launch_bounds__(256, 2) void nm_dense_grad_kernel(NmDenseGradArgs p
         }
         __syncthreads();
     }
-    float* out = p.part + ((long long)split * (p.n_tiles * p.k_tiles) + tile) * 16384 + wave * 4096;
+    if (p.part) {
+        float* out = p.part + ((long long)split * (p.n_tiles * p.k_tiles) + tile) * 16384 + wave * 4096;
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
+        for (int i = 0; i < 2; ++i)
 #pragma unroll
-        for (int j = 0; j < 2; ++j)
+            for (int j = 0; j < 2; ++j)
 #pragma unroll
-            for (int r = 0; r < 16; r += 4)
-                *reinterpret_cast<float4*>(out + ((i * 2 + j) * 4 + (r >> 2)) * 256 + lane * 4) =
-                    make_float4(acc[i][j][r], acc[i][j][r + 1], acc[i][j][r + 2], acc[i][j][r + 3]);
+                for (int r = 0; r < 16; r += 4)
+                    *reinterpret_cast<float4*>(out + ((i * 2 + j) * 4 + (r >> 2)) * 256 + lane * 4) =
+                        make_float4(acc[i][j][r], acc[i][j][r + 1], acc[i][j][r + 2], acc[i][j][r + 3]);
+    } else if (p.dw) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+#pragma unroll
+                for (int r = 0; r < 16; r += 4)
+                    nm_d_put_grad<DT>((T*)p.dw, p.N, p.K, tn, tk, 2 * wn + i, 2 * wk + j, lane, r >> 2,
+                                      make_float4(acc[i][j][r], acc[i][j][r + 1], acc[i][j][r + 2], acc[i][j][r + 3]));
+    }
     if (!want_bias) return;                                  // (uniform over the workgroup)
     float* sh = reinterpret_cast<float*>(lds);               // [row group][128]
 #pragma unroll
@@ -905,7 +933,15 @@ __global__ __launch_bounds__(256, 2) void nm_dense_grad_kernel(NmDenseGradArgs p
         float b = 0.f;
 #pragma unroll
         for (int g = 0; g < ROWS / 8; ++g) b += sh[g * 128 + t];
-        p.bias_part[((long long)split * p.n_tiles + tn) * 128 + t] = b;
+        if (p.bias_part) {
+            p.bias_part[((long long)split * p.n_tiles + tn) * 128 + t] = b;
+        } else {
+            const int gn = tn * 128 + t / CG * CG, n = nm_d_group<DT>(gn, p.N) + t % CG;
+            if (n >= gn && n < p.N) {
+                if (p.db_f32) ((float*)p.db)[n] = b;
+                else ((T*)p.db)[n] = (T)b;
+            }
+        }
     }
 }
 
@@ -947,19 +983,8 @@ __global__ __launch_bounds__(256) void nm_dense_sum_kernel(const float* __restri
         const float4 v = sh[o][threadIdx.x];
         s.x += v.x; s.y += v.y; s.z += v.z; s.w += v.w;
     }
-    const int tile = (int)(t >> 12), e4 = (int)(t & 4095);
-    const int wave = e4 >> 10, sub = (e4 >> 6) & 15, lane = e4 & 63, li = lane & 31, h = lane >> 5;
-    const int i = sub >> 3, j = (sub >> 2) & 1, rq = sub & 3;
-    int gr, e;
-    nm_d_place<DT>(2 * (wave >> 1) + j, li, gr, e);
-    const int gk = (tile % k_tiles) * 128 + gr * CG, k = nm_d_group<DT>(gk, K) + e;
-    if (k < gk || k >= K) return;
-#pragma unroll
-    for (int q = 0; q < 4; ++q) {
-        nm_d_place<DT>(2 * (wave & 1) + i, q + 8 * rq + 4 * h, gr, e);
-        const int gn = (tile / k_tiles) * 128 + gr * CG, n = nm_d_group<DT>(gn, N) + e;
-        if (n >= gn && n < N) dw[(long long)n * K + k] = (T)(q == 0 ? s.x : q == 1 ? s.y : q == 2 ? s.z : s.w);
-    }
+    const int tile = (int)(t >> 12), e4 = (int)(t & 4095), wave = e4 >> 10, sub = (e4 >> 6) & 15;
+    nm_d_put_grad<DT>(dw, N, K, tile / k_tiles, tile % k_tiles, 2 * (wave & 1) + (sub >> 3), 2 * (wave >> 1) + ((sub >> 2) & 1), e4 & 63, sub & 3, s);
 }
 
 // ------------------------------------------------------------------------------------------------ launch plans
@@ -1002,8 +1027,8 @@ static NmDenseGradPlan nm_d_grad_plan(long long M, long long N, long long K) {
     if (splits > most) splits = most < 1 ? 1 : most;
     p.rows = nm_d_up(nm_d_up(M, splits), 64) * 64;
     p.splits = (int)(M > 0 ? nm_d_up(M, p.rows) : 1);
-    p.bytes_part = nm_d_align((long long)p.splits * tiles * 16384 * 4);
-    p.bytes = p.bytes_part + nm_d_align((long long)p.splits * p.n_tiles * 128 * 4);
+    p.bytes_part = p.splits > 1 ? nm_d_align((long long)p.splits * tiles * 16384 * 4) : 0;
+    p.bytes = p.splits > 1 ? p.bytes_part + nm_d_align((long long)p.splits * p.n_tiles * 128 * 4) : 0;
     return p;
 }
 
@@ -1096,7 +1121,12 @@ static int nm_d_backward(const void* g, long long ldg, const void* deriv, const 
     const NmDenseGradPlan pl = nm_d_grad_plan(M, N, dw ? K : 1);      // (db alone: no columns of x)
     NmDenseGradArgs a = {};
     a.G = g; a.ldg = ldg; a.D = deriv; a.X = x; a.ldx = ldx; a.R = M; a.N = N; a.K = dw ? K : 0; a.n_tiles = pl.n_tiles; a.k_tiles = pl.k_tiles; a.rows = pl.rows;
-    a.part = (float*)ws; a.bias_part = db ? (float*)(ws + pl.bytes_part) : nullptr;
+    if (pl.splits > 1) {
+        a.part = (float*)ws;
+        a.bias_part = db ? (float*)(ws + pl.bytes_part) : nullptr;
+    } else {
+        a.dw = dw; a.db = db; a.db_f32 = bias_dt == NM_F32;
+    }
     const long long tiles = (long long)pl.n_tiles * pl.k_tiles;
     const long long groups = tiles * nm_d_up(pl.splits, 8) * 8;
     a.splits = pl.splits;
@@ -1104,6 +1134,10 @@ static int nm_d_backward(const void* g, long long ldg, const void* deriv, const 
     const dim3 grid((unsigned)groups), block(256);
     if (deriv) hipLaunchKernelGGL((nm_dense_grad_kernel<DT, true>), grid, block, 0, stream, a);
     else hipLaunchKernelGGL((nm_dense_grad_kernel<DT, false>), grid, block, 0, stream, a);
+    if (pl.splits == 1) {
+        NM_LAUNCH_CHECK();
+        return 0;
+    }
     const long long pieces = tiles * 4096 > N ? tiles * 4096 : N;
     hipLaunchKernelGGL((nm_dense_sum_kernel<DT>), dim3((unsigned)nm_d_up(pieces, 64)), dim3(256), 0, stream, a.part, a.bias_part, pl.splits, N, a.K, pl.n_tiles,
                        pl.k_tiles, (T*)dw, db, bias_dt == NM_F32);
@@ -1165,7 +1199,7 @@ int nm_dense_backward(const void* g, int64_t ldg, const void* deriv, const void*
     if ((M > 0 && N > 0 && !g) || (dx && N > 0 && !weight) || (dweight && M > 0 && !x)) return nm_fail("nm_dense_backward: NULL argument");
     if (ldg > NM_D_MAX_LD || ldx > NM_D_MAX_LD || ldw > NM_D_MAX_LD || lddx > NM_D_MAX_LD) return nm_fail("nm_dense_backward: row stride beyond 2^24");
     if (ldg < N || (dx && (ldw < K || lddx < K)) || (dweight && ldx < K)) return nm_fail("nm_dense_backward: row stride shorter than a row");
-    if (!workspace || workspace_bytes < nm_dense_workspace_bytes(M, K, N, dtype, 1)) return nm_fail("nm_dense_backward: workspace too small");
+    if (workspace_bytes < nm_dense_workspace_bytes(M, K, N, dtype, 1) || (workspace_bytes > 0 && !workspace)) return nm_fail("nm_dense_backward: workspace too small");
     const int k = (int)K, n = (int)N;
     char* ws = (char*)workspace;
     if (dtype == NM_F32) return nm_d_backward<NM_F32>(g, ldg, deriv, x, ldx, weight, ldw, M, k, n, dx, lddx, dweight, dbias, bias_dtype, ws, stream);

@@ -29,10 +29,11 @@ struct NmScanArgs {
     const int* cu;                       // packed: [S + 1]
     long long L, S, chunk;               // chunk: steps of one workgroup
     unsigned T;
-    int D, reverse, blend, cl_log2, blocks, map_only;
+    int D, reverse, blend, cl_log2, blocks;
     void* states;                        // [L, D] or NULL
     float* last;                         // [S, D]
-    float* keep;                         // states at the tile starts, [chunks][tiles per chunk][D], or NULL
+    float* keep; int keep_steps;         // states before every keep_steps-th step, [chunks][pieces][D] counted from a range's start, or (keep_seq)
+    int keep_seq;                        // [S][pieces][D] from a sequence's start, in the order of the recurrence; or NULL
     float* map_a; float* map_h; int* map_f;     // [chunks, D] x 2, [chunks]
     const float* carry;                  // [chunks, D] or NULL
     // backward
@@ -58,106 +59,310 @@ __device__ __forceinline__ void nm_s_store(typename NmType<DT>::elem* p, const f
     __builtin_memcpy(p, &v, sizeof(v));
 }
 
-// the affine map h -> A h + H of a stretch of steps; F: it starts anew, whatever came before
-template <int VEC> struct NmMap { float a[VEC], h[VEC]; int f; };
-
-// `m` applied after the state `s`
-template <int VEC>
-__device__ __forceinline__ void nm_s_apply(const NmMap<VEC>& m, float (&s)[VEC]) {
+// Where a thread's steps lie: step s is row `row` + `lane` + s, or - s.  `row` is uniform over the workgroup and `lane` within the tile, so that an address is
+// a scalar base and a 32-bit offset (tile x D elements stay below 2^30).
+struct NmPlace {
+    long long row;
+    unsigned lane;
+    int reverse;
+};
+template <typename T> struct NmRow {
+    char* base; long long stride; unsigned off;
+    __device__ __forceinline__ T* at(int s) const { return (T*)(base + s * stride + (size_t)off); }
+};
+template <typename T>
+__device__ __forceinline__ NmRow<T> nm_s_rows(T* base, const NmPlace& w, int D, unsigned ch) {
+    return {(char*)(base + w.row * D), (w.reverse ? -1LL : 1LL) * D * (long long)sizeof(T), (w.lane * (unsigned)D + ch) * (unsigned)sizeof(T)};
+}
+// A thread's n <= SEG consecutive steps of VEC channels, a vector per row.
+template <int DT, int VEC, int SEG>
+__device__ __forceinline__ void nm_s_load_steps(const typename NmType<DT>::elem* base, const NmPlace& w, int D, int ch, int n, NmVec<DT, VEC> (&v)[SEG]) {
+    const NmRow<const typename NmType<DT>::elem> r = nm_s_rows(base, w, D, ch);
+    if (n == SEG) {
 #pragma unroll
-    for (int k = 0; k < VEC; ++k) s[k] = m.f ? m.h[k] : fmaf(m.a[k], s[k], m.h[k]);
+        for (int s = 0; s < SEG; ++s) v[s] = nm_s_load<DT, VEC>(r.at(s));
+    } else {
+#pragma unroll
+        for (int s = 0; s < SEG; ++s) {
+            v[s] = {};
+            if (s < n) v[s] = nm_s_load<DT, VEC>(r.at(s));
+        }
+    }
+}
+// The same where a row has exactly VEC elements, so that the steps are one stretch of memory: read as such, in descending order if the recurrence runs
+// backwards.
+template <int DT, int VEC, int SEG>
+__device__ __forceinline__ void nm_s_load_whole(const typename NmType<DT>::elem* base, const NmPlace& at, int n, NmVec<DT, VEC> (&v)[SEG]) {
+    if (n < SEG) {
+        nm_s_load_steps<DT, VEC, SEG>(base, at, VEC, 0, n, v);
+        return;
+    }
+    NmVec<DT, VEC * SEG> w;
+    __builtin_memcpy(&w, nm_s_rows(base, at, VEC, 0).at(at.reverse ? SEG - 1 : 0), sizeof(w));
+    if (at.reverse) {                    // (uniform)
+#pragma unroll
+        for (int s = 0; s < SEG; ++s)
+#pragma unroll
+            for (int k = 0; k < VEC; ++k) v[s].e[k] = w.e[(SEG - 1 - s) * VEC + k];
+    } else {
+#pragma unroll
+        for (int s = 0; s < SEG; ++s)
+#pragma unroll
+            for (int k = 0; k < VEC; ++k) v[s].e[k] = w.e[s * VEC + k];
+    }
+}
+// ... by the whole workgroup: a tile of 256 SEG steps from step b on is one stretch of memory, read in 16-byte pieces side by side and dealt out through
+// LDS (PIECES per thread, at an odd stride from three on: four workgroups per CU).  Pieces beyond the array's ends are left out; what lies beyond the workgroup's range is not used.
+template <int DT, int VEC, int SEG> struct NmStage {
+    static constexpr int PIECES = SEG * VEC * (int)sizeof(typename NmType<DT>::elem) / 16, STRIDE = PIECES < 3 ? PIECES : PIECES | 1;
+    static_assert(SEG * VEC * sizeof(typename NmType<DT>::elem) % 16 == 0, "whole pieces per thread");
+};
+template <int DT, int VEC, int SEG>
+__device__ __forceinline__ void nm_s_stage(const typename NmType<DT>::elem* base, long long b, long long L, int reverse, uint4* lds, int t) {
+    typedef typename NmType<DT>::elem T;
+    typedef NmStage<DT, VEC, SEG> G;
+    constexpr int E = 16 / (int)sizeof(T);
+    const long long first = (reverse ? L - b - 256LL * SEG : b) * VEC, end = L * VEC;      // element of memory that piece 0 starts with
+#pragma unroll
+    for (int i = 0; i < G::PIECES; ++i) {
+        const int j = t + 256 * i;
+        const long long e0 = first + (long long)j * E;
+        uint4 v = make_uint4(0, 0, 0, 0);
+        if (e0 >= 0 && e0 + E <= end) {
+            __builtin_memcpy(&v, base + e0, 16);
+        } else if (e0 > -E && e0 < end) {
+            T x[E];
+#pragma unroll
+            for (int k = 0; k < E; ++k) x[k] = e0 + k >= 0 && e0 + k < end ? base[e0 + k] : (T)0.f;
+            __builtin_memcpy(&v, x, 16);
+        }
+        lds[j / G::PIECES * G::STRIDE + j % G::PIECES] = v;
+    }
+}
+template <int DT, int VEC, int SEG>
+__device__ __forceinline__ void nm_s_unstage(const uint4* lds, int reverse, int t, NmVec<DT, VEC> (&v)[SEG]) {
+    typedef NmStage<DT, VEC, SEG> G;
+    NmVec<DT, VEC * SEG> w;
+    __builtin_memcpy(&w, lds + (reverse ? 255 - t : t) * G::STRIDE, sizeof(w));
+    if (reverse) {                       // (uniform)
+#pragma unroll
+        for (int s = 0; s < SEG; ++s)
+#pragma unroll
+            for (int k = 0; k < VEC; ++k) v[s].e[k] = w.e[(SEG - 1 - s) * VEC + k];
+    } else {
+#pragma unroll
+        for (int s = 0; s < SEG; ++s)
+#pragma unroll
+            for (int k = 0; k < VEC; ++k) v[s].e[k] = w.e[s * VEC + k];
+    }
+}
+template <int DT, int VEC, int SEG>
+__device__ __forceinline__ void nm_s_store_whole(typename NmType<DT>::elem* base, const NmPlace& at, int n, const float (&f)[SEG][VEC]) {
+    typedef typename NmType<DT>::elem T;
+    if (n == SEG) {
+        NmVec<DT, VEC * SEG> w;
+#pragma unroll
+        for (int s = 0; s < SEG; ++s)
+#pragma unroll
+            for (int k = 0; k < VEC; ++k) w.e[s * VEC + k] = (T)(at.reverse ? f[SEG - 1 - s][k] : f[s][k]);
+        __builtin_memcpy(nm_s_rows(base, at, VEC, 0).at(at.reverse ? SEG - 1 : 0), &w, sizeof(w));
+    } else {
+#pragma unroll
+        for (int s = 0; s < SEG; ++s)
+            if (s < n) nm_s_store<DT, VEC>(nm_s_rows(base, at, VEC, 0).at(s), f[s]);
+    }
+}
+
+// the affine map h -> A h + H of a stretch of steps; F: it starts anew, whatever came before.  AV: a shared gate's factor is one for all channels.
+template <int VEC, int AV> struct NmMap { float a[AV], h[VEC]; int f; };
+
+template <int VEC, int AV>
+__device__ __forceinline__ void nm_s_identity(NmMap<VEC, AV>& m) {
+#pragma unroll
+    for (int k = 0; k < AV; ++k) m.a[k] = 1.f;
+#pragma unroll
+    for (int k = 0; k < VEC; ++k) m.h[k] = 0.f;
+    m.f = 0;
+}
+// `m` applied after the state `s`
+template <int VEC, int AV>
+__device__ __forceinline__ void nm_s_apply(const NmMap<VEC, AV>& m, float (&s)[VEC]) {
+#pragma unroll
+    for (int k = 0; k < VEC; ++k) s[k] = m.f ? m.h[k] : fmaf(m.a[AV == 1 ? 0 : k], s[k], m.h[k]);
+}
+// the map `m` followed by `n`, in m
+template <int VEC, int AV>
+__device__ __forceinline__ void nm_s_then(NmMap<VEC, AV>& m, const NmMap<VEC, AV>& n) {
+    nm_s_apply(n, m.h);
+#pragma unroll
+    for (int k = 0; k < AV; ++k) m.a[k] = n.f ? 0.f : m.a[k] * n.a[k];
+    m.f |= n.f;
+}
+template <int VEC, int AV>
+__device__ __forceinline__ void nm_s_from_lane(const NmMap<VEC, AV>& m, int src, NmMap<VEC, AV>& p) {
+    p.f = __shfl(m.f, src);
+#pragma unroll
+    for (int k = 0; k < AV; ++k) p.a[k] = __shfl(m.a[k], src);
+#pragma unroll
+    for (int k = 0; k < VEC; ++k) p.h[k] = __shfl(m.h[k], src);
 }
 
 // exclusive scan of the lanes' maps in time order within a wave (DIR = 1: lower lanes come first, -1: higher lanes); the wave's total is left in the
 // last lane's `m`.  Lanes of one time are neighbours: exchanges go over multiples of cl.
-template <int VEC, int DIR>
-__device__ __forceinline__ void nm_s_wave_scan(NmMap<VEC>& m, NmMap<VEC>& before, int lane, int cl) {
+template <int VEC, int AV, int DIR>
+__device__ __forceinline__ void nm_s_wave_scan(NmMap<VEC, AV>& m, NmMap<VEC, AV>& before, int lane, int cl) {
     for (int o = cl; o < 64; o <<= 1) {
-        NmMap<VEC> p;
+        NmMap<VEC, AV> p;
         const int src = lane - DIR * o;
-        const bool has = src >= 0 && src < 64;
-        p.f = __shfl(m.f, src & 63);
+        nm_s_from_lane(m, src & 63, p);
+        if (src >= 0 && src < 64 && !m.f) {                  // p followed by m
 #pragma unroll
-        for (int k = 0; k < VEC; ++k) {
-            p.a[k] = __shfl(m.a[k], src & 63);
-            p.h[k] = __shfl(m.h[k], src & 63);
-        }
-        if (has && !m.f) {
+            for (int k = 0; k < VEC; ++k) m.h[k] = fmaf(m.a[AV == 1 ? 0 : k], p.h[k], m.h[k]);
 #pragma unroll
-            for (int k = 0; k < VEC; ++k) {
-                m.h[k] = fmaf(m.a[k], p.h[k], m.h[k]);
-                m.a[k] *= p.a[k];
-            }
+            for (int k = 0; k < AV; ++k) m.a[k] *= p.a[k];
             m.f = p.f;
         }
     }
     const int src = lane - DIR * cl;
-    const bool has = src >= 0 && src < 64;
-    before.f = __shfl(m.f, src & 63);
-#pragma unroll
-    for (int k = 0; k < VEC; ++k) {
-        before.a[k] = __shfl(m.a[k], src & 63);
-        before.h[k] = __shfl(m.h[k], src & 63);
-        if (!has) { before.a[k] = 1.f; before.h[k] = 0.f; }
-    }
-    if (!has) before.f = 0;
+    nm_s_from_lane(m, src & 63, before);
+    if (src < 0 || src >= 64) nm_s_identity(before);
 }
 
-// which sequence the thread's steps belong to: index (-1: none), bit s of first / final: the step is its sequence's first / last
-template <int SEG> struct NmSteps { int seq[SEG]; unsigned first, final; int n; };
+// the maps of the four waves, per channel lane
+// (fewer than four channels: one lane holds a whole row)
+template <int VEC, int AV> struct NmShared { float a[4][(VEC < 4 ? 1 : 64) * AV], h[4][(VEC < 4 ? 1 : 64) * VEC]; int f[4]; };
+
+template <int VEC, int AV>
+__device__ __forceinline__ void nm_s_put(NmShared<VEC, AV>& sh, int wave, int cx, const NmMap<VEC, AV>& m) {
+#pragma unroll
+    for (int k = 0; k < AV; ++k) sh.a[wave][cx * AV + k] = m.a[k];
+#pragma unroll
+    for (int k = 0; k < VEC; ++k) sh.h[wave][cx * VEC + k] = m.h[k];
+    if (cx == 0) sh.f[wave] = m.f;
+}
+template <int VEC, int AV>
+__device__ __forceinline__ void nm_s_get(const NmShared<VEC, AV>& sh, int wave, int cx, NmMap<VEC, AV>& m) {
+#pragma unroll
+    for (int k = 0; k < AV; ++k) m.a[k] = sh.a[wave][cx * AV + k];
+#pragma unroll
+    for (int k = 0; k < VEC; ++k) m.h[k] = sh.h[wave][cx * VEC + k];
+    m.f = sh.f[wave];
+}
+
+// What a thread knows of its steps: bit s of first / final: the step is its sequence's first / last; none: it belongs to no sequence.
+struct NmSteps {
+    unsigned first, final, none;
+    int n, q;                            // n: steps of this thread; q, pos: sequence of step 0 in the order of the recurrence, and its place in it
+    unsigned pos;                        // (equal lengths)
+};
 
 template <int SEG>
-__device__ __forceinline__ NmSteps<SEG> nm_s_steps(const NmScanArgs& p, long long c0, long long c1, long long i0, unsigned pos0, long long q0) {
-    NmSteps<SEG> t;
-    t.first = t.final = 0u;
-    const long long left = c1 - i0;
-    t.n = left >= SEG ? SEG : left > 0 ? (int)left : 0;
+__device__ __forceinline__ NmSteps nm_s_steps(const NmScanArgs& p, const NmPlace& at, long long c0, long long c1, long long i0, unsigned pos0, long long q0) {
+    NmSteps t;
+    t.first = t.final = t.none = 0u;
+    t.n = c1 - i0 >= SEG ? SEG : c1 > i0 ? (int)(c1 - i0) : 0;
+    t.q = 0;
+    t.pos = 0;
     if (p.seg) {
-        int before = -2;
-        if (t.n > 0 && i0 > 0) before = p.seg[p.reverse ? p.L - i0 : i0 - 1];
+        if (t.n == 0) return t;
+        NmVec<NM_F32, 1> v[SEG];         // (bits of the sequence numbers)
+        nm_s_load_whole<NM_F32, 1, SEG>((const float*)p.seg, at, t.n, v);
+        int prev = -2, next = -2;
+        if (i0 > 0) prev = p.seg[p.reverse ? p.L - i0 : i0 - 1];
+        if (i0 + t.n < p.L) next = p.seg[p.reverse ? p.L - 1 - (i0 + t.n) : i0 + t.n];
 #pragma unroll
         for (int s = 0; s < SEG; ++s) {
-            t.seq[s] = -1;
-            if (s < t.n) t.seq[s] = p.seg[p.reverse ? p.L - 1 - (i0 + s) : i0 + s];
+            if (s >= t.n) continue;
+            const int q = __float_as_int(v[s].e[0]), after = s + 1 < t.n ? __float_as_int(v[s + 1 < SEG ? s + 1 : s].e[0]) : next;
+            if (prev != q || q < 0) t.first |= 1u << s;
+            if (after != q || q < 0) t.final |= 1u << s;
+            if (q < 0) t.none |= 1u << s;
+            prev = q;
         }
-        int after = -2;
-        if (t.n == SEG && i0 + SEG < p.L) after = p.seg[p.reverse ? p.L - 1 - (i0 + SEG) : i0 + SEG];
-        else if (t.n > 0 && t.n < SEG && i0 + t.n < p.L) after = p.seg[p.reverse ? p.L - 1 - (i0 + t.n) : i0 + t.n];
-#pragma unroll
-        for (int s = 0; s < SEG; ++s) {
-            const int prev = s == 0 ? before : t.seq[s > 0 ? s - 1 : 0], next = s + 1 < t.n ? t.seq[s + 1 < SEG ? s + 1 : s] : after;
-            if (prev != t.seq[s] || t.seq[s] < 0) t.first |= 1u << s;
-            if (next != t.seq[s] || t.seq[s] < 0) t.final |= 1u << s;
-        }
+        return t;
+    }
+    const unsigned valid = (1u << t.n) - 1u;
+    const unsigned off = (unsigned)(i0 - c0) + pos0, q = off / p.T, pos = off - q * p.T;
+    t.q = (int)(q0 + q);
+    t.pos = pos;
+    if (p.T >= SEG) {                    // one border at most
+        const unsigned k = p.T - pos;    // steps up to it
+        t.first = (pos == 0 ? 1u : 0u) | (k < SEG ? 1u << k : 0u);
+        t.final = k <= SEG ? 1u << (k - 1) : 0u;
     } else {
-        const unsigned off = (unsigned)(i0 - c0) + pos0, q = off / p.T;
-        unsigned pos = off - q * p.T;
-        int b = (int)(q0 + q);
-#pragma unroll
+        unsigned at = pos;
         for (int s = 0; s < SEG; ++s) {
-            t.seq[s] = p.reverse ? (int)(p.S - 1) - b : b;
-            if (pos == 0) t.first |= 1u << s;
-            if (pos + 1 == p.T) {
+            if (at == 0) t.first |= 1u << s;
+            if (++at == p.T) {
                 t.final |= 1u << s;
-                pos = 0;
-                ++b;
-            } else {
-                ++pos;
+                at = 0;
             }
         }
     }
+    t.first &= valid;
+    t.final &= valid;
     return t;
+}
+// sequence of step s (at borders only)
+__device__ __forceinline__ long long nm_s_sequence(const NmScanArgs& p, const NmSteps& t, long long i0, int s) {
+    if (p.seg) return p.seg[p.reverse ? p.L - 1 - (i0 + s) : i0 + s];
+    const int b = t.q + __popc(t.first & ((2u << s) - 2u));
+    return p.reverse ? p.S - 1 - b : b;
+}
+
+// where bit s of `border` is set: the value with which the sequence of step s starts (src [S, D], NULL: 0) instead of v
+template <int VEC>
+__device__ __forceinline__ void nm_s_enter(const NmScanArgs& p, const float* src, const NmSteps& t, unsigned border, long long i0, int s, int ch, float (&v)[VEC]) {
+    const bool at = (border >> s) & 1;
+#pragma unroll
+    for (int k = 0; k < VEC; ++k) v[k] = at ? 0.f : v[k];
+    if (src && at && !((t.none >> s) & 1)) {
+        const float* from = src + nm_s_sequence(p, t, i0, s) * p.D + ch;
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) v[k] = from[k];
+    }
+}
+
+// r and w of a gate a: plain a and 1, blend 1 - a and a
+template <int DG>
+__device__ __forceinline__ float nm_s_factor(typename NmType<DG>::elem e, int blend) {
+    return fmaf(nm_to_float<DG>(e), blend ? -1.0f : 1.0f, blend ? 1.0f : 0.0f);
+}
+// h -> r h + w x
+template <int DX, int DG, int VEC, int AV>
+__device__ __forceinline__ void nm_s_step(const NmVec<DG, AV>& g, const NmVec<DX, VEC>& x, int blend, float (&h)[VEC]) {
+#pragma unroll
+    for (int k = 0; k < VEC; ++k) {
+        const float a = nm_to_float<DG>(g.e[AV == 1 ? 0 : k]), v = nm_to_float<DX>(x.e[k]);
+        h[k] = fmaf(nm_s_factor<DG>(g.e[AV == 1 ? 0 : k], blend), h[k], blend ? a * v : v);
+    }
+}
+// steps beyond a thread's n: gates that leave the state as it is (the other operands are 0 there), so that no later pass has to ask
+template <int DG, int AV, int SEG>
+__device__ __forceinline__ void nm_s_pad(NmVec<DG, AV> (&g)[SEG], int n, int blend) {
+#pragma unroll
+    for (int s = 0; s < SEG; ++s)
+#pragma unroll
+        for (int k = 0; k < AV; ++k) g[s].e[k] = s < n ? g[s].e[k] : nm_from_float<DG>(blend ? 0.f : 1.f);
 }
 
 #define NM_S_THREADS 256
+// Steps of a thread.  Forward: as many as 32 .. 64 registers of operands allow (the scan's own instructions are per thread; with 4 steps they bound
+// short sequences at 2.4 TB/s).  Backward: three operands and the recomputed states.
+template <int VEC, bool SHARED> struct NmSeg {
+    static constexpr int F = VEC == 8 ? (SHARED ? 8 : 4) : 8;
+    static constexpr int B = VEC == 4 ? 4 : 8;
+};
 
-template <int DX, int DG, int VEC, int SEG, bool SHARED>
+// MAP: only the range's map, from its last sequence start on
+template <int DX, int DG, int VEC, bool SHARED, bool MAP>
 __global__ __launch_bounds__(NM_S_THREADS) void nm_scan_forward_kernel(NmScanArgs p) {
     typedef typename NmType<DX>::elem TX;
     typedef typename NmType<DG>::elem TG;
-    constexpr int GV = SHARED ? 1 : VEC;
-    __shared__ float sh_a[2][4][64 * VEC], sh_h[2][4][64 * VEC];
-    __shared__ int sh_f[2][4];
+    constexpr int AV = SHARED ? 1 : VEC, SEG = NmSeg<VEC, SHARED>::F;
+    constexpr bool WHOLE = VEC < 4;
+    __shared__ NmShared<VEC, AV> sh[2];
+    __shared__ uint4 lds_g[WHOLE ? 256 * NmStage<DG, AV, SEG>::STRIDE : 1], lds_x[WHOLE ? 256 * NmStage<DX, VEC, SEG>::STRIDE : 1];
     const int t = threadIdx.x, lane = t & 63, wave = t >> 6, cl = 1 << p.cl_log2, cx = t & (cl - 1), tl = t >> p.cl_log2;
     const int tile = (NM_S_THREADS >> p.cl_log2) * SEG;
     const long long c = blockIdx.x / p.blocks;
@@ -166,383 +371,332 @@ __global__ __launch_bounds__(NM_S_THREADS) void nm_scan_forward_kernel(NmScanArg
     // (channels that would end beyond D are the last VEC: computed twice, written twice with the same value)
     int ch = (blk * cl + cx) * VEC;
     if (ch + VEC > p.D) ch = p.D - VEC;
-    const long long step = p.reverse ? -1 : 1;
     const long long q0 = p.seg ? 0 : c0 / p.T;
     const unsigned pos0 = p.seg ? 0u : (unsigned)(c0 - q0 * p.T);
-    const long long tiles_per_chunk = (p.chunk + tile - 1) / tile;
 
-    NmMap<VEC> total;                    // map_only: everything before the current tile
+    NmMap<VEC, AV> total;                // MAP: everything before the current tile
     float state[VEC];                    // otherwise: the state before the current tile
-    total.f = 0;
+    nm_s_identity(total);
 #pragma unroll
-    for (int k = 0; k < VEC; ++k) {
-        total.a[k] = 1.f;
-        total.h[k] = 0.f;
-        state[k] = p.carry ? p.carry[c * p.D + ch + k] : 0.f;
-    }
+    for (int k = 0; k < VEC; ++k) state[k] = !MAP && p.carry ? p.carry[c * p.D + ch + k] : 0.f;
     long long b0 = c0;
-    if (p.map_only) {                    // what comes before the range's last sequence start does not matter
+    if constexpr (MAP) {                 // what comes before the range's last sequence start does not matter
         const long long s0 = p.seg ? nm_scan_reduce_from(p.cu, p.seg[p.reverse ? p.L - c1 : c1 - 1], p.reverse, p.L, c0, c1) : (c1 - 1) / p.T * p.T;
-        if (s0 > c0) b0 = c0 + (s0 - c0) / tile * tile;
+        if (s0 > c0) b0 = s0;
     }
     int buf = 0;
     for (long long b = b0; b < c1; b += tile, buf ^= 1) {
         const long long i0 = b + tl * SEG;
-        const long long row0 = p.reverse ? p.L - 1 - i0 : i0;
-        const TX* px = (const TX*)p.x + row0 * p.D + ch;
-        const TG* pg = (const TG*)p.gate + (SHARED ? row0 : row0 * p.D + ch);
-        const long long gs = SHARED ? step : step * p.D;
+        const NmPlace at = {p.reverse ? p.L - b - tile : b, (unsigned)(p.reverse ? tile - 1 - tl * SEG : tl * SEG), p.reverse};
+        const int n = c1 - i0 >= SEG ? SEG : c1 > i0 ? (int)(c1 - i0) : 0;
         NmVec<DX, VEC> xv[SEG];
-        NmVec<DG, GV> gv[SEG];
-        if (b + tile <= c1) {
-#pragma unroll
-            for (int s = 0; s < SEG; ++s) {
-                gv[s] = nm_s_load<DG, GV>(pg + s * gs);
-                xv[s] = nm_s_load<DX, VEC>(px + s * step * p.D);
-            }
+        NmVec<DG, AV> gv[SEG];
+        if constexpr (WHOLE) {
+            __syncthreads();             // (everybody has read the tile before)
+            nm_s_stage<DG, AV, SEG>((const TG*)p.gate, b, p.L, p.reverse, lds_g, t);
+            nm_s_stage<DX, VEC, SEG>((const TX*)p.x, b, p.L, p.reverse, lds_x, t);
+            __syncthreads();
+            nm_s_unstage<DG, AV, SEG>(lds_g, p.reverse, t, gv);
+            nm_s_unstage<DX, VEC, SEG>(lds_x, p.reverse, t, xv);
         } else {
+            if constexpr (SHARED) nm_s_load_whole<DG, 1, SEG>((const TG*)p.gate, at, n, gv);
+            else nm_s_load_steps<DG, AV, SEG>((const TG*)p.gate, at, p.D, ch, n, gv);
+            nm_s_load_steps<DX, VEC, SEG>((const TX*)p.x, at, p.D, ch, n, xv);
+        }
+        const NmSteps st = nm_s_steps<SEG>(p, at, c0, c1, i0, pos0, q0);
+        if (p.seg && __any(st.none != 0)) {                  // rows of no sequence: operands of 0 keep their states and gradients 0
 #pragma unroll
-            for (int s = 0; s < SEG; ++s) {
-                gv[s] = {};
-                xv[s] = {};
-                if (i0 + s < c1) {
-                    gv[s] = nm_s_load<DG, GV>(pg + s * gs);
-                    xv[s] = nm_s_load<DX, VEC>(px + s * step * p.D);
+            for (int s = 0; s < SEG; ++s)
+                if ((st.none >> s) & 1) {
+                    gv[s] = {};
+                    xv[s] = {};
                 }
+        }
+        if (n < SEG) {
+            nm_s_pad<DG, AV, SEG>(gv, n, p.blend);
+            if constexpr (WHOLE) {       // (staged rows beyond the range)
+#pragma unroll
+                for (int s = 0; s < SEG; ++s)
+                    if (s >= n) xv[s] = {};
             }
         }
-        const NmSteps<SEG> st = nm_s_steps<SEG>(p, c0, c1, i0, pos0, q0);
         // one step: state h -> r h + u
         auto advance = [&](int s, float (&h)[VEC]) {
-            if (((st.first >> s) & 1) != 0) {
-#pragma unroll
-                for (int k = 0; k < VEC; ++k) h[k] = p.h0 && st.seq[s] >= 0 ? p.h0[(long long)st.seq[s] * p.D + ch + k] : 0.f;
-            }
-#pragma unroll
-            for (int k = 0; k < VEC; ++k) {
-                const float a = (float)gv[s].e[SHARED ? 0 : k], x = (float)xv[s].e[k];
-                h[k] = p.blend ? fmaf(1.0f - a, h[k], a * x) : fmaf(a, h[k], x);
-                if (st.seq[s] < 0) h[k] = 0.f;
-            }
+            nm_s_enter(p, p.h0, st, st.first, i0, s, ch, h);
+            nm_s_step<DX, DG, VEC, AV>(gv[s], xv[s], p.blend, h);
         };
-        NmMap<VEC> m, before;
-        m.f = 0;
-#pragma unroll
-        for (int k = 0; k < VEC; ++k) {
-            m.a[k] = 1.f;
-            m.h[k] = 0.f;
-        }
+        NmMap<VEC, AV> m, before;
+        nm_s_identity(m);
 #pragma unroll
         for (int s = 0; s < SEG; ++s) {
-            if (s >= st.n) break;
-            if ((st.first >> s) & 1) m.f = 1;
             advance(s, m.h);
 #pragma unroll
-            for (int k = 0; k < VEC; ++k) {
-                const float a = (float)gv[s].e[SHARED ? 0 : k];
-                m.a[k] *= p.blend ? 1.0f - a : a;
-            }
+            for (int k = 0; k < AV; ++k) m.a[k] *= nm_s_factor<DG>(gv[s].e[k], p.blend);
         }
-        nm_s_wave_scan<VEC, 1>(m, before, lane, cl);
-        if (lane >= 64 - cl) {
-#pragma unroll
-            for (int k = 0; k < VEC; ++k) {
-                sh_a[buf][wave][cx * VEC + k] = m.a[k];
-                sh_h[buf][wave][cx * VEC + k] = m.h[k];
-            }
-            if (lane == 63) sh_f[buf][wave] = m.f;
-        }
+        m.f = st.first ? 1 : 0;
+        nm_s_wave_scan<VEC, AV, 1>(m, before, lane, cl);
+        if (lane >= 64 - cl) nm_s_put(sh[buf], wave, cx, m);
         __syncthreads();                 // (two buffers: a wave that is a tile ahead writes the other one)
-        if (!p.map_only && p.keep && tl == 0) {
-#pragma unroll
-            for (int k = 0; k < VEC; ++k) p.keep[(c * tiles_per_chunk + (b - c0) / tile) * p.D + ch + k] = state[k];
-        }
         float h[VEC];
 #pragma unroll
         for (int w = 0; w < 4; ++w) {
-            NmMap<VEC> mw;
-            mw.f = sh_f[buf][w];
+            NmMap<VEC, AV> mw;
+            nm_s_get(sh[buf], w, cx, mw);
+            if constexpr (MAP) {
+                nm_s_then(total, mw);
+            } else {
 #pragma unroll
-            for (int k = 0; k < VEC; ++k) {
-                mw.a[k] = sh_a[buf][w][cx * VEC + k];
-                mw.h[k] = sh_h[buf][w][cx * VEC + k];
-                if (w == wave) h[k] = state[k];
-            }
-            nm_s_apply(mw, state);
-            if (p.map_only) {
-#pragma unroll
-                for (int k = 0; k < VEC; ++k) total.a[k] = total.f || mw.f ? 0.f : total.a[k] * mw.a[k];
-                total.f |= mw.f;
+                for (int k = 0; k < VEC; ++k)
+                    if (w == wave) h[k] = state[k];
+                nm_s_apply(mw, state);
             }
         }
-        if (p.map_only) continue;
-        nm_s_apply(before, h);
+        if constexpr (!MAP) {
+            nm_s_apply(before, h);
+            if (p.keep && !p.keep_seq && n > 0 && ((unsigned)(i0 - c0) & (unsigned)(p.keep_steps - 1)) == 0) {
+                float* dst = p.keep + (c * ((p.chunk + p.keep_steps - 1) / p.keep_steps) + (i0 - c0) / p.keep_steps) * p.D + ch;
 #pragma unroll
-        for (int s = 0; s < SEG; ++s) {
-            if (s >= st.n) break;
-            advance(s, h);
-            if (p.states) nm_s_store<DX, VEC>((TX*)p.states + (row0 + s * step) * p.D + ch, h);
-            if (((st.final >> s) & 1) && st.seq[s] >= 0) {
+                for (int k = 0; k < VEC; ++k) dst[k] = h[k];
+            }
+            if (p.states || p.keep_seq || __any(st.final != 0)) {
+                float out[WHOLE ? SEG : 1][VEC];
+                const NmRow<TX> so = nm_s_rows((TX*)p.states, at, p.D, ch);
 #pragma unroll
-                for (int k = 0; k < VEC; ++k) p.last[(long long)st.seq[s] * p.D + ch + k] = h[k];
+                for (int s = 0; s < SEG; ++s) {
+                    if (p.keep_seq && s < n) {               // (sequences longer than keep_steps: one border in these steps at most)
+                        const unsigned left = p.T - st.pos, at_s = (unsigned)s < left ? st.pos + s : s - left;
+                        if (at_s > 0 && (at_s & (unsigned)(p.keep_steps - 1)) == 0) {
+                            const long long piece = (st.q + ((unsigned)s < left ? 0 : 1)) * (long long)((p.T + p.keep_steps - 1) / p.keep_steps) + at_s / p.keep_steps;
+#pragma unroll
+                            for (int k = 0; k < VEC; ++k) p.keep[piece * p.D + ch + k] = h[k];
+                        }
+                    }
+                    advance(s, h);
+                    if constexpr (WHOLE) {
+#pragma unroll
+                        for (int k = 0; k < VEC; ++k) out[s][k] = h[k];
+                    } else {
+                        if (p.states && s < n) nm_s_store<DX, VEC>(so.at(s), h);
+                    }
+                    if (((st.final & ~st.none) >> s) & 1) {
+                        float* dst = p.last + nm_s_sequence(p, st, i0, s) * p.D + ch;
+#pragma unroll
+                        for (int k = 0; k < VEC; ++k) dst[k] = h[k];
+                    }
+                }
+                if constexpr (WHOLE) {
+                    if (p.states) nm_s_store_whole<DX, VEC, SEG>((TX*)p.states, at, n, out);
+                }
             }
         }
     }
-    if (p.map_only && tl == 0) {
+    if (MAP && tl == 0) {
 #pragma unroll
         for (int k = 0; k < VEC; ++k) {
-            p.map_a[c * p.D + ch + k] = total.a[k];
-            p.map_h[c * p.D + ch + k] = state[k];
+            p.map_a[c * p.D + ch + k] = total.a[SHARED ? 0 : k];
+            p.map_h[c * p.D + ch + k] = total.h[k];
         }
         if (blk == 0 && cx == 0) p.map_f[c] = total.f || b0 > c0;
     }
 }
 
-template <int DX, int DG, int VEC, int SEG, bool SHARED>
+// MAP: only the range's map of the flow, up to its first sequence end
+template <int DX, int DG, int VEC, bool SHARED, bool MAP>
 __global__ __launch_bounds__(NM_S_THREADS) void nm_scan_backward_kernel(NmScanArgs p) {
     typedef typename NmType<DX>::elem TX;
     typedef typename NmType<DG>::elem TG;
-    constexpr int GV = SHARED ? 1 : VEC;
-    __shared__ float sh_a[2][4][64 * VEC], sh_h[2][4][64 * VEC], sh_b[2][4][64 * VEC], sh_r[2][4][64 * VEC];
-    __shared__ int sh_f[2][4], sh_e[2][4];
+    constexpr int AV = SHARED ? 1 : VEC, SEG = NmSeg<VEC, SHARED>::B;
+    constexpr bool WHOLE = VEC < 4;
+    __shared__ NmShared<VEC, AV> sh_r[2], sh_h[MAP ? 1 : 2];
     const int t = threadIdx.x, lane = t & 63, wave = t >> 6, cl = 1 << p.cl_log2, cx = t & (cl - 1), tl = t >> p.cl_log2;
     const int tile = (NM_S_THREADS >> p.cl_log2) * SEG;
     const long long c = blockIdx.x / p.blocks;
     const int blk = (int)(blockIdx.x % p.blocks);
-    const long long c0 = c * p.chunk, c1 = c0 + p.chunk < p.L ? c0 + p.chunk : p.L;
+    const long long c0 = c * p.chunk;
+    long long c1 = c0 + p.chunk < p.L ? c0 + p.chunk : p.L;
     const int own = (blk * cl + cx) * VEC;                   // first channel that is this thread's own (see the forward kernel)
     int ch = own;
     if (ch + VEC > p.D) ch = p.D - VEC;
-    const long long step = p.reverse ? -1 : 1;
     const long long q0 = p.seg ? 0 : c0 / p.T;
     const unsigned pos0 = p.seg ? 0u : (unsigned)(c0 - q0 * p.T);
-    const long long tiles_per_chunk = (p.chunk + tile - 1) / tile;
 
-    NmMap<VEC> total;                    // map_only: everything after the current tile
-    float flow[VEC];                     // f of the step after the current tile
-    total.f = 0;
+    NmMap<VEC, AV> total;                // MAP: everything after the current tile
+    float flow[VEC];                     // otherwise: f of the step after the current tile
+    nm_s_identity(total);
 #pragma unroll
-    for (int k = 0; k < VEC; ++k) {
-        total.a[k] = 1.f;
-        flow[k] = p.carry ? p.carry[c * p.D + ch + k] : 0.f;
-    }
-    long long tiles = (c1 - c0 + tile - 1) / tile;
+    for (int k = 0; k < VEC; ++k) flow[k] = !MAP && p.carry ? p.carry[c * p.D + ch + k] : 0.f;
     bool cut = false;
-    if (p.map_only) {                    // what comes after the range's first sequence end does not matter
+    if constexpr (MAP) {                 // what comes after the range's first sequence end does not matter
         const long long e = p.seg ? nm_scan_reduce_to(p.cu, p.seg[p.reverse ? p.L - 1 - c0 : c0], p.reverse, p.L, c0, c1) : c0 / p.T * p.T + p.T - 1;
-        if (e < c1) {
-            const long long need = (e - c0) / tile + 1;
-            cut = need < tiles;
-            tiles = need;
+        if (e + 1 < c1) {
+            cut = true;
+            c1 = e + 1;
         }
     }
+    const long long tiles = (c1 - c0 + tile - 1) / tile;
+    const bool want_x = !MAP && (p.dgate || p.dgate_part);
     int buf = 0;
     for (long long j = tiles - 1; j >= 0; --j, buf ^= 1) {
         const long long b = c0 + j * tile, i0 = b + tl * SEG;
-        const long long row0 = p.reverse ? p.L - 1 - i0 : i0;
-        const long long gs = SHARED ? step : step * p.D;
-        const TX* px = (const TX*)p.x + row0 * p.D + ch;
-        const TX* pc = (const TX*)p.g + row0 * p.D + ch;
-        const TG* pg = (const TG*)p.gate + (SHARED ? row0 : row0 * p.D + ch);
+        const NmPlace at = {p.reverse ? p.L - b - tile : b, (unsigned)(p.reverse ? tile - 1 - tl * SEG : tl * SEG), p.reverse};
+        const int n = c1 - i0 >= SEG ? SEG : c1 > i0 ? (int)(c1 - i0) : 0;
         NmVec<DX, VEC> xv[SEG], cv[SEG];
-        NmVec<DG, GV> gv[SEG];
-        const bool inside = b + tile <= c1, want_x = !p.map_only && (p.dgate || p.dgate_part);
+        NmVec<DG, AV> gv[SEG];
 #pragma unroll
         for (int s = 0; s < SEG; ++s) {
-            gv[s] = {};
             xv[s] = {};
             cv[s] = {};
         }
-        if (inside) {
-#pragma unroll
-            for (int s = 0; s < SEG; ++s) {
-                gv[s] = nm_s_load<DG, GV>(pg + s * gs);
-                if (p.g) cv[s] = nm_s_load<DX, VEC>(pc + s * step * p.D);
-                if (want_x) xv[s] = nm_s_load<DX, VEC>(px + s * step * p.D);
-            }
+        if constexpr (SHARED || WHOLE) nm_s_load_whole<DG, AV, SEG>((const TG*)p.gate, at, n, gv);
+        else nm_s_load_steps<DG, AV, SEG>((const TG*)p.gate, at, p.D, ch, n, gv);
+        if constexpr (WHOLE) {
+            if (p.g) nm_s_load_whole<DX, VEC, SEG>((const TX*)p.g, at, n, cv);
+            if (want_x) nm_s_load_whole<DX, VEC, SEG>((const TX*)p.x, at, n, xv);
         } else {
+            if (p.g) nm_s_load_steps<DX, VEC, SEG>((const TX*)p.g, at, p.D, ch, n, cv);
+            if (want_x) nm_s_load_steps<DX, VEC, SEG>((const TX*)p.x, at, p.D, ch, n, xv);
+        }
+        const NmSteps st = nm_s_steps<SEG>(p, at, c0, c1, i0, pos0, q0);
+        if (p.seg && __any(st.none != 0)) {                  // rows of no sequence: operands of 0 keep their states and gradients 0
 #pragma unroll
             for (int s = 0; s < SEG; ++s)
-                if (i0 + s < c1) {
-                    gv[s] = nm_s_load<DG, GV>(pg + s * gs);
-                    if (p.g) cv[s] = nm_s_load<DX, VEC>(pc + s * step * p.D);
-                    if (want_x) xv[s] = nm_s_load<DX, VEC>(px + s * step * p.D);
+                if ((st.none >> s) & 1) {
+                    gv[s] = {};
+                    xv[s] = {};
+                    cv[s] = {};
                 }
         }
-        const NmSteps<SEG> st = nm_s_steps<SEG>(p, c0, c1, i0, pos0, q0);
-        auto enter = [&](int s, float (&h)[VEC]) {           // state before step s, where it is a sequence's first
-            if ((st.first >> s) & 1) {
-#pragma unroll
-                for (int k = 0; k < VEC; ++k) h[k] = p.h0 && st.seq[s] >= 0 ? p.h0[(long long)st.seq[s] * p.D + ch + k] : 0.f;
-            }
-        };
-        auto advance = [&](int s, float (&h)[VEC]) {
-#pragma unroll
-            for (int k = 0; k < VEC; ++k) {
-                const float a = (float)gv[s].e[SHARED ? 0 : k], x = (float)xv[s].e[k];
-                h[k] = p.blend ? fmaf(1.0f - a, h[k], a * x) : fmaf(a, h[k], x);
-                if (st.seq[s] < 0) h[k] = 0.f;
-            }
-        };
+        auto enter = [&](int s, float (&h)[VEC]) { nm_s_enter(p, p.h0, st, st.first, i0, s, ch, h); };
+        if (n < SEG) nm_s_pad<DG, AV, SEG>(gv, n, p.blend);
+        auto advance = [&](int s, float (&h)[VEC]) { nm_s_step<DX, DG, VEC, AV>(gv[s], xv[s], p.blend, h); };
         auto retreat = [&](int s, float (&f)[VEC], float (&lam)[VEC]) {     // f of the step after s -> lambda and f of s
-            const bool end = (st.final >> s) & 1;
+            nm_s_enter(p, p.g_last, st, st.final, i0, s, ch, f);
 #pragma unroll
             for (int k = 0; k < VEC; ++k) {
-                const float a = (float)gv[s].e[SHARED ? 0 : k], r = p.blend ? 1.0f - a : a;
-                float v = end ? 0.f : f[k];
-                if (end && p.g_last && st.seq[s] >= 0) v = p.g_last[(long long)st.seq[s] * p.D + ch + k];
-                lam[k] = (float)cv[s].e[k] + v;
-                f[k] = r * lam[k];
-                if (st.seq[s] < 0) lam[k] = f[k] = 0.f;
+                lam[k] = nm_to_float<DX>(cv[s].e[k]) + f[k];
+                f[k] = nm_s_factor<DG>(gv[s].e[AV == 1 ? 0 : k], p.blend) * lam[k];
             }
         };
-        NmMap<VEC> mf, mr, bf, br;
-        mf.f = mr.f = 0;
-#pragma unroll
-        for (int k = 0; k < VEC; ++k) {
-            mf.a[k] = 1.f;
-            mf.h[k] = mr.h[k] = 0.f;
-        }
+        NmMap<VEC, AV> mf, mr, bf, br;
+        nm_s_identity(mf);
+        nm_s_identity(mr);
 #pragma unroll
         for (int s = 0; s < SEG; ++s) {
-            if (s >= st.n) break;
             if (want_x) {
-                if ((st.first >> s) & 1) mf.f = 1;
                 enter(s, mf.h);
                 advance(s, mf.h);
             }
 #pragma unroll
-            for (int k = 0; k < VEC; ++k) {
-                const float a = (float)gv[s].e[SHARED ? 0 : k];
-                mf.a[k] *= p.blend ? 1.0f - a : a;
-            }
+            for (int k = 0; k < AV; ++k) mf.a[k] *= nm_s_factor<DG>(gv[s].e[k], p.blend);
         }
 #pragma unroll
+        for (int k = 0; k < AV; ++k) mr.a[k] = mf.a[k];
+        mf.f = st.first ? 1 : 0;
+        mr.f = st.final ? 1 : 0;
+#pragma unroll
         for (int s = SEG - 1; s >= 0; --s) {
-            if (s >= st.n) continue;
             float lam[VEC];
-            if ((st.final >> s) & 1) mr.f = 1;
             retreat(s, mr.h, lam);
         }
-#pragma unroll
-        for (int k = 0; k < VEC; ++k) mr.a[k] = mf.a[k];
-        if (want_x) nm_s_wave_scan<VEC, 1>(mf, bf, lane, cl);
-        nm_s_wave_scan<VEC, -1>(mr, br, lane, cl);
-        if (want_x && lane >= 64 - cl) {
-#pragma unroll
-            for (int k = 0; k < VEC; ++k) {
-                sh_a[buf][wave][cx * VEC + k] = mf.a[k];
-                sh_h[buf][wave][cx * VEC + k] = mf.h[k];
-            }
-            if (lane == 63) sh_f[buf][wave] = mf.f;
-        }
-        if (lane < cl) {
-#pragma unroll
-            for (int k = 0; k < VEC; ++k) {
-                sh_b[buf][wave][cx * VEC + k] = mr.a[k];
-                sh_r[buf][wave][cx * VEC + k] = mr.h[k];
-            }
-            if (lane == 0) sh_e[buf][wave] = mr.f;
+        nm_s_wave_scan<VEC, AV, -1>(mr, br, lane, cl);
+        if (lane < cl) nm_s_put(sh_r[buf], wave, cx, mr);
+        if (want_x) {
+            nm_s_wave_scan<VEC, AV, 1>(mf, bf, lane, cl);
+            if (lane >= 64 - cl) nm_s_put(sh_h[MAP ? 0 : buf], wave, cx, mf);
         }
         __syncthreads();
-        float f[VEC], hp[SEG][VEC];
+        float f[VEC];
 #pragma unroll
         for (int w = 3; w >= 0; --w) {
-            NmMap<VEC> mw;
-            mw.f = sh_e[buf][w];
+            NmMap<VEC, AV> mw;
+            nm_s_get(sh_r[buf], w, cx, mw);
+            if constexpr (MAP) {
+                nm_s_then(total, mw);
+            } else {
 #pragma unroll
-            for (int k = 0; k < VEC; ++k) {
-                mw.a[k] = sh_b[buf][w][cx * VEC + k];
-                mw.h[k] = sh_r[buf][w][cx * VEC + k];
-                if (w == wave) f[k] = flow[k];
-            }
-            nm_s_apply(mw, flow);
-            if (p.map_only) {
-#pragma unroll
-                for (int k = 0; k < VEC; ++k) total.a[k] = total.f || mw.f ? 0.f : total.a[k] * mw.a[k];
-                total.f |= mw.f;
+                for (int k = 0; k < VEC; ++k)
+                    if (w == wave) f[k] = flow[k];
+                nm_s_apply(mw, flow);
             }
         }
-        if (p.map_only) continue;
-        nm_s_apply(br, f);
-        if (want_x) {
-            float h[VEC];
-#pragma unroll
-            for (int k = 0; k < VEC; ++k) h[k] = p.keep[(c * tiles_per_chunk + j) * p.D + ch + k];
-#pragma unroll
-            for (int w = 0; w < 3; ++w) {
-                NmMap<VEC> mw;
-                mw.f = sh_f[buf][w];
-#pragma unroll
-                for (int k = 0; k < VEC; ++k) {
-                    mw.a[k] = sh_a[buf][w][cx * VEC + k];
-                    mw.h[k] = sh_h[buf][w][cx * VEC + k];
-                }
-                if (w < wave) nm_s_apply(mw, h);
-            }
-            nm_s_apply(bf, h);
-#pragma unroll
-            for (int s = 0; s < SEG; ++s) {
-                if (s >= st.n) break;
-                enter(s, h);
-#pragma unroll
-                for (int k = 0; k < VEC; ++k) hp[s][k] = h[k];
-                advance(s, h);
-            }
-        }
-#pragma unroll
-        for (int s = SEG - 1; s >= 0; --s) {
-            if (s >= st.n) continue;
-            float lam[VEC], o[VEC];
-            retreat(s, f, lam);
-            if (p.dx) {
-#pragma unroll
-                for (int k = 0; k < VEC; ++k) o[k] = p.blend ? (float)gv[s].e[SHARED ? 0 : k] * lam[k] : lam[k];
-                if (st.seq[s] < 0) {
-#pragma unroll
-                    for (int k = 0; k < VEC; ++k) o[k] = 0.f;
-                }
-                nm_s_store<DX, VEC>((TX*)p.dx + (row0 + s * step) * p.D + ch, o);
-            }
+        if constexpr (!MAP) {
+            nm_s_apply(br, f);
+            float hp[SEG][VEC];          // states before the steps, then the gradient of the gate
             if (want_x) {
+                float h[VEC];
 #pragma unroll
-                for (int k = 0; k < VEC; ++k) {
-                    o[k] = lam[k] * (p.blend ? (float)xv[s].e[k] - hp[s][k] : hp[s][k]);
-                    if (st.seq[s] < 0) o[k] = 0.f;
+                for (int k = 0; k < VEC; ++k) h[k] = p.keep ? p.keep[(c * ((p.chunk + tile - 1) / tile) + j) * p.D + ch + k] : 0.f;
+#pragma unroll
+                for (int w = 0; w < 3; ++w) {
+                    NmMap<VEC, AV> mw;
+                    nm_s_get(sh_h[buf], w, cx, mw);
+                    if (w < wave) nm_s_apply(mw, h);
                 }
-                if constexpr (SHARED) {
-                    float sum = 0.f;
-#pragma unroll
-                    for (int k = 0; k < VEC; ++k) sum += ch + k >= own ? o[k] : 0.f;     // (own channels only)
-                    hp[s][0] = sum;
-                } else {
-                    nm_s_store<DG, VEC>((TG*)p.dgate + (row0 + s * step) * p.D + ch, o);
-                }
-            }
-            if (p.dh0 && ((st.first >> s) & 1) && st.seq[s] >= 0) {
-#pragma unroll
-                for (int k = 0; k < VEC; ++k) p.dh0[(long long)st.seq[s] * p.D + ch + k] = f[k];
-            }
-        }
-        if constexpr (SHARED) {
-            if (want_x) {                // sum over the channel lanes (all lanes of the wave take part)
+                nm_s_apply(bf, h);
 #pragma unroll
                 for (int s = 0; s < SEG; ++s) {
-                    float sum = s < st.n ? hp[s][0] : 0.f;
-                    for (int o = 1; o < cl; o <<= 1) sum += __shfl_xor(sum, o);
-                    if (s < st.n && cx == 0) {
-                        if (p.dgate_part) p.dgate_part[(long long)blk * p.L + row0 + s * step] = sum;
-                        else ((TG*)p.dgate)[row0 + s * step] = (TG)sum;
+                    enter(s, h);
+#pragma unroll
+                    for (int k = 0; k < VEC; ++k) hp[s][k] = h[k];
+                    advance(s, h);
+                }
+            }
+            float ox[WHOLE ? SEG : 1][VEC];
+            const NmRow<TX> rx = nm_s_rows((TX*)p.dx, at, p.D, ch);
+            const NmRow<TG> rg = nm_s_rows((TG*)p.dgate, at, SHARED ? 1 : p.D, SHARED ? 0 : ch);
+#pragma unroll
+            for (int s = SEG - 1; s >= 0; --s) {
+                float lam[VEC], o[VEC];
+                retreat(s, f, lam);
+#pragma unroll
+                for (int k = 0; k < VEC; ++k) {
+                    o[k] = p.blend ? nm_to_float<DG>(gv[s].e[SHARED ? 0 : k]) * lam[k] : lam[k];
+                    if constexpr (WHOLE) ox[s][k] = o[k];
+                }
+                if constexpr (!WHOLE) {
+                    if (p.dx && s < n) nm_s_store<DX, VEC>(rx.at(s), o);
+                }
+                if (want_x) {
+#pragma unroll
+                    for (int k = 0; k < VEC; ++k) hp[s][k] = lam[k] * (p.blend ? nm_to_float<DX>(xv[s].e[k]) - hp[s][k] : hp[s][k]);
+                    if constexpr (!SHARED && !WHOLE)
+                        if (s < n) nm_s_store<DG, VEC>(rg.at(s), hp[s]);
+                }
+                if (p.dh0 && (((st.first & ~st.none) >> s) & 1)) {
+                    float* dst = p.dh0 + nm_s_sequence(p, st, i0, s) * p.D + ch;
+#pragma unroll
+                    for (int k = 0; k < VEC; ++k) dst[k] = f[k];
+                }
+            }
+            if constexpr (WHOLE) {
+                if (p.dx) nm_s_store_whole<DX, VEC, SEG>((TX*)p.dx, at, n, ox);
+                if constexpr (!SHARED) {
+                    if (want_x) nm_s_store_whole<DG, VEC, SEG>((TG*)p.dgate, at, n, hp);
+                }
+            }
+            if constexpr (SHARED) {
+                if (want_x) {            // sum over the channels: own ones only, then the channel lanes (all lanes of the wave take part)
+                    float sum[SEG][1];
+#pragma unroll
+                    for (int s = 0; s < SEG; ++s) {
+                        sum[s][0] = 0.f;
+#pragma unroll
+                        for (int k = 0; k < VEC; ++k) sum[s][0] += ch + k >= own ? hp[s][k] : 0.f;
+                        for (int o = 1; o < cl; o <<= 1) sum[s][0] += __shfl_xor(sum[s][0], o);
+                    }
+                    if (cx == 0) {
+                        if (p.dgate_part) nm_s_store_whole<NM_F32, 1, SEG>(p.dgate_part + (long long)blk * p.L, at, n, sum);
+                        else nm_s_store_whole<DG, 1, SEG>((TG*)p.dgate, at, n, sum);
                     }
                 }
             }
         }
     }
-    if (p.map_only && tl == 0) {
+    if (MAP && tl == 0) {
 #pragma unroll
         for (int k = 0; k < VEC; ++k) {
-            p.map_a[c * p.D + ch + k] = total.a[k];
-            p.map_h[c * p.D + ch + k] = flow[k];
+            p.map_a[c * p.D + ch + k] = total.a[SHARED ? 0 : k];
+            p.map_h[c * p.D + ch + k] = total.h[k];
         }
         if (blk == 0 && cx == 0) p.map_f[c] = total.f || cut;
     }
@@ -560,7 +714,7 @@ __global__ __launch_bounds__(NM_S_THREADS) void nm_scan_carry_kernel(const float
     float state = 0.f;
     int buf = 0;
     for (long long b = 0; b < n; b += 512, buf ^= 1) {
-        NmMap<1> m, before, v[16];
+        NmMap<1, 1> m, before, v[16];
         m.a[0] = 1.f; m.h[0] = 0.f; m.f = 0;
 #pragma unroll
         for (int s = 0; s < 16; ++s) {
@@ -574,7 +728,7 @@ __global__ __launch_bounds__(NM_S_THREADS) void nm_scan_carry_kernel(const float
             m.a[0] *= v[s].a[0];
             m.f |= v[s].f;
         }
-        nm_s_wave_scan<1, 1>(m, before, lane, 8);
+        nm_s_wave_scan<1, 1, 1>(m, before, lane, 8);
         if (lane >= 56) {
             sh_a[buf][wave][cx] = m.a[0];
             sh_h[buf][wave][cx] = m.h[0];
@@ -585,7 +739,7 @@ __global__ __launch_bounds__(NM_S_THREADS) void nm_scan_carry_kernel(const float
 #pragma unroll
         for (int w = 0; w < 4; ++w) {
             if (w == wave) h[0] = all[0];
-            NmMap<1> mw;
+            NmMap<1, 1> mw;
             mw.a[0] = sh_a[buf][w][cx]; mw.h[0] = sh_h[buf][w][cx]; mw.f = sh_f[buf][w];
             nm_s_apply(mw, all);
         }
@@ -600,11 +754,11 @@ __global__ __launch_bounds__(NM_S_THREADS) void nm_scan_carry_kernel(const float
     }
 }
 
-// packed sequences: the sequence of every row (-1: none), and the result of empty sequences (their state / their cotangent passes through).
+// packed sequences: the sequence of every row (-1: none), and the result of empty sequences (their state / their cotangent passes through)
 __global__ __launch_bounds__(256) void nm_scan_rows_kernel(const int* __restrict__ cu, long long S, long long L, int D, const float* __restrict__ src, float* __restrict__ dst,
                                                            int* __restrict__ seg) {
     const long long t = (long long)blockIdx.x * 256 + threadIdx.x;
-    if (t < L) seg[t] = nm_scan_sequence(cu, S, t);
+    if (seg && t < L) seg[t] = nm_scan_sequence(cu, S, t);
     if (dst && t < S * D) {
         const long long s = t / D;
         if (cu[s + 1] <= cu[s]) dst[t] = src ? src[t] : 0.f;
@@ -631,74 +785,94 @@ __global__ __launch_bounds__(256) void nm_scan_gate_sum_kernel(const float* __re
 static inline long long nm_s_up(long long a, long long b) { return (a + b - 1) / b; }
 static inline size_t nm_s_align(size_t x) { return (x + 255) & ~(size_t)255; }
 
+struct NmScanShape { int vec, cl_log2, blocks, tile; };      // of one direction: channels and channel lanes, tile in steps
 struct NmScanPlan {
-    int vec, seg, cl_log2, blocks;
+    NmScanShape f, b;
     bool split;                          // ranges cut sequences: maps and carried states
-    long long tile, chunk, chunks, tiles_per_chunk;
+    long long chunk_f, chunks_f, chunk_b, chunks_b, keep_elems;
+    bool keep_seq;                       // kept states are counted from the sequences' starts (needed by those longer than a backward tile)
+    long long keep_rows;                 // packed: words of `keep` (and of the workspace) that hold the sequence of every row
     size_t off_seg, off_a, off_h, off_f, off_carry, off_part, bytes;
 };
 
 #define NM_S_FILL 1024       // workgroups that fill the chip
 
-static NmScanPlan nm_s_plan(long long L, long long S, int D, int dtype, bool packed, bool part) {
+static NmScanShape nm_s_shape(int D, int vec, int seg) {
+    NmScanShape s;
+    s.vec = vec;
+    const int groups = (int)nm_s_up(D, vec);
+    s.cl_log2 = 0;
+    while ((1 << s.cl_log2) < groups && s.cl_log2 < 6) ++s.cl_log2;
+    s.blocks = (int)nm_s_up(groups, 1 << s.cl_log2);
+    s.tile = (NM_S_THREADS >> s.cl_log2) * seg;
+    return s;
+}
+
+static NmScanPlan nm_s_plan(long long L, long long S, int D, int dtype, bool shared, bool packed) {
     NmScanPlan p;
-    p.vec = D >= 4 ? 4 : dtype == NM_F32 && D == 3 ? 3 : 1;
-    p.seg = p.vec == 4 ? 4 : 8;
-    const int groups = (int)nm_s_up(D, p.vec);
-    p.cl_log2 = 0;
-    while ((1 << p.cl_log2) < groups && p.cl_log2 < 6) ++p.cl_log2;
-    p.blocks = (int)nm_s_up(groups, 1 << p.cl_log2);
-    p.tile = (NM_S_THREADS >> p.cl_log2) * p.seg;
+    const int vb = D >= 4 ? 4 : D, vf = dtype != NM_F32 && D >= 8 ? 8 : vb;
+    const int seg_f = vf == 8 ? (shared ? NmSeg<8, true>::F : NmSeg<8, false>::F) : vf == 4 ? NmSeg<4, true>::F : NmSeg<1, true>::F;
+    const int seg_b = vb == 4 ? NmSeg<4, true>::B : NmSeg<1, true>::B;
+    p.f = nm_s_shape(D, vf, seg_f);
+    p.b = nm_s_shape(D, vb, seg_b);
+    // ranges: whole tiles of both directions (powers of two of the same), or whole sequences
+    const long long tile = p.f.tile > p.b.tile ? p.f.tile : p.b.tile;
+    const int blocks = p.f.blocks < p.b.blocks ? p.f.blocks : p.b.blocks;
     const long long T = packed || S == 0 ? 0 : L / S;
-    p.split = true;
-    if (!packed) {
-        const long long whole = T >= p.tile ? T : p.tile / (T > 0 ? T : 1) * T;       // steps of the sequences that fit a tile, or of one
-        if (T <= p.tile || nm_s_up(L, whole) * p.blocks >= NM_S_FILL / 2) {
-            p.split = false;
-            p.chunk = whole;
-        }
+    p.split = packed || (T > tile && S * blocks < NM_S_FILL / 2);
+    if (p.split) {
+        p.chunk_f = p.chunk_b = nm_s_up(nm_s_up(L, tile) * blocks, NM_S_FILL) * tile;
+        p.keep_elems = nm_s_up(L, p.chunk_b) * (p.chunk_b / p.b.tile) * D;
+        if (p.chunk_f >= L) p.split = false;                 // (one range)
+        p.keep_seq = false;
+    } else {
+        const long long t = T > 0 ? T : 1;
+        p.chunk_f = t >= p.f.tile ? t : p.f.tile / t * t;    // the sequences that fit a tile, or one
+        p.chunk_b = t >= p.b.tile ? t : p.b.tile / t * t;
+        p.keep_seq = t > p.b.tile;
+        p.keep_elems = p.keep_seq ? S * nm_s_up(t, p.b.tile) * D : 0;
     }
-    if (p.split) p.chunk = nm_s_up(nm_s_up(L, p.tile) * p.blocks, NM_S_FILL) * p.tile;
-    if (p.chunk < 1) p.chunk = 1;
-    p.chunks = nm_s_up(L, p.chunk);
-    if (p.chunks <= 1) p.split = false;
-    p.tiles_per_chunk = nm_s_up(p.chunk, p.tile);
+    p.chunks_f = nm_s_up(L, p.chunk_f);
+    p.chunks_b = nm_s_up(L, p.chunk_b);
+    p.keep_rows = packed ? nm_s_up(L, 64) * 64 : 0;
     size_t off = 0;
     p.off_seg = off;
-    if (packed) off += nm_s_align((size_t)L * 4);
+    off += (size_t)p.keep_rows * 4;
     p.off_a = off;
-    const size_t map = p.split ? nm_s_align((size_t)p.chunks * D * 4) : 0;
+    const size_t map = p.split ? nm_s_align((size_t)p.chunks_f * D * 4) : 0;
     off += map;
     p.off_h = off;
     off += map;
     p.off_carry = off;
     off += map;
     p.off_f = off;
-    if (p.split) off += nm_s_align((size_t)p.chunks * 4);
+    if (p.split) off += nm_s_align((size_t)p.chunks_f * 4);
     p.off_part = off;
-    if (part && p.blocks > 1) off += nm_s_align((size_t)p.blocks * L * 4);
+    if (shared && p.b.blocks > 1) off += nm_s_align((size_t)p.b.blocks * L * 4);
     p.bytes = off;
     return p;
 }
 
-#define NM_S_LAUNCH(KERNEL, DX, DG, VEC, SEG)                                                                                     \
+#define NM_S_LAUNCH(KERNEL, DX, DG, VEC, MAP)                                                                                     \
     do {                                                                                                                          \
-        if (shared) hipLaunchKernelGGL((KERNEL<DX, DG, VEC, SEG, true>), grid, dim3(NM_S_THREADS), 0, stream, a);                  \
-        else hipLaunchKernelGGL((KERNEL<DX, DG, VEC, SEG, false>), grid, dim3(NM_S_THREADS), 0, stream, a);                        \
+        if (shared) hipLaunchKernelGGL((KERNEL<DX, DG, VEC, true, MAP>), grid, dim3(NM_S_THREADS), 0, stream, a);                  \
+        else hipLaunchKernelGGL((KERNEL<DX, DG, VEC, false, MAP>), grid, dim3(NM_S_THREADS), 0, stream, a);                        \
     } while (0)
-#define NM_S_PICK_VEC(KERNEL, DX, DG)                                                                                             \
+#define NM_S_PICK_VEC(KERNEL, DX, DG, MAP, WIDE)                                                                                  \
     do {                                                                                                                          \
-        if (pl.vec == 4) NM_S_LAUNCH(KERNEL, DX, DG, 4, 4);                                                                       \
-        else NM_S_LAUNCH(KERNEL, DX, DG, 1, 8);                                                                                   \
+        if (shape.vec == 8) { if constexpr (WIDE) NM_S_LAUNCH(KERNEL, DX, DG, 8, MAP); }                                          \
+        else if (shape.vec == 4) NM_S_LAUNCH(KERNEL, DX, DG, 4, MAP);                                                             \
+        else if (shape.vec == 3) NM_S_LAUNCH(KERNEL, DX, DG, 3, MAP);                                                             \
+        else if (shape.vec == 2) NM_S_LAUNCH(KERNEL, DX, DG, 2, MAP);                                                             \
+        else NM_S_LAUNCH(KERNEL, DX, DG, 1, MAP);                                                                                 \
     } while (0)
-#define NM_S_PICK(KERNEL)                                                                                                         \
+#define NM_S_PICK(KERNEL, MAP, WIDE)                                                                                              \
     do {                                                                                                                          \
-        if (dtype == NM_F32 && pl.vec == 3) NM_S_LAUNCH(KERNEL, NM_F32, NM_F32, 3, 8);                                            \
-        else if (dtype == NM_F32) NM_S_PICK_VEC(KERNEL, NM_F32, NM_F32);                                                          \
-        else if (dtype == NM_F16 && gate_dtype == NM_F32) NM_S_PICK_VEC(KERNEL, NM_F16, NM_F32);                                  \
-        else if (dtype == NM_F16) NM_S_PICK_VEC(KERNEL, NM_F16, NM_F16);                                                          \
-        else if (gate_dtype == NM_F32) NM_S_PICK_VEC(KERNEL, NM_BF16, NM_F32);                                                    \
-        else NM_S_PICK_VEC(KERNEL, NM_BF16, NM_BF16);                                                                             \
+        if (dtype == NM_F32) NM_S_PICK_VEC(KERNEL, NM_F32, NM_F32, MAP, false);                                                   \
+        else if (dtype == NM_F16 && gate_dtype == NM_F32) NM_S_PICK_VEC(KERNEL, NM_F16, NM_F32, MAP, WIDE);                       \
+        else if (dtype == NM_F16) NM_S_PICK_VEC(KERNEL, NM_F16, NM_F16, MAP, WIDE);                                               \
+        else if (gate_dtype == NM_F32) NM_S_PICK_VEC(KERNEL, NM_BF16, NM_F32, MAP, WIDE);                                         \
+        else NM_S_PICK_VEC(KERNEL, NM_BF16, NM_BF16, MAP, WIDE);                                                                  \
     } while (0)
 
 static int nm_s_check(const char* who, int64_t L, int64_t S, int64_t D, int dtype, int gate_dtype, bool packed) {
@@ -708,12 +882,13 @@ static int nm_s_check(const char* who, int64_t L, int64_t S, int64_t D, int dtyp
     return 0;
 }
 
-static void nm_s_fill(NmScanArgs& a, const NmScanPlan& pl, const void* gate, const void* x, const float* h0, const int* cu, int64_t L, int64_t S, int64_t D, int reverse,
-                      int blend, char* ws) {
+static void nm_s_fill(NmScanArgs& a, const NmScanPlan& pl, const NmScanShape& shape, const void* gate, const void* x, const float* h0, const int* cu, int64_t L, int64_t S, int64_t D, int reverse,
+                      int blend, char* ws, int* rows) {
     a.gate = gate; a.x = x; a.h0 = h0; a.cu = cu;
-    a.seg = cu ? (const int*)(ws + pl.off_seg) : nullptr;
-    a.L = L; a.S = S; a.chunk = pl.chunk; a.T = cu || S == 0 ? 1u : (unsigned)(L / S); a.D = (int)D;
-    a.reverse = reverse ? 1 : 0; a.blend = blend ? 1 : 0; a.cl_log2 = pl.cl_log2; a.blocks = pl.blocks;
+    a.seg = cu ? rows : nullptr;
+    a.L = L; a.S = S; a.chunk = &shape == &pl.f ? pl.chunk_f : pl.chunk_b; a.T = cu || S == 0 ? 1u : (unsigned)(L / S); a.D = (int)D;
+    a.reverse = reverse ? 1 : 0; a.blend = blend ? 1 : 0; a.cl_log2 = shape.cl_log2; a.blocks = shape.blocks;
+    a.keep_steps = pl.b.tile;
     if (pl.split) {
         a.map_a = (float*)(ws + pl.off_a); a.map_h = (float*)(ws + pl.off_h); a.map_f = (int*)(ws + pl.off_f);
     }
@@ -721,16 +896,16 @@ static void nm_s_fill(NmScanArgs& a, const NmScanPlan& pl, const void* gate, con
 
 extern "C" {
 
-int64_t nm_scan_workspace_bytes(int64_t L, int64_t S, int64_t D, int dtype, int packed, int backward) {
+int64_t nm_scan_workspace_bytes(int64_t L, int64_t S, int64_t D, int dtype, int shared_gate, int packed) {
     if (nm_s_check("nm_scan_workspace_bytes", L, S, D, dtype, dtype, packed != 0)) return -1;
-    return L == 0 || D == 0 ? 0 : (int64_t)nm_s_plan(L, S, (int)D, dtype, packed != 0, backward != 0).bytes;
+    return L == 0 || D == 0 ? 0 : (int64_t)nm_s_plan(L, S, (int)D, dtype, shared_gate != 0, packed != 0).bytes;
 }
 
-int64_t nm_scan_keep_elems(int64_t L, int64_t S, int64_t D, int dtype, int packed) {
+int64_t nm_scan_keep_elems(int64_t L, int64_t S, int64_t D, int dtype, int shared_gate, int packed) {
     if (nm_s_check("nm_scan_keep_elems", L, S, D, dtype, dtype, packed != 0)) return -1;
     if (L == 0 || D == 0) return 0;
-    const NmScanPlan pl = nm_s_plan(L, S, (int)D, dtype, packed != 0, false);
-    return pl.chunks * pl.tiles_per_chunk * D;
+    const NmScanPlan pl = nm_s_plan(L, S, (int)D, dtype, shared_gate != 0, packed != 0);
+    return pl.keep_rows + pl.keep_elems;
 }
 
 int nm_scan_forward(const void* gate, int gate_dtype, int shared_gate, const void* x, int dtype, const float* h0, const int32_t* cu_seqlens, int64_t L, int64_t S, int64_t D,
@@ -745,27 +920,28 @@ int nm_scan_forward(const void* gate, int gate_dtype, int shared_gate, const voi
         NM_LAUNCH_CHECK();
         return 0;
     }
-    const NmScanPlan pl = nm_s_plan(L, S, (int)D, dtype, packed, false);
+    const NmScanPlan pl = nm_s_plan(L, S, (int)D, dtype, shared, packed);
+    const NmScanShape& shape = pl.f;
     if ((size_t)(workspace_bytes < 0 ? 0 : workspace_bytes) < pl.bytes || (pl.bytes > 0 && !workspace)) return nm_fail("nm_scan_forward: workspace too small");
-    if (pl.chunks * pl.blocks > 0x7fffffffLL) return nm_fail("nm_scan_forward: %lld steps x %lld channels exceed one launch", (long long)L, (long long)D);
+    if (pl.chunks_f * shape.blocks > 0x7fffffffLL) return nm_fail("nm_scan_forward: %lld steps x %lld channels exceed one launch", (long long)L, (long long)D);
     char* ws = (char*)workspace;
+    int* rows = packed ? keep ? (int*)keep : (int*)(ws + pl.off_seg) : nullptr;
     if (packed) {
         const long long n = L > S * D ? L : S * D;
-        hipLaunchKernelGGL(nm_scan_rows_kernel, dim3((unsigned)nm_s_up(n, 256)), dim3(256), 0, stream, cu_seqlens, (long long)S, (long long)L, (int)D, h0, last, (int*)(ws + pl.off_seg));
+        hipLaunchKernelGGL(nm_scan_rows_kernel, dim3((unsigned)nm_s_up(n, 256)), dim3(256), 0, stream, cu_seqlens, (long long)S, (long long)L, (int)D, h0, last, rows);
     }
     NmScanArgs a = {};
-    nm_s_fill(a, pl, gate, x, h0, cu_seqlens, L, S, D, reverse, blend, ws);
-    a.states = states; a.last = last; a.keep = keep;
-    const dim3 grid((unsigned)(pl.chunks * pl.blocks));
+    nm_s_fill(a, pl, shape, gate, x, h0, cu_seqlens, L, S, D, reverse, blend, ws, rows);
+    a.states = states; a.last = last; a.keep = keep && pl.keep_elems > 0 ? keep + pl.keep_rows : nullptr;
+    a.keep_seq = a.keep && pl.keep_seq;
+    const dim3 grid((unsigned)(pl.chunks_f * shape.blocks));
     if (pl.split) {
         float* carry = (float*)(ws + pl.off_carry);
-        a.map_only = 1;
-        NM_S_PICK(nm_scan_forward_kernel);
-        hipLaunchKernelGGL(nm_scan_carry_kernel<1>, dim3((unsigned)nm_s_up(D, 8)), dim3(NM_S_THREADS), 0, stream, a.map_a, a.map_h, a.map_f, pl.chunks, (int)D, carry);
-        a.map_only = 0;
+        NM_S_PICK(nm_scan_forward_kernel, true, true);
+        hipLaunchKernelGGL(nm_scan_carry_kernel<1>, dim3((unsigned)nm_s_up(D, 8)), dim3(NM_S_THREADS), 0, stream, a.map_a, a.map_h, a.map_f, pl.chunks_f, (int)D, carry);
         a.carry = carry;
     }
-    NM_S_PICK(nm_scan_forward_kernel);
+    NM_S_PICK(nm_scan_forward_kernel, false, true);
     NM_LAUNCH_CHECK();
     return 0;
 }
@@ -777,41 +953,41 @@ int nm_scan_backward(const void* gate, int gate_dtype, int shared_gate, const vo
     const bool packed = cu_seqlens != nullptr, shared = shared_gate != 0;
     if (nm_s_check("nm_scan_backward", L, S, D, dtype, gate_dtype, packed)) return 1;
     if (D == 0 || (L == 0 && S == 0) || (!dgate && !dx && !dh0)) return 0;
-    if (L > 0 && (!gate || (dgate && (!x || !keep)))) return nm_fail("nm_scan_backward: NULL argument");
+    if (L > 0 && (!gate || (dgate && (!x || (!keep && nm_scan_keep_elems(L, S, D, dtype, shared_gate, packed) > 0))))) return nm_fail("nm_scan_backward: NULL argument");
     if (L == 0) {
         if (!dh0) return 0;
         hipLaunchKernelGGL(nm_scan_pass_kernel, dim3((unsigned)nm_s_up(S * D, 256)), dim3(256), 0, stream, g_last, dh0, (long long)(S * D));
         NM_LAUNCH_CHECK();
         return 0;
     }
-    const NmScanPlan pl = nm_s_plan(L, S, (int)D, dtype, packed, true);
+    const NmScanPlan pl = nm_s_plan(L, S, (int)D, dtype, shared, packed);
+    const NmScanShape& shape = pl.b;
     if ((size_t)(workspace_bytes < 0 ? 0 : workspace_bytes) < pl.bytes || (pl.bytes > 0 && !workspace)) return nm_fail("nm_scan_backward: workspace too small");
-    if (pl.chunks * pl.blocks > 0x7fffffffLL) return nm_fail("nm_scan_backward: %lld steps x %lld channels exceed one launch", (long long)L, (long long)D);
+    if (pl.chunks_b * shape.blocks > 0x7fffffffLL) return nm_fail("nm_scan_backward: %lld steps x %lld channels exceed one launch", (long long)L, (long long)D);
     char* ws = (char*)workspace;
-    if (packed) {
-        const long long n = L > S * D ? L : S * D;
-        hipLaunchKernelGGL(nm_scan_rows_kernel, dim3((unsigned)nm_s_up(n, 256)), dim3(256), 0, stream, cu_seqlens, (long long)S, (long long)L, (int)D, g_last, dh0, (int*)(ws + pl.off_seg));
+    int* rows = packed ? keep ? (int*)const_cast<float*>(keep) : (int*)(ws + pl.off_seg) : nullptr;
+    if (packed && (!keep || dh0)) {      // (the rows' sequences are kept from the forward pass)
+        const long long n = keep ? S * D : L > S * D ? L : S * D;
+        hipLaunchKernelGGL(nm_scan_rows_kernel, dim3((unsigned)nm_s_up(n, 256)), dim3(256), 0, stream, cu_seqlens, (long long)S, (long long)L, (int)D, g_last, dh0, keep ? nullptr : rows);
     }
     NmScanArgs a = {};
-    nm_s_fill(a, pl, gate, x, h0, cu_seqlens, L, S, D, reverse, blend, ws);
-    a.keep = const_cast<float*>(keep); a.g = g_states; a.g_last = g_last; a.dgate = dgate; a.dx = dx; a.dh0 = dh0;
-    const bool parts = shared && dgate && pl.blocks > 1;
+    nm_s_fill(a, pl, shape, gate, x, h0, cu_seqlens, L, S, D, reverse, blend, ws, rows);
+    a.keep = keep && pl.keep_elems > 0 ? const_cast<float*>(keep) + pl.keep_rows : nullptr; a.g = g_states; a.g_last = g_last; a.dgate = dgate; a.dx = dx; a.dh0 = dh0;
+    const bool parts = shared && dgate && shape.blocks > 1;
     if (parts) a.dgate_part = (float*)(ws + pl.off_part);
-    const dim3 grid((unsigned)(pl.chunks * pl.blocks));
+    const dim3 grid((unsigned)(pl.chunks_b * shape.blocks));
     if (pl.split) {
         float* carry = (float*)(ws + pl.off_carry);
-        a.map_only = 1;
-        NM_S_PICK(nm_scan_backward_kernel);
-        hipLaunchKernelGGL(nm_scan_carry_kernel<-1>, dim3((unsigned)nm_s_up(D, 8)), dim3(NM_S_THREADS), 0, stream, a.map_a, a.map_h, a.map_f, pl.chunks, (int)D, carry);
-        a.map_only = 0;
+        NM_S_PICK(nm_scan_backward_kernel, true, false);
+        hipLaunchKernelGGL(nm_scan_carry_kernel<-1>, dim3((unsigned)nm_s_up(D, 8)), dim3(NM_S_THREADS), 0, stream, a.map_a, a.map_h, a.map_f, pl.chunks_b, (int)D, carry);
         a.carry = carry;
     }
-    NM_S_PICK(nm_scan_backward_kernel);
+    NM_S_PICK(nm_scan_backward_kernel, false, false);
     if (parts) {
         const dim3 g2((unsigned)nm_s_up(L, 256));
-        if (gate_dtype == NM_F32) hipLaunchKernelGGL(nm_scan_gate_sum_kernel<NM_F32>, g2, dim3(256), 0, stream, a.dgate_part, pl.blocks, (long long)L, (float*)dgate);
-        else if (gate_dtype == NM_F16) hipLaunchKernelGGL(nm_scan_gate_sum_kernel<NM_F16>, g2, dim3(256), 0, stream, a.dgate_part, pl.blocks, (long long)L, (_Float16*)dgate);
-        else hipLaunchKernelGGL(nm_scan_gate_sum_kernel<NM_BF16>, g2, dim3(256), 0, stream, a.dgate_part, pl.blocks, (long long)L, (__bf16*)dgate);
+        if (gate_dtype == NM_F32) hipLaunchKernelGGL(nm_scan_gate_sum_kernel<NM_F32>, g2, dim3(256), 0, stream, a.dgate_part, shape.blocks, (long long)L, (float*)dgate);
+        else if (gate_dtype == NM_F16) hipLaunchKernelGGL(nm_scan_gate_sum_kernel<NM_F16>, g2, dim3(256), 0, stream, a.dgate_part, shape.blocks, (long long)L, (_Float16*)dgate);
+        else hipLaunchKernelGGL(nm_scan_gate_sum_kernel<NM_BF16>, g2, dim3(256), 0, stream, a.dgate_part, shape.blocks, (long long)L, (__bf16*)dgate);
     }
     NM_LAUNCH_CHECK();
     return 0;

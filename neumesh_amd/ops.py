@@ -75,13 +75,18 @@ def _once(who):
 # ------------------------------------------------------------------------------------------------ dense layers
 def _rows(t, n: int):
     """[..., n] as rows with a unit last stride -> (tensor [M, n], row stride in elements)."""
-    t = t.reshape(math.prod(t.shape[:-1]), n)
-    if (n > 1 and t.stride(1) != 1) or (t.shape[0] > 1 and not n <= t.stride(0) <= _MAX_STRIDE):
-        t = t.contiguous()
-    return t, (t.stride(0) if t.shape[0] > 1 else n)
+    if t.dim() != 2:
+        t = t.reshape(math.prod(t.shape[:-1]), n)
+    if t.is_contiguous():
+        return t, n
+    m, k = t.stride()
+    if (n > 1 and k != 1) or (t.shape[0] > 1 and not n <= m <= _MAX_STRIDE):
+        return t.contiguous(), n
+    return t, (m if t.shape[0] > 1 else n)
 
 
 def _dense_forward(x, weight, bias, residual, act: int, beta: float, want_deriv: bool):
+    """-> (y, what the backward pass needs besides tensors: sizes and strides; rows of x, rows of the weight, act'(z))"""
     lib = _lib.load()
     N, K = weight.shape
     x2, ldx = _rows(x, K)
@@ -96,37 +101,39 @@ def _dense_forward(x, weight, bias, residual, act: int, beta: float, want_deriv:
     with _on(dev):
         _lib.check(lib.nm_dense_forward(x2.data_ptr(), ldx, w2.data_ptr(), ldw, _ptr(b), dt if b is None else _DTYPES[b.dtype], _ptr(r2), ldr, M, K, N, dt, act, beta,
                                         y.data_ptr(), N, _ptr(deriv), _ptr(ws), nbytes, _stream(dev)), "nm_dense_forward")
-    return y, x2, deriv
+    return y, (M, K, N, ldx, ldw, dt), x2, w2, deriv
 
 
 class _Dense(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, residual, act, beta):
-        y, x2, deriv = _dense_forward(x, weight, bias, residual, act, beta, any(ctx.needs_input_grad[:3]))
-        ctx.save_for_backward(x2 if ctx.needs_input_grad[1] else None, weight, deriv)
-        ctx.x_shape, ctx.bias_dtype, ctx.act = x.shape, None if bias is None else bias.dtype, act
+        need = ctx.needs_input_grad
+        y, ctx.sizes, x2, w2, ctx.deriv = _dense_forward(x, weight, bias, residual, act, beta, need[0] or need[1] or need[2])
+        ctx.save_for_backward(x2 if need[1] else None, w2 if need[0] else None)
+        ctx.x_shape, ctx.weight_dtype, ctx.bias_dtype = x.shape, weight.dtype, None if bias is None else bias.dtype
         return y
 
     @staticmethod
     def backward(ctx, g):
+        # (runs on the engine's own thread, where every Python line costs twice: sizes and strides come from the forward pass)
         _once("dense")
-        lib = _lib.load()
-        x2, weight, deriv = ctx.saved_tensors
         need_x, need_w, need_b, need_r = ctx.needs_input_grad[:4]
-        dev, dt = weight.device, _DTYPES[weight.dtype]
-        N, K = weight.shape
-        g2, ldg = _rows(g, N)
-        M = g2.shape[0]
-        dx = torch.empty(ctx.x_shape, dtype=weight.dtype, device=dev) if need_x else None
-        dw = torch.empty((N, K), dtype=weight.dtype, device=dev) if need_w else None
-        db = torch.empty((N,), dtype=ctx.bias_dtype, device=dev) if need_b else None
+        dx = dw = db = None
         if need_x or need_w or need_b:
-            w2, ldw = _rows(weight, K)
-            x2, ldx = (None, K) if x2 is None else _rows(x2, K)
+            lib, dev, empty = _lib.load(), g.device, torch.empty
+            x2, w2 = ctx.saved_tensors
+            M, K, N, ldx, ldw, dt = ctx.sizes
+            g2, ldg = (g, N) if g.is_contiguous() else _rows(g, N)
+            if need_x:
+                dx = empty(ctx.x_shape, dtype=ctx.weight_dtype, device=dev)
+            if need_w:
+                dw = empty((N, K), dtype=ctx.weight_dtype, device=dev)
+            if need_b:
+                db = empty((N,), dtype=ctx.bias_dtype, device=dev)
             nbytes = lib.nm_dense_workspace_bytes(M, K, N, dt, 1)
-            ws = torch.empty((nbytes,), dtype=torch.uint8, device=dev) if nbytes > 0 else None
+            ws = empty((nbytes,), dtype=torch.uint8, device=dev) if nbytes > 0 else None
             with _on(dev):
-                _lib.check(lib.nm_dense_backward(g2.data_ptr(), ldg, _ptr(deriv), _ptr(x2), ldx, w2.data_ptr(), ldw, M, K, N, dt, _ptr(dx), K, _ptr(dw), _ptr(db),
+                _lib.check(lib.nm_dense_backward(g2.data_ptr(), ldg, _ptr(ctx.deriv), _ptr(x2), ldx, _ptr(w2), ldw, M, K, N, dt, _ptr(dx), K, _ptr(dw), _ptr(db),
                                                  dt if db is None else _DTYPES[db.dtype], _ptr(ws), nbytes, _stream(dev)), "nm_dense_backward")
         return dx, dw, db, (g if need_r else None), None, None
 
@@ -172,14 +179,14 @@ def _scan_forward(gate, x, h0, cu, reverse, blend, need_states, want_keep):
     lib = _lib.load()
     dev, dt = x.device, _DTYPES[x.dtype]
     L, S, D = _scan_sizes(x, cu)
-    packed = int(cu is not None)
+    packed, shared = int(cu is not None), int(gate.shape[-1] != D)
     states = torch.empty_like(x) if need_states else None
     last = torch.empty((S, D), dtype=torch.float32, device=dev)
-    keep = torch.empty((lib.nm_scan_keep_elems(L, S, D, dt, packed),), dtype=torch.float32, device=dev) if want_keep else None
-    nbytes = lib.nm_scan_workspace_bytes(L, S, D, dt, packed, 0)
+    keep = torch.empty((lib.nm_scan_keep_elems(L, S, D, dt, shared, packed),), dtype=torch.float32, device=dev) if want_keep else None
+    nbytes = lib.nm_scan_workspace_bytes(L, S, D, dt, shared, packed)
     ws = torch.empty((nbytes,), dtype=torch.uint8, device=dev) if nbytes > 0 else None
     with _on(dev):
-        _lib.check(lib.nm_scan_forward(gate.data_ptr(), _DTYPES[gate.dtype], int(gate.shape[-1] != D), x.data_ptr(), dt, _ptr(h0), _ptr(cu), L, S, D, int(reverse),
+        _lib.check(lib.nm_scan_forward(gate.data_ptr(), _DTYPES[gate.dtype], shared, x.data_ptr(), dt, _ptr(h0), _ptr(cu), L, S, D, int(reverse),
                                        int(blend), _ptr(states), last.data_ptr(), _ptr(keep), _ptr(ws), nbytes, _stream(dev)), "nm_scan_forward")
     return states, last, keep
 
@@ -188,8 +195,8 @@ class _GatedScan(torch.autograd.Function):
     @staticmethod
     def forward(ctx, gate, x, h0, cu, reverse, blend, need_states):
         ctx.set_materialize_grads(False)
-        states, last, keep = _scan_forward(gate, x, h0, cu, reverse, blend, need_states, ctx.needs_input_grad[0])
-        ctx.save_for_backward(gate, x, h0, cu, keep)
+        states, last, ctx.keep = _scan_forward(gate, x, h0, cu, reverse, blend, need_states, ctx.needs_input_grad[0] or cu is not None)
+        ctx.save_for_backward(gate, x, h0, cu)
         ctx.reverse, ctx.blend = reverse, blend
         return states, last
 
@@ -197,21 +204,21 @@ class _GatedScan(torch.autograd.Function):
     def backward(ctx, g_states, g_last):
         _once("gated_scan")
         lib = _lib.load()
-        gate, x, h0, cu, keep = ctx.saved_tensors
+        gate, x, h0, cu = ctx.saved_tensors
         dev, dt = x.device, _DTYPES[x.dtype]
         L, S, D = _scan_sizes(x, cu)
-        packed = int(cu is not None)
+        packed, shared = int(cu is not None), int(gate.shape[-1] != D)
         need_gate, need_x, need_h0 = ctx.needs_input_grad[:3]
         g_states = None if g_states is None else g_states.contiguous()
         g_last = None if g_last is None else g_last.contiguous()
         dgate = torch.empty_like(gate) if need_gate else None
         dx = torch.empty_like(x) if need_x else None
         dh0 = torch.empty_like(h0) if need_h0 else None
-        nbytes = lib.nm_scan_workspace_bytes(L, S, D, dt, packed, 1)
+        nbytes = lib.nm_scan_workspace_bytes(L, S, D, dt, shared, packed)
         ws = torch.empty((nbytes,), dtype=torch.uint8, device=dev) if nbytes > 0 else None
         with _on(dev):
-            _lib.check(lib.nm_scan_backward(gate.data_ptr(), _DTYPES[gate.dtype], int(gate.shape[-1] != D), x.data_ptr(), dt, _ptr(h0), _ptr(cu), L, S, D,
-                                            int(ctx.reverse), int(ctx.blend), _ptr(keep), _ptr(g_states), _ptr(g_last), _ptr(dgate), _ptr(dx), _ptr(dh0),
+            _lib.check(lib.nm_scan_backward(gate.data_ptr(), _DTYPES[gate.dtype], shared, x.data_ptr(), dt, _ptr(h0), _ptr(cu), L, S, D,
+                                            int(ctx.reverse), int(ctx.blend), _ptr(ctx.keep), _ptr(g_states), _ptr(g_last), _ptr(dgate), _ptr(dx), _ptr(dh0),
                                             _ptr(ws), nbytes, _stream(dev)), "nm_scan_backward")
         return dgate, dx, dh0, None, None, None, None
 

@@ -358,7 +358,7 @@ def check_scan(a, x, h0, cu, D, shared, blend, reverse, packed, states=True, use
 
 
 SCANS = [(1, 1, 1), (3, 1, 5), (512, 1, 9), (2, 7, 3), (5, 127, 3), (40, 16, 2), (4, 64, 32), (2, 1000, 8), (1, 5000, 4), (3, 129, 257), (2, 40, 6), (1, 2300, 1), (6, 300, 33),
-         (1, 700, 1030)]
+         (1, 700, 1030), (40, 100, 33), (180, 35, 1030)]
 
 
 @pytest.mark.parametrize("dtype", [("fp32", "fp32"), ("bf16", "bf16"), ("bf16", "fp32"), ("fp16", "fp16"), ("fp16", "fp32")], ids="/".join)

@@ -57,7 +57,7 @@ def test_c_entries_refuse(dtype):
 
     def bwd(g=p, ldg=4, x=p, ldx=8, w=p, ldw=8, M=20, K=8, N=4, dt=dtype, dx=p, lddx=8, dw=p, db=p, bdt=dtype, ws=p, n=1 << 30):
         return lib.nm_dense_backward(g, ldg, None, x, ldx, w, ldw, M, K, N, dt, dx, lddx, dw, db, bdt, ws, n, None)
-    for bad in (dict(g=None), dict(x=None), dict(w=None), dict(ldg=3), dict(ldx=7), dict(ldw=7), dict(lddx=7), dict(dt=5), dict(bdt=5), dict(n=16), dict(ws=None), dict(M=-2)):
+    for bad in (dict(g=None), dict(x=None), dict(w=None), dict(ldg=3), dict(ldx=7), dict(ldw=7), dict(lddx=7), dict(dt=5), dict(bdt=5), dict(M=3000, n=16), dict(M=3000, n=-1), dict(M=3000, ws=None), dict(M=-2)):
         assert bwd(**bad) == 1 and lib.nm_last_error(), bad
     assert bwd(dx=None, dw=None, db=None, g=None) == 0
 
@@ -68,15 +68,15 @@ def test_c_entries_refuse(dtype):
         assert scan(**bad) == 1 and lib.nm_last_error(), bad
     assert scan(D=0) == 0 and scan(L=0, S=0) == 0
 
-    def back(gate=p, x=p, keep=p, dt=dtype, cu=None, L=12, S=3, D=4, dgate=p, dx=p, dh0=p, ws=p, n=1 << 30):
+    def back(gate=p, x=p, keep=p, dt=dtype, cu=None, L=12000, S=3, D=4, dgate=p, dx=p, dh0=p, ws=p, n=1 << 30):
         return lib.nm_scan_backward(gate, dt, 0, x, dt, None, cu, L, S, D, 0, 0, keep, None, None, dgate, dx, dh0, ws, n, None)
-    for bad in (dict(gate=None), dict(x=None), dict(keep=None), dict(dt=9), dict(L=13), dict(cu=p, n=4), dict(cu=p, ws=None)):
+    for bad in (dict(gate=None), dict(x=None), dict(keep=None), dict(dt=9), dict(L=12001), dict(cu=p, n=4), dict(cu=p, ws=None)):
         assert back(**bad) == 1 and lib.nm_last_error(), bad
     assert back(dgate=None, dx=None, dh0=None) == 0
     for sizes in ((0, 0, 0), (0, 3, 3), (3, 0, 3), (3, 3, 0)):                # sizes of zero are answered
         assert lib.nm_dense_workspace_bytes(*sizes, dtype, 0) >= 0 and lib.nm_dense_workspace_bytes(*sizes, dtype, 1) >= 0
-        assert lib.nm_scan_workspace_bytes(0, sizes[0], sizes[1], dtype, 0, 1) >= 0 and lib.nm_scan_keep_elems(0, sizes[0], sizes[1], dtype, 0) >= 0
-    assert lib.nm_dense_workspace_bytes(-1, 1, 1, dtype, 0) == -1 and lib.nm_scan_workspace_bytes(5, 2, 1, dtype, 0, 0) == -1 and lib.nm_scan_keep_elems(5, 2, 1, dtype, 0) == -1
+        assert lib.nm_scan_workspace_bytes(0, sizes[0], sizes[1], dtype, 0, 1) >= 0 and lib.nm_scan_keep_elems(0, sizes[0], sizes[1], dtype, 0, 0) >= 0
+    assert lib.nm_dense_workspace_bytes(-1, 1, 1, dtype, 0) == -1 and lib.nm_scan_workspace_bytes(5, 2, 1, dtype, 0, 0) == -1 and lib.nm_scan_keep_elems(5, 2, 1, dtype, 0, 0) == -1
 
 
 def test_workspaces_cover_every_subset_of_gradients():
