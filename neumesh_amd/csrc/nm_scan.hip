@@ -33,6 +33,7 @@ struct NmScanArgs {
     void* states;                        // [L, D] or NULL
     float* last;                         // [S, D]
     float* keep; int keep_steps;         // states before every keep_steps-th step, [chunks][pieces][D] counted from a range's start, or (keep_seq)
+    int pieces;                          // kept states per range or sequence
     int keep_seq;                        // [S][pieces][D] from a sequence's start, in the order of the recurrence; or NULL
     float* map_a; float* map_h; int* map_f;     // [chunks, D] x 2, [chunks]
     const float* carry;                  // [chunks, D] or NULL
@@ -254,37 +255,55 @@ struct NmSteps {
     unsigned first, final, none;
     int n, q;                            // n: steps of this thread; q, pos: sequence of step 0 in the order of the recurrence, and its place in it
     unsigned pos;                        // (equal lengths)
+    int q_first, q_final;                // sequence of the first bit of first / final whose step belongs to one
 };
+// packed: the sequences of a thread's steps and of its neighbours.  Asked for before the operands, so that start values can be asked for while those come
+template <int SEG> struct NmSeqs { NmVec<NM_F32, 1> v[SEG]; int prev, next; };      // (bits of the sequence numbers)
 
 template <int SEG>
-__device__ __forceinline__ NmSteps nm_s_steps(const NmScanArgs& p, const NmPlace& at, long long c0, long long c1, long long i0, unsigned pos0, long long q0) {
+__device__ __forceinline__ void nm_s_seqs(const NmScanArgs& p, const NmPlace& at, int n, long long i0, NmSeqs<SEG>& w) {
+    w.prev = w.next = -2;
+#pragma unroll
+    for (int s = 0; s < SEG; ++s) w.v[s] = {};
+    if (!p.seg || n == 0) return;
+    nm_s_load_whole<NM_F32, 1, SEG>((const float*)p.seg, at, n, w.v);
+    if (i0 > 0) w.prev = p.seg[p.reverse ? p.L - i0 : i0 - 1];
+    if (i0 + n < p.L) w.next = p.seg[p.reverse ? p.L - 1 - (i0 + n) : i0 + n];
+}
+
+template <int SEG>
+__device__ __forceinline__ NmSteps nm_s_steps(const NmScanArgs& p, const NmSeqs<SEG>& w, int n, unsigned off, int q0) {
     NmSteps t;
     t.first = t.final = t.none = 0u;
-    t.n = c1 - i0 >= SEG ? SEG : c1 > i0 ? (int)(c1 - i0) : 0;
-    t.q = 0;
+    t.n = n;
+    t.q = t.q_first = t.q_final = 0;
     t.pos = 0;
     if (p.seg) {
-        if (t.n == 0) return t;
-        NmVec<NM_F32, 1> v[SEG];         // (bits of the sequence numbers)
-        nm_s_load_whole<NM_F32, 1, SEG>((const float*)p.seg, at, t.n, v);
-        int prev = -2, next = -2;
-        if (i0 > 0) prev = p.seg[p.reverse ? p.L - i0 : i0 - 1];
-        if (i0 + t.n < p.L) next = p.seg[p.reverse ? p.L - 1 - (i0 + t.n) : i0 + t.n];
+        if (n == 0) return t;
+        int prev = w.prev;
 #pragma unroll
         for (int s = 0; s < SEG; ++s) {
-            if (s >= t.n) continue;
-            const int q = __float_as_int(v[s].e[0]), after = s + 1 < t.n ? __float_as_int(v[s + 1 < SEG ? s + 1 : s].e[0]) : next;
-            if (prev != q || q < 0) t.first |= 1u << s;
-            if (after != q || q < 0) t.final |= 1u << s;
+            if (s >= n) continue;
+            const int q = __float_as_int(w.v[s].e[0]), after = s + 1 < n ? __float_as_int(w.v[s + 1 < SEG ? s + 1 : s].e[0]) : w.next;
+            if (prev != q || q < 0) {
+                if (!(t.first & ~t.none)) t.q_first = q;
+                t.first |= 1u << s;
+            }
+            if (after != q || q < 0) {
+                if (!(t.final & ~t.none)) t.q_final = q;
+                t.final |= 1u << s;
+            }
             if (q < 0) t.none |= 1u << s;
             prev = q;
         }
         return t;
     }
-    const unsigned valid = (1u << t.n) - 1u;
-    const unsigned off = (unsigned)(i0 - c0) + pos0, q = off / p.T, pos = off - q * p.T;
-    t.q = (int)(q0 + q);
+    const unsigned valid = (1u << n) - 1u;
+    const unsigned q = off / p.T, pos = off - q * p.T;       // off: steps since the start of sequence q0
+    t.q = q0 + (int)q;
     t.pos = pos;
+    t.q_final = p.reverse ? (int)p.S - 1 - t.q : t.q;
+    t.q_first = t.q_final + (pos == 0 ? 0 : p.reverse ? -1 : 1);
     if (p.T >= SEG) {                    // one border at most
         const unsigned k = p.T - pos;    // steps up to it
         t.first = (pos == 0 ? 1u : 0u) | (k < SEG ? 1u << k : 0u);
@@ -303,21 +322,34 @@ __device__ __forceinline__ NmSteps nm_s_steps(const NmScanArgs& p, const NmPlace
     t.final &= valid;
     return t;
 }
-// sequence of step s (at borders only)
-__device__ __forceinline__ long long nm_s_sequence(const NmScanArgs& p, const NmSteps& t, long long i0, int s) {
+// sequence of step s, which is a bit of `border` (first or final); `q`: that of the first such bit.  Threads with more of them look the others up.
+__device__ __forceinline__ long long nm_s_sequence(const NmScanArgs& p, const NmSteps& t, unsigned border, int q, long long i0, int s) {
+    if (!(border & ~t.none & ((1u << s) - 1u))) return q;
     if (p.seg) return p.seg[p.reverse ? p.L - 1 - (i0 + s) : i0 + s];
     const int b = t.q + __popc(t.first & ((2u << s) - 2u));
     return p.reverse ? p.S - 1 - b : b;
 }
 
-// where bit s of `border` is set: the value with which the sequence of step s starts (src [S, D], NULL: 0) instead of v
+// the value (src [S, D], NULL: 0) with which the sequence of a thread's first border starts
 template <int VEC>
-__device__ __forceinline__ void nm_s_enter(const NmScanArgs& p, const float* src, const NmSteps& t, unsigned border, long long i0, int s, int ch, float (&v)[VEC]) {
-    const bool at = (border >> s) & 1;
+__device__ __forceinline__ void nm_s_start(const NmScanArgs& p, const float* src, const NmSteps& t, unsigned border, int q, int ch, float (&v)[VEC]) {
 #pragma unroll
-    for (int k = 0; k < VEC; ++k) v[k] = at ? 0.f : v[k];
-    if (src && at && !((t.none >> s) & 1)) {
-        const float* from = src + nm_s_sequence(p, t, i0, s) * p.D + ch;
+    for (int k = 0; k < VEC; ++k) v[k] = 0.f;
+    if (src && (border & ~t.none)) {
+        const NmVec<NM_F32, VEC> f = nm_s_load<NM_F32, VEC>(src + (long long)q * p.D + ch);
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) v[k] = f.e[k];
+    }
+}
+// where bit s of `border` is set: the start value instead of v
+template <int VEC>
+__device__ __forceinline__ void nm_s_enter(const NmScanArgs& p, const float* src, const NmSteps& t, unsigned border, int q, const float (&start)[VEC], long long i0, int s, int ch,
+                                           float (&v)[VEC]) {
+    const unsigned bit = 1u << s, own = border & ~t.none;
+#pragma unroll
+    for (int k = 0; k < VEC; ++k) v[k] = border & bit ? (t.none & bit ? 0.f : start[k]) : v[k];
+    if (src && (own & bit) && (own & (bit - 1u))) {          // a later border of the same thread
+        const float* from = src + nm_s_sequence(p, t, border, q, i0, s) * p.D + ch;
 #pragma unroll
         for (int k = 0; k < VEC; ++k) v[k] = from[k];
     }
@@ -346,6 +378,18 @@ __device__ __forceinline__ void nm_s_pad(NmVec<DG, AV> (&g)[SEG], int n, int ble
         for (int k = 0; k < AV; ++k) g[s].e[k] = s < n ? g[s].e[k] : nm_from_float<DG>(blend ? 0.f : 1.f);
 }
 
+// Operands between two passes over them: what the first pass derived from them (factors, converted values) is not to wait in registers for the second one.
+template <typename T, int SEG>
+__device__ __forceinline__ void nm_s_forget(T (&v)[SEG]) {
+    constexpr int N = (int)sizeof(v) / 4;
+    static_assert(sizeof(v) % 4 == 0, "whole registers");
+    unsigned w[N];
+    __builtin_memcpy(w, &v, sizeof(v));
+#pragma unroll
+    for (int i = 0; i < N; ++i) asm volatile("" : "+v"(w[i]));
+    __builtin_memcpy(&v, w, sizeof(v));
+}
+
 #define NM_S_THREADS 256
 // Steps of a thread.  Forward: as many as 32 .. 64 registers of operands allow (the scan's own instructions are per thread; with 4 steps they bound
 // short sequences at 2.4 TB/s).  Backward: three operands and the recomputed states.
@@ -365,14 +409,14 @@ __global__ __launch_bounds__(NM_S_THREADS) void nm_scan_forward_kernel(NmScanArg
     __shared__ uint4 lds_g[WHOLE ? 256 * NmStage<DG, AV, SEG>::STRIDE : 1], lds_x[WHOLE ? 256 * NmStage<DX, VEC, SEG>::STRIDE : 1];
     const int t = threadIdx.x, lane = t & 63, wave = t >> 6, cl = 1 << p.cl_log2, cx = t & (cl - 1), tl = t >> p.cl_log2;
     const int tile = (NM_S_THREADS >> p.cl_log2) * SEG;
-    const long long c = blockIdx.x / p.blocks;
-    const int blk = (int)(blockIdx.x % p.blocks);
+    const unsigned blk_c = blockIdx.x / (unsigned)p.blocks;
+    const long long c = blk_c;
+    const int blk = (int)(blockIdx.x - blk_c * (unsigned)p.blocks);
     const long long c0 = c * p.chunk, c1 = c0 + p.chunk < p.L ? c0 + p.chunk : p.L;
     // (channels that would end beyond D are the last VEC: computed twice, written twice with the same value)
     int ch = (blk * cl + cx) * VEC;
     if (ch + VEC > p.D) ch = p.D - VEC;
-    const long long q0 = p.seg ? 0 : c0 / p.T;
-    const unsigned pos0 = p.seg ? 0u : (unsigned)(c0 - q0 * p.T);
+    const unsigned q0 = p.seg ? 0u : (unsigned)c0 / p.T, pos0 = (unsigned)c0 - q0 * p.T;      // (L < 2^31)
 
     NmMap<VEC, AV> total;                // MAP: everything before the current tile
     float state[VEC];                    // otherwise: the state before the current tile
@@ -381,7 +425,7 @@ __global__ __launch_bounds__(NM_S_THREADS) void nm_scan_forward_kernel(NmScanArg
     for (int k = 0; k < VEC; ++k) state[k] = !MAP && p.carry ? p.carry[c * p.D + ch + k] : 0.f;
     long long b0 = c0;
     if constexpr (MAP) {                 // what comes before the range's last sequence start does not matter
-        const long long s0 = p.seg ? nm_scan_reduce_from(p.cu, p.seg[p.reverse ? p.L - c1 : c1 - 1], p.reverse, p.L, c0, c1) : (c1 - 1) / p.T * p.T;
+        const long long s0 = p.seg ? nm_scan_reduce_from(p.cu, p.seg[p.reverse ? p.L - c1 : c1 - 1], p.reverse, p.L, c0, c1) : (long long)((unsigned)(c1 - 1) / p.T * p.T);
         if (s0 > c0) b0 = s0;
     }
     int buf = 0;
@@ -391,6 +435,8 @@ __global__ __launch_bounds__(NM_S_THREADS) void nm_scan_forward_kernel(NmScanArg
         const int n = c1 - i0 >= SEG ? SEG : c1 > i0 ? (int)(c1 - i0) : 0;
         NmVec<DX, VEC> xv[SEG];
         NmVec<DG, AV> gv[SEG];
+        NmSeqs<SEG> sq;
+        nm_s_seqs(p, at, n, i0, sq);
         if constexpr (WHOLE) {
             __syncthreads();             // (everybody has read the tile before)
             nm_s_stage<DG, AV, SEG>((const TG*)p.gate, b, p.L, p.reverse, lds_g, t);
@@ -403,7 +449,7 @@ __global__ __launch_bounds__(NM_S_THREADS) void nm_scan_forward_kernel(NmScanArg
             else nm_s_load_steps<DG, AV, SEG>((const TG*)p.gate, at, p.D, ch, n, gv);
             nm_s_load_steps<DX, VEC, SEG>((const TX*)p.x, at, p.D, ch, n, xv);
         }
-        const NmSteps st = nm_s_steps<SEG>(p, at, c0, c1, i0, pos0, q0);
+        const NmSteps st = nm_s_steps<SEG>(p, sq, n, (unsigned)(i0 - c0) + pos0, (int)q0);
         if (p.seg && __any(st.none != 0)) {                  // rows of no sequence: operands of 0 keep their states and gradients 0
 #pragma unroll
             for (int s = 0; s < SEG; ++s)
@@ -420,9 +466,11 @@ __global__ __launch_bounds__(NM_S_THREADS) void nm_scan_forward_kernel(NmScanArg
                     if (s >= n) xv[s] = {};
             }
         }
+        float start[VEC];
+        nm_s_start(p, p.h0, st, st.first, st.q_first, ch, start);
         // one step: state h -> r h + u
         auto advance = [&](int s, float (&h)[VEC]) {
-            nm_s_enter(p, p.h0, st, st.first, i0, s, ch, h);
+            nm_s_enter(p, p.h0, st, st.first, st.q_first, start, i0, s, ch, h);
             nm_s_step<DX, DG, VEC, AV>(gv[s], xv[s], p.blend, h);
         };
         NmMap<VEC, AV> m, before;
@@ -450,11 +498,15 @@ __global__ __launch_bounds__(NM_S_THREADS) void nm_scan_forward_kernel(NmScanArg
                     if (w == wave) h[k] = state[k];
                 nm_s_apply(mw, state);
             }
+            __builtin_amdgcn_sched_barrier(0);               // (one wave's map in registers at a time)
         }
         if constexpr (!MAP) {
+            nm_s_forget(gv);
+            nm_s_forget(xv);
+            nm_s_forget(start);
             nm_s_apply(before, h);
             if (p.keep && !p.keep_seq && n > 0 && ((unsigned)(i0 - c0) & (unsigned)(p.keep_steps - 1)) == 0) {
-                float* dst = p.keep + (c * ((p.chunk + p.keep_steps - 1) / p.keep_steps) + (i0 - c0) / p.keep_steps) * p.D + ch;
+                float* dst = p.keep + (c * p.pieces + (unsigned)(i0 - c0) / (unsigned)p.keep_steps) * p.D + ch;
 #pragma unroll
                 for (int k = 0; k < VEC; ++k) dst[k] = h[k];
             }
@@ -466,7 +518,7 @@ __global__ __launch_bounds__(NM_S_THREADS) void nm_scan_forward_kernel(NmScanArg
                     if (p.keep_seq && s < n) {               // (sequences longer than keep_steps: one border in these steps at most)
                         const unsigned left = p.T - st.pos, at_s = (unsigned)s < left ? st.pos + s : s - left;
                         if (at_s > 0 && (at_s & (unsigned)(p.keep_steps - 1)) == 0) {
-                            const long long piece = (st.q + ((unsigned)s < left ? 0 : 1)) * (long long)((p.T + p.keep_steps - 1) / p.keep_steps) + at_s / p.keep_steps;
+                            const long long piece = (st.q + ((unsigned)s < left ? 0 : 1)) * (long long)p.pieces + at_s / (unsigned)p.keep_steps;
 #pragma unroll
                             for (int k = 0; k < VEC; ++k) p.keep[piece * p.D + ch + k] = h[k];
                         }
@@ -479,7 +531,7 @@ __global__ __launch_bounds__(NM_S_THREADS) void nm_scan_forward_kernel(NmScanArg
                         if (p.states && s < n) nm_s_store<DX, VEC>(so.at(s), h);
                     }
                     if (((st.final & ~st.none) >> s) & 1) {
-                        float* dst = p.last + nm_s_sequence(p, st, i0, s) * p.D + ch;
+                        float* dst = p.last + nm_s_sequence(p, st, st.final, st.q_final, i0, s) * p.D + ch;
 #pragma unroll
                         for (int k = 0; k < VEC; ++k) dst[k] = h[k];
                     }
@@ -510,15 +562,15 @@ __global__ __launch_bounds__(NM_S_THREADS) void nm_scan_backward_kernel(NmScanAr
     __shared__ NmShared<VEC, AV> sh_r[2], sh_h[MAP ? 1 : 2];
     const int t = threadIdx.x, lane = t & 63, wave = t >> 6, cl = 1 << p.cl_log2, cx = t & (cl - 1), tl = t >> p.cl_log2;
     const int tile = (NM_S_THREADS >> p.cl_log2) * SEG;
-    const long long c = blockIdx.x / p.blocks;
-    const int blk = (int)(blockIdx.x % p.blocks);
+    const unsigned blk_c = blockIdx.x / (unsigned)p.blocks;
+    const long long c = blk_c;
+    const int blk = (int)(blockIdx.x - blk_c * (unsigned)p.blocks);
     const long long c0 = c * p.chunk;
     long long c1 = c0 + p.chunk < p.L ? c0 + p.chunk : p.L;
     const int own = (blk * cl + cx) * VEC;                   // first channel that is this thread's own (see the forward kernel)
     int ch = own;
     if (ch + VEC > p.D) ch = p.D - VEC;
-    const long long q0 = p.seg ? 0 : c0 / p.T;
-    const unsigned pos0 = p.seg ? 0u : (unsigned)(c0 - q0 * p.T);
+    const unsigned q0 = p.seg ? 0u : (unsigned)c0 / p.T, pos0 = (unsigned)c0 - q0 * p.T;      // (L < 2^31)
 
     NmMap<VEC, AV> total;                // MAP: everything after the current tile
     float flow[VEC];                     // otherwise: f of the step after the current tile
@@ -527,21 +579,23 @@ __global__ __launch_bounds__(NM_S_THREADS) void nm_scan_backward_kernel(NmScanAr
     for (int k = 0; k < VEC; ++k) flow[k] = !MAP && p.carry ? p.carry[c * p.D + ch + k] : 0.f;
     bool cut = false;
     if constexpr (MAP) {                 // what comes after the range's first sequence end does not matter
-        const long long e = p.seg ? nm_scan_reduce_to(p.cu, p.seg[p.reverse ? p.L - 1 - c0 : c0], p.reverse, p.L, c0, c1) : c0 / p.T * p.T + p.T - 1;
+        const long long e = p.seg ? nm_scan_reduce_to(p.cu, p.seg[p.reverse ? p.L - 1 - c0 : c0], p.reverse, p.L, c0, c1) : (long long)q0 * p.T + p.T - 1;
         if (e + 1 < c1) {
             cut = true;
             c1 = e + 1;
         }
     }
-    const long long tiles = (c1 - c0 + tile - 1) / tile;
+    const int tiles = (int)((unsigned)(c1 - c0 + tile - 1) / (unsigned)tile);
     const bool want_x = !MAP && (p.dgate || p.dgate_part);
     int buf = 0;
-    for (long long j = tiles - 1; j >= 0; --j, buf ^= 1) {
-        const long long b = c0 + j * tile, i0 = b + tl * SEG;
+    for (int j = tiles - 1; j >= 0; --j, buf ^= 1) {
+        const long long b = c0 + (long long)j * tile, i0 = b + tl * SEG;
         const NmPlace at = {p.reverse ? p.L - b - tile : b, (unsigned)(p.reverse ? tile - 1 - tl * SEG : tl * SEG), p.reverse};
         const int n = c1 - i0 >= SEG ? SEG : c1 > i0 ? (int)(c1 - i0) : 0;
         NmVec<DX, VEC> xv[SEG], cv[SEG];
         NmVec<DG, AV> gv[SEG];
+        NmSeqs<SEG> sq;
+        nm_s_seqs(p, at, n, i0, sq);
 #pragma unroll
         for (int s = 0; s < SEG; ++s) {
             xv[s] = {};
@@ -556,7 +610,7 @@ __global__ __launch_bounds__(NM_S_THREADS) void nm_scan_backward_kernel(NmScanAr
             if (p.g) nm_s_load_steps<DX, VEC, SEG>((const TX*)p.g, at, p.D, ch, n, cv);
             if (want_x) nm_s_load_steps<DX, VEC, SEG>((const TX*)p.x, at, p.D, ch, n, xv);
         }
-        const NmSteps st = nm_s_steps<SEG>(p, at, c0, c1, i0, pos0, q0);
+        const NmSteps st = nm_s_steps<SEG>(p, sq, n, (unsigned)(i0 - c0) + pos0, (int)q0);
         if (p.seg && __any(st.none != 0)) {                  // rows of no sequence: operands of 0 keep their states and gradients 0
 #pragma unroll
             for (int s = 0; s < SEG; ++s)
@@ -566,11 +620,14 @@ __global__ __launch_bounds__(NM_S_THREADS) void nm_scan_backward_kernel(NmScanAr
                     cv[s] = {};
                 }
         }
-        auto enter = [&](int s, float (&h)[VEC]) { nm_s_enter(p, p.h0, st, st.first, i0, s, ch, h); };
+        float start[VEC], end[VEC];
+        nm_s_start(p, want_x ? p.h0 : nullptr, st, st.first, st.q_first, ch, start);
+        nm_s_start(p, p.g_last, st, st.final, st.q_final, ch, end);
+        auto enter = [&](int s, float (&h)[VEC]) { nm_s_enter(p, p.h0, st, st.first, st.q_first, start, i0, s, ch, h); };
         if (n < SEG) nm_s_pad<DG, AV, SEG>(gv, n, p.blend);
         auto advance = [&](int s, float (&h)[VEC]) { nm_s_step<DX, DG, VEC, AV>(gv[s], xv[s], p.blend, h); };
         auto retreat = [&](int s, float (&f)[VEC], float (&lam)[VEC]) {     // f of the step after s -> lambda and f of s
-            nm_s_enter(p, p.g_last, st, st.final, i0, s, ch, f);
+            nm_s_enter(p, p.g_last, st, st.final, st.q_final, end, i0, s, ch, f);
 #pragma unroll
             for (int k = 0; k < VEC; ++k) {
                 lam[k] = nm_to_float<DX>(cv[s].e[k]) + f[k];
@@ -593,6 +650,10 @@ __global__ __launch_bounds__(NM_S_THREADS) void nm_scan_backward_kernel(NmScanAr
         for (int k = 0; k < AV; ++k) mr.a[k] = mf.a[k];
         mf.f = st.first ? 1 : 0;
         mr.f = st.final ? 1 : 0;
+        if (want_x) {
+            nm_s_wave_scan<VEC, AV, 1>(mf, bf, lane, cl);
+            if (lane >= 64 - cl) nm_s_put(sh_h[MAP ? 0 : buf], wave, cx, mf);
+        }
 #pragma unroll
         for (int s = SEG - 1; s >= 0; --s) {
             float lam[VEC];
@@ -600,10 +661,6 @@ __global__ __launch_bounds__(NM_S_THREADS) void nm_scan_backward_kernel(NmScanAr
         }
         nm_s_wave_scan<VEC, AV, -1>(mr, br, lane, cl);
         if (lane < cl) nm_s_put(sh_r[buf], wave, cx, mr);
-        if (want_x) {
-            nm_s_wave_scan<VEC, AV, 1>(mf, bf, lane, cl);
-            if (lane >= 64 - cl) nm_s_put(sh_h[MAP ? 0 : buf], wave, cx, mf);
-        }
         __syncthreads();
         float f[VEC];
 #pragma unroll
@@ -618,19 +675,26 @@ __global__ __launch_bounds__(NM_S_THREADS) void nm_scan_backward_kernel(NmScanAr
                     if (w == wave) f[k] = flow[k];
                 nm_s_apply(mw, flow);
             }
+            __builtin_amdgcn_sched_barrier(0);               // (one wave's map in registers at a time)
         }
         if constexpr (!MAP) {
+            nm_s_forget(gv);
+            nm_s_forget(xv);
+            nm_s_forget(cv);
+            nm_s_forget(start);
+            nm_s_forget(end);
             nm_s_apply(br, f);
             float hp[SEG][VEC];          // states before the steps, then the gradient of the gate
             if (want_x) {
                 float h[VEC];
 #pragma unroll
-                for (int k = 0; k < VEC; ++k) h[k] = p.keep ? p.keep[(c * ((p.chunk + tile - 1) / tile) + j) * p.D + ch + k] : 0.f;
+                for (int k = 0; k < VEC; ++k) h[k] = p.keep ? p.keep[(c * p.pieces + j) * p.D + ch + k] : 0.f;
 #pragma unroll
                 for (int w = 0; w < 3; ++w) {
                     NmMap<VEC, AV> mw;
                     nm_s_get(sh_h[buf], w, cx, mw);
                     if (w < wave) nm_s_apply(mw, h);
+                    __builtin_amdgcn_sched_barrier(0);
                 }
                 nm_s_apply(bf, h);
 #pragma unroll
@@ -663,7 +727,7 @@ __global__ __launch_bounds__(NM_S_THREADS) void nm_scan_backward_kernel(NmScanAr
                         if (s < n) nm_s_store<DG, VEC>(rg.at(s), hp[s]);
                 }
                 if (p.dh0 && (((st.first & ~st.none) >> s) & 1)) {
-                    float* dst = p.dh0 + nm_s_sequence(p, st, i0, s) * p.D + ch;
+                    float* dst = p.dh0 + nm_s_sequence(p, st, st.first, st.q_first, i0, s) * p.D + ch;
 #pragma unroll
                     for (int k = 0; k < VEC; ++k) dst[k] = f[k];
                 }
@@ -889,6 +953,7 @@ static void nm_s_fill(NmScanArgs& a, const NmScanPlan& pl, const NmScanShape& sh
     a.L = L; a.S = S; a.chunk = &shape == &pl.f ? pl.chunk_f : pl.chunk_b; a.T = cu || S == 0 ? 1u : (unsigned)(L / S); a.D = (int)D;
     a.reverse = reverse ? 1 : 0; a.blend = blend ? 1 : 0; a.cl_log2 = shape.cl_log2; a.blocks = shape.blocks;
     a.keep_steps = pl.b.tile;
+    a.pieces = (int)nm_s_up(pl.chunk_b, pl.b.tile);
     if (pl.split) {
         a.map_a = (float*)(ws + pl.off_a); a.map_h = (float*)(ws + pl.off_h); a.map_f = (int*)(ws + pl.off_f);
     }
