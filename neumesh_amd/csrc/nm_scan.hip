@@ -766,31 +766,40 @@ __global__ __launch_bounds__(NM_S_THREADS) void nm_scan_backward_kernel(NmScanAr
     }
 }
 
-// maps of the ranges -> the state before every range (DIR = 1), or the flow after it (-1).  8 channels x 32 lanes in time, 16 ranges each.
+// maps of the ranges -> the state before every range (DIR = 1), or the flow after it (-1).  8 channels x 128 lanes in time, 16 ranges each: one round for
+// all the ranges of a launch (nm_s_plan makes some NM_S_FILL_PACKED at most, so that offsets stay far below 2^32), for what a round costs is its latency.
+#define NM_S_CARRY 1024
 template <int DIR>
-__global__ __launch_bounds__(NM_S_THREADS) void nm_scan_carry_kernel(const float* __restrict__ map_a, const float* __restrict__ map_h, const int* __restrict__ map_f, long long n,
-                                                                     int D, float* __restrict__ carry) {
-    __shared__ float sh_a[2][4][8], sh_h[2][4][8];
-    __shared__ int sh_f[2][4];
+__global__ __launch_bounds__(NM_S_CARRY) void nm_scan_carry_kernel(const float* __restrict__ map_a, const float* __restrict__ map_h, const int* __restrict__ map_f, int n, int D,
+                                                                   float* __restrict__ carry) {
+    constexpr int WAVES = NM_S_CARRY / 64;
+    __shared__ float sh_a[2][WAVES][8], sh_h[2][WAVES][8];
+    __shared__ int sh_f[2][WAVES];
     const int t = threadIdx.x, lane = t & 63, wave = t >> 6, cx = t & 7, tl = t >> 3;
-    int ch = blockIdx.x * 8 + cx;
-    if (ch >= D) ch = D - 1;
+    unsigned ch = blockIdx.x * 8u + cx;
+    if (ch >= (unsigned)D) ch = D - 1;
     float state = 0.f;
     int buf = 0;
-    for (long long b = 0; b < n; b += 512, buf ^= 1) {
-        NmMap<1, 1> m, before, v[16];
-        m.a[0] = 1.f; m.h[0] = 0.f; m.f = 0;
+    for (int b = 0; b < n; b += NM_S_CARRY * 2, buf ^= 1) {
+        const int i0 = b + tl * 16;
+        float a[16], h[16];
+        unsigned fresh = 0u;
 #pragma unroll
         for (int s = 0; s < 16; ++s) {
-            const long long i = b + tl * 16 + s, c = DIR > 0 ? i : n - 1 - i;
-            v[s].a[0] = 1.f; v[s].h[0] = 0.f; v[s].f = 0;
-            if (i < n) { v[s].a[0] = map_a[c * D + ch]; v[s].h[0] = map_h[c * D + ch]; v[s].f = map_f[c]; }
+            const bool in = i0 + s < n;
+            const unsigned c = in ? (unsigned)(DIR > 0 ? i0 + s : n - 1 - i0 - s) : 0u;
+            a[s] = in ? map_a[c * (unsigned)D + ch] : 1.f;
+            h[s] = in ? map_h[c * (unsigned)D + ch] : 0.f;
+            if (in && map_f[c]) fresh |= 1u << s;
         }
+        auto step = [&](int s, float& v) { v = (fresh >> s) & 1 ? h[s] : fmaf(a[s], v, h[s]); };
+        NmMap<1, 1> m, before;
+        nm_s_identity(m);
+        m.f = fresh ? 1 : 0;
 #pragma unroll
         for (int s = 0; s < 16; ++s) {
-            nm_s_apply(v[s], m.h);
-            m.a[0] *= v[s].a[0];
-            m.f |= v[s].f;
+            step(s, m.h[0]);
+            m.a[0] *= a[s];
         }
         nm_s_wave_scan<1, 1, 1>(m, before, lane, 8);
         if (lane >= 56) {
@@ -799,21 +808,20 @@ __global__ __launch_bounds__(NM_S_THREADS) void nm_scan_carry_kernel(const float
             if (lane == 63) sh_f[buf][wave] = m.f;
         }
         __syncthreads();
-        float h[1] = {0.f}, all[1] = {state};
-#pragma unroll
-        for (int w = 0; w < 4; ++w) {
-            if (w == wave) h[0] = all[0];
+        float v[1] = {0.f}, all[1] = {state};
+#pragma unroll 4
+        for (int w = 0; w < WAVES; ++w) {
+            if (w == wave) v[0] = all[0];
             NmMap<1, 1> mw;
             mw.a[0] = sh_a[buf][w][cx]; mw.h[0] = sh_h[buf][w][cx]; mw.f = sh_f[buf][w];
             nm_s_apply(mw, all);
         }
         state = all[0];
-        nm_s_apply(before, h);
+        nm_s_apply(before, v);
 #pragma unroll
         for (int s = 0; s < 16; ++s) {
-            const long long i = b + tl * 16 + s, c = DIR > 0 ? i : n - 1 - i;
-            if (i < n) carry[c * D + ch] = h[0];
-            nm_s_apply(v[s], h);
+            if (i0 + s < n) carry[(unsigned)(DIR > 0 ? i0 + s : n - 1 - i0 - s) * (unsigned)D + ch] = v[0];
+            step(s, v[0]);
         }
     }
 }
@@ -859,7 +867,11 @@ struct NmScanPlan {
     size_t off_seg, off_a, off_h, off_f, off_carry, off_part, bytes;
 };
 
-#define NM_S_FILL 1024       // workgroups that fill the chip
+// Workgroups of a launch over ranges that cut sequences.  Packed ones twice as many: their maps end at the first border, so that more ranges cost them
+// little, and the longest waits less for its tiles (8192 sequences of 96 steps x 32 channels fp32, backward: 117 us instead of 138).  Equal lengths read all
+// operands for the maps either way (4 x 16384 x 512 bf16: 69 us for maps and states with either number).
+#define NM_S_FILL 1024
+#define NM_S_FILL_PACKED 2048
 
 static NmScanShape nm_s_shape(int D, int vec, int seg) {
     NmScanShape s;
@@ -885,7 +897,7 @@ static NmScanPlan nm_s_plan(long long L, long long S, int D, int dtype, bool sha
     const long long T = packed || S == 0 ? 0 : L / S;
     p.split = packed || (T > tile && S * blocks < NM_S_FILL / 2);
     if (p.split) {
-        p.chunk_f = p.chunk_b = nm_s_up(nm_s_up(L, tile) * blocks, NM_S_FILL) * tile;
+        p.chunk_f = p.chunk_b = nm_s_up(nm_s_up(L, tile) * blocks, packed ? NM_S_FILL_PACKED : NM_S_FILL) * tile;
         p.keep_elems = nm_s_up(L, p.chunk_b) * (p.chunk_b / p.b.tile) * D;
         if (p.chunk_f >= L) p.split = false;                 // (one range)
         p.keep_seq = false;
@@ -1003,7 +1015,7 @@ int nm_scan_forward(const void* gate, int gate_dtype, int shared_gate, const voi
     if (pl.split) {
         float* carry = (float*)(ws + pl.off_carry);
         NM_S_PICK(nm_scan_forward_kernel, true, true);
-        hipLaunchKernelGGL(nm_scan_carry_kernel<1>, dim3((unsigned)nm_s_up(D, 8)), dim3(NM_S_THREADS), 0, stream, a.map_a, a.map_h, a.map_f, pl.chunks_f, (int)D, carry);
+        hipLaunchKernelGGL(nm_scan_carry_kernel<1>, dim3((unsigned)nm_s_up(D, 8)), dim3(NM_S_CARRY), 0, stream, a.map_a, a.map_h, a.map_f, (int)pl.chunks_f, (int)D, carry);
         a.carry = carry;
     }
     NM_S_PICK(nm_scan_forward_kernel, false, true);
@@ -1044,7 +1056,7 @@ int nm_scan_backward(const void* gate, int gate_dtype, int shared_gate, const vo
     if (pl.split) {
         float* carry = (float*)(ws + pl.off_carry);
         NM_S_PICK(nm_scan_backward_kernel, true, false);
-        hipLaunchKernelGGL(nm_scan_carry_kernel<-1>, dim3((unsigned)nm_s_up(D, 8)), dim3(NM_S_THREADS), 0, stream, a.map_a, a.map_h, a.map_f, pl.chunks_b, (int)D, carry);
+        hipLaunchKernelGGL(nm_scan_carry_kernel<-1>, dim3((unsigned)nm_s_up(D, 8)), dim3(NM_S_CARRY), 0, stream, a.map_a, a.map_h, a.map_f, (int)pl.chunks_b, (int)D, carry);
         a.carry = carry;
     }
     NM_S_PICK(nm_scan_backward_kernel, false, false);
