@@ -71,7 +71,7 @@ __device__ __forceinline__ float nm_d_log1p(float e) {
 // values z -> act(z) in place, derivatives -> d.  sigmoid, SiLU and GELU are one form, z or 1 times sigmoid(c1 z + c3 z^3); the tests are on the
 // launch's activation, once per group.
 template <bool F32, int N>
-__device__ __forceinline__ void nm_d_act(int act, float beta, float ibeta, float (&z)[N], float (&d)[N]) {
+__device__ __forceinline__ void nm_d_act(int act, float beta, float ibeta, bool want, float (&z)[N], float (&d)[N]) {
     if (act == NM_ACT_NONE) {
 #pragma unroll
         for (int i = 0; i < N; ++i) d[i] = 1.f;
@@ -84,9 +84,12 @@ __device__ __forceinline__ void nm_d_act(int act, float beta, float ibeta, float
     } else if (act == NM_ACT_SOFTPLUS) {
 #pragma unroll
         for (int i = 0; i < N; ++i) {
-            const float u = beta * z[i], e = nm_d_exp<F32>(-fabsf(u)), r = nm_d_rcp<F32>(1.0f + e);
+            const float u = beta * z[i], e = nm_d_exp<F32>(-fabsf(u));
             z[i] = fmaf(nm_d_log1p<F32>(e), ibeta, fmaxf(z[i], 0.f));
-            d[i] = u >= 0.f ? r : e * r;
+            if (want) {
+                const float r = nm_d_rcp<F32>(1.0f + e);
+                d[i] = u >= 0.f ? r : e * r;
+            }
         }
     } else {
         const float c1 = act == NM_ACT_GELU_TANH ? 1.59576912160573071f : 1.0f;      // 2 sqrt(2 / pi)
@@ -98,7 +101,7 @@ __device__ __forceinline__ void nm_d_act(int act, float beta, float ibeta, float
             const float u = c1 * t * fmaf(c3, t2, 1.0f);
             const float e = nm_d_exp<F32>(-fabsf(u)), r = nm_d_rcp<F32>(1.0f + e), er = e * r;
             const float q = z[i] != z[i] ? z[i] : u >= 0.f ? r : er, q1 = u >= 0.f ? er : r;
-            d[i] = gate_only ? q * q1 : fmaf(t * q, q1 * (c1 * fmaf(3.0f * c3, t2, 1.0f)), q);
+            if (want) d[i] = gate_only ? q * q1 : fmaf(t * q, q1 * (c1 * fmaf(3.0f * c3, t2, 1.0f)), q);
             z[i] = gate_only ? q : z[i] * q;
         }
     }
@@ -356,7 +359,7 @@ __device__ __forceinline__ void nm_d_epilogue(const NmDenseArgs& p, const nm_v4f
             nm_oct_to_float<DT>(rs[k % AHEAD], q);
             fetch(k + AHEAD);
         }
-        if constexpr (!PROD) nm_d_act<DT == NM_F32>(p.act, p.beta, ibeta, z, dv);
+        if constexpr (!PROD) nm_d_act<DT == NM_F32>(p.act, p.beta, ibeta, p.DV != nullptr, z, dv);
         if (m >= p.R) continue;
         if constexpr (!PROD) {
             if (p.DV) nm_d_store_cols<DD>((typename NmType<DD>::elem*)p.DV + m * p.C, dv, c, p.C);
@@ -539,6 +542,87 @@ __global__ __launch_bounds__(512, 2) void nm_dense_resident_kernel(NmDenseArgs p
     }
 }
 
+// Large 16-bit layers in W's own layout: 256 rows x 256 columns per workgroup of eight waves (128 x 64 each).  Both operands come in panels of 64
+// contraction elements as whole 128-byte lines, eight lanes a line -- read straight into fragments, sixteen rows side by side, the rows of a
+// 16384 x 1024 -> 1024 layer kept the address units busy for 72 % of 93 us -- and go through LDS, in two buffers, with one barrier per panel and the
+// next panel in flight in registers.  The eight 16-byte pieces of an LDS row are exchanged by the row's number, so that the sixteen rows of a fragment
+// lie in different banks.
+template <int DT>
+__global__ __launch_bounds__(512, 2) void nm_dense_tile_kernel(NmDenseArgs p) {
+    typedef typename NmType<DT>::elem T;
+    __shared__ uint4 lds[2][2][256 * 8];                     // [buffer][rows, columns][row][piece]
+    __shared__ float bias[256];
+    const int t = threadIdx.x, lane = t & 63, wave = t >> 6, li = lane & 15, h = lane >> 4, wr = wave >> 2, wc = wave & 3;
+    const unsigned id = blockIdx.x, turn = id >> 3;          // (XCDs: see above)
+    const long long rb = (long long)(turn / p.col_blocks) * 8 + (id & 7);
+    const int cb = (int)(turn % p.col_blocks);
+    if (rb * 256 >= p.R) return;
+    const int panels = (p.Q + 63) / 64, piece = t & 7;
+    // this thread's pieces: rows t / 8 + 64 i of both sides (LDS row n of the columns' side: the column that nm_d_column puts there)
+    const T* src[2][4];
+    int dst[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int n = (t >> 3) + 64 * i;
+        const long long m = rb * 256 + n;
+        const int c = cb * 256 + nm_d_column<DT>(n >> 4, n & 15);
+        src[0][i] = (const T*)p.A + (m < p.R ? m : p.R - 1) * p.lda;
+        src[1][i] = (const T*)p.W + (long long)(c < p.C ? c : p.C - 1) * p.ldw;
+        dst[i] = n * 8 + (piece ^ ((n >> 1) & 7));
+    }
+    NmOct<DT> v[2][4];
+    auto load = [&](int panel) {
+#pragma unroll
+        for (int o = 0; o < 2; ++o)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v[o][i] = nm_d_fetch<DT>(src[o][i], panel * 64 + 8 * piece, p.Q);
+    };
+    auto store = [&](int panel) {
+        if ((panel + 1) * 64 > p.Q && p.Q >= 8) {            // what the last whole load repeated
+            const int q = panel * 64 + 8 * piece, sh = q + 8 <= p.Q ? 0 : q + 8 - p.Q;
+#pragma unroll
+            for (int o = 0; o < 2; ++o)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) v[o][i] = nm_oct_clear_first<DT>(v[o][i], sh < 8 ? sh : 8);
+        }
+#pragma unroll
+        for (int o = 0; o < 2; ++o)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) lds[panel & 1][o][dst[i]] = v[o][i].v[0];
+    };
+    nm_v4f acc[8][4];
+#pragma unroll
+    for (int r = 0; r < 8; ++r)
+#pragma unroll
+        for (int n = 0; n < 4; ++n) acc[r][n] = nm_v4f{0.f, 0.f, 0.f, 0.f};
+
+    if (p.bias && t < 256) bias[t] = nm_d_bias<DT>(p, cb * 256 + t);
+    load(0);
+    store(0);
+    __syncthreads();
+    const int at = li * 8 + (h ^ (li >> 1));                 // piece h of a fragment's row; the panel's second half: ^ 4
+    for (int k = 0; k < panels; ++k) {
+        // (a wave that is a panel ahead fills the OTHER buffer; nobody is two panels ahead)
+        if (k + 1 < panels) load(k + 1);
+        const uint4 *x = lds[k & 1][0] + wr * 1024, *w = lds[k & 1][1] + wc * 512;
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+            uint4 b[4][1];
+#pragma unroll
+            for (int n = 0; n < 4; ++n) b[n][0] = w[n * 128 + (at ^ (4 * s))];
+#pragma unroll
+            for (int r = 0; r < 8; ++r) {
+                uint4 a[1] = {x[r * 128 + (at ^ (4 * s))]};
+#pragma unroll
+                for (int n = 0; n < 4; ++n) acc[r][n] = nm_d_products<DT>(b[n], a, acc[r][n]);
+            }
+        }
+        if (k + 1 < panels) store(k + 1);
+        __syncthreads();
+    }
+    nm_d_epilogue<DT, false, true, 8, 2>(p, acc, bias + wc * 64, rb * 256 + wr * 128, cb * 4 + wc, lane);
+}
+
 // Otherwise: one workgroup: 4 waves, 64 RT rows x 32 NP columns, both sides streamed.  The rows as above; the column operand is shared by the four waves
 // through LDS, PS steps at a time in two buffers, one barrier per panel, both sides' next panel in flight in registers meanwhile.
 template <int DT, bool PROD, int RT, int NP, int PS>
@@ -692,7 +776,7 @@ __global__ __launch_bounds__(256) void nm_dense_few_kernel(const typename NmType
     if (n >= N || sub >= M) return;
     if (bias) z += bias_f32 ? ((const float*)bias)[n] : (float)((const T*)bias)[n];
     float hv[1] = {z}, d[1];
-    nm_d_act<DT == NM_F32>(act, beta, 1.0f / beta, hv, d);
+    nm_d_act<DT == NM_F32>(act, beta, 1.0f / beta, dv != nullptr, hv, d);
     float h = hv[0];
     if (res) h += (float)res[sub * ldr + n];
     y[sub * ldy + n] = (T)h;
@@ -991,10 +1075,12 @@ __global__ __launch_bounds__(256) void nm_dense_sum_kernel(const float* __restri
 static inline long long nm_d_up(long long a, long long b) { return (a + b - 1) / b; }
 static inline long long nm_d_align(long long b) { return nm_d_up(b, 256) * 256; }
 
-struct NmDensePlan { bool resident; int np, tiles, col_blocks, rt; long long steps, bytes; };
+struct NmDensePlan { bool resident, tile; int np, tiles, col_blocks, rt; long long steps, bytes; };
+
+#define NM_D_TILES 128   // tiles of 256 x 256 from which nm_dense_tile_kernel is taken
 
 // columns C, contraction Q, rows R: which kernel, and its column blocks of 32 np columns
-static NmDensePlan nm_d_plan(int dt, bool prod, bool res, long long R, long long C, long long Q) {
+static NmDensePlan nm_d_plan(int dt, bool prod, bool res, bool trans, long long R, long long C, long long Q) {
     NmDensePlan p;
     const int pieces = dt == NM_F32 ? 3 : 1;
     const long long steps = nm_d_up(Q, 32);
@@ -1003,6 +1089,7 @@ static NmDensePlan nm_d_plan(int dt, bool prod, bool res, long long R, long long
     if (res && fit == 8) fit = 4;                            // (the residual of eight pieces is in flight at once)
     while (fit > 0 && 2 * steps * pieces * fit > NM_D_RESIDENT) fit >>= 1;
     p.resident = fit > 0 && nm_d_up(C, 32 * fit) <= 4;
+    p.tile = !p.resident && dt != NM_F32 && !prod && !trans && nm_d_up(R, 256) * nm_d_up(C, 256) >= NM_D_TILES && 4 * C >= 3 * 256 * nm_d_up(C, 256);
     p.np = p.resident ? fit : p.np > 4 ? 4 : p.np;
     // few rows: narrower column blocks until every wave has a tile (streaming: every CU a workgroup)
     while (p.np > 1 && (p.resident ? nm_d_up(R, 32) * nm_d_up(C, 32 * p.np) < 1024 : nm_d_up(R, 128) * nm_d_up(C, 32 * p.np) < 256)) p.np >>= 1;
@@ -1012,7 +1099,8 @@ static NmDensePlan nm_d_plan(int dt, bool prod, bool res, long long R, long long
     p.tiles = (int)(nm_d_up(C, 32 * p.np) * p.np * 2);
     p.col_blocks = p.tiles / (2 * p.np);
     p.steps = p.resident ? steps : nm_d_up(steps, ps) * ps;
-    p.bytes = p.resident ? 0 : nm_d_align(p.steps * p.tiles * pieces * 1024);
+    if (p.tile) p.col_blocks = (int)nm_d_up(C, 256);
+    p.bytes = p.resident || p.tile ? 0 : nm_d_align(p.steps * p.tiles * pieces * 1024);
     return p;
 }
 
@@ -1054,10 +1142,12 @@ static int nm_d_launch(const NmDensePlan& pl, NmDenseArgs a, hipStream_t stream)
         NM_LAUNCH_CHECK();
         return 0;
     }
-    const long long groups = nm_d_up(nm_d_up(a.R, 64 * pl.rt), 8) * 8 * pl.col_blocks;
+    const long long groups = nm_d_up(nm_d_up(a.R, pl.tile ? 256 : 64 * pl.rt), 8) * 8 * pl.col_blocks;
     if (groups > 0x7fffffffLL) return nm_fail("nm_dense: %lld rows x %d columns exceed one launch", a.R, a.C);
     const dim3 grid((unsigned)groups), block(256);
-    if (pl.rt == 4) {
+    if (pl.tile) {
+        if constexpr (!F && !PROD) hipLaunchKernelGGL((nm_dense_tile_kernel<DT>), grid, dim3(512), 0, stream, a);
+    } else if (pl.rt == 4) {
         if constexpr (!F && !PROD) hipLaunchKernelGGL((nm_dense_stream_kernel<DT, PROD, 4, 4, 2>), grid, block, 0, stream, a);
     } else {
         switch (pl.np) {
@@ -1072,7 +1162,7 @@ static int nm_d_launch(const NmDensePlan& pl, NmDenseArgs a, hipStream_t stream)
 
 template <int DT>
 static int nm_d_pack(const NmDensePlan& pl, const NmDenseArgs& a, char* ws, hipStream_t stream) {
-    if (pl.resident || pl.steps == 0) return 0;
+    if (pl.resident || pl.tile || pl.steps == 0) return 0;
     hipLaunchKernelGGL((nm_dense_pack_kernel<DT>), dim3((unsigned)nm_d_up(pl.steps * pl.tiles * 64, 256)), dim3(256), 0, stream, (const typename NmType<DT>::elem*)a.W,
                        a.ldw, a.trans, a.C, a.Q, pl.tiles, (int)pl.steps, (uint4*)ws);
     NM_LAUNCH_CHECK();
@@ -1097,7 +1187,7 @@ static int nm_d_forward(const void* x, long long ldx, const void* w, long long l
         NM_LAUNCH_CHECK();
         return 0;
     }
-    const NmDensePlan pl = nm_d_plan(DT, false, res != nullptr, M, N, K);
+    const NmDensePlan pl = nm_d_plan(DT, false, res != nullptr, false, M, N, K);
     NmDenseArgs a = {};
     a.A = x; a.lda = ldx; a.W = w; a.ldw = ldw; a.P = (const uint4*)ws; a.bias = bias; a.bias_f32 = bias_dt == NM_F32;
     a.res = res; a.ldr = ldr; a.Y = y; a.ldy = ldy; a.DV = deriv; a.R = M; a.Q = K; a.C = N; a.act = act; a.beta = beta;
@@ -1110,7 +1200,7 @@ static int nm_d_backward(const void* g, long long ldg, const void* deriv, const 
                          long long lddx, void* dw, void* db, int bias_dt, char* ws, hipStream_t stream) {
     typedef typename NmType<DT>::elem T;
     if (dx) {
-        const NmDensePlan pl = nm_d_plan(DT, deriv != nullptr, false, M, K, N);
+        const NmDensePlan pl = nm_d_plan(DT, deriv != nullptr, false, true, M, K, N);
         NmDenseArgs a = {};
         a.A = g; a.lda = ldg; a.D = deriv; a.W = w; a.ldw = ldw; a.trans = 1; a.P = (const uint4*)ws; a.Y = dx; a.ldy = lddx; a.R = M; a.Q = N; a.C = K; a.act = NM_ACT_NONE; a.beta = 1.f;
         if (nm_d_pack<DT>(pl, a, ws, stream)) return 1;
@@ -1159,12 +1249,12 @@ int64_t nm_dense_workspace_bytes(int64_t M, int64_t K, int64_t N, int dtype, int
     if (nm_d_check("nm_dense_workspace_bytes", M, K, N, dtype, dtype)) return -1;
     if (!backward) {
         if (M <= NM_D_FEW) return 0;
-        const long long with = nm_d_plan(dtype, false, true, M, N, K).bytes, without = nm_d_plan(dtype, false, false, M, N, K).bytes;
+        const long long with = nm_d_plan(dtype, false, true, false, M, N, K).bytes, without = nm_d_plan(dtype, false, false, false, M, N, K).bytes;
         return with > without ? with : without;
     }
     // (the bias gradient alone is a plan of its own: one block of columns, more splits)
     const long long both = nm_d_grad_plan(M, N, K).bytes, bias = nm_d_grad_plan(M, N, 1).bytes;
-    return nm_d_plan(dtype, false, false, M, K, N).bytes + (both > bias ? both : bias);
+    return nm_d_plan(dtype, false, false, true, M, K, N).bytes + (both > bias ? both : bias);
 }
 
 int nm_dense_forward(const void* x, int64_t ldx, const void* weight, int64_t ldw, const void* bias, int bias_dtype, const void* residual, int64_t ldr, int64_t M,

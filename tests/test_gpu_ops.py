@@ -93,7 +93,8 @@ def dense_inputs(M, K, N, t, seed, residual=True, exact=False):
 
 
 SIZES = [(1, 1, 1), (1, 256, 256), (2, 300, 20), (3, 7, 5), (8, 64, 33), (9, 16, 16), (12, 3, 300), (31, 177, 131), (128, 8, 9), (129, 207, 256), (257, 256, 257),
-         (300, 1, 300), (70, 300, 1), (640, 72, 40), (1000, 520, 130)]
+         (300, 1, 300), (70, 300, 1), (640, 72, 40), (1000, 520, 130),
+         (8200, 264, 1030), (4200, 521, 2050)]
 
 
 @pytest.mark.parametrize("dtype", TYPES)
