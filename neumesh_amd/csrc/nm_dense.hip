@@ -85,7 +85,9 @@ __device__ __forceinline__ void nm_d_act(int act, float beta, float ibeta, bool 
 #pragma unroll
         for (int i = 0; i < N; ++i) {
             const float u = beta * z[i], e = nm_d_exp<F32>(-fabsf(u));
-            z[i] = fmaf(nm_d_log1p<F32>(e), ibeta, fmaxf(z[i], 0.f));
+            // 16 bits: the hardware's logarithm, off by 1e-7 near 1, so that a small e has its series (the next term is e^2 / 3 < 6e-6 of it)
+            const float l = F32 ? nm_d_log1p<F32>(e) : e < 0x1p-8f ? fmaf(-0.5f * e, e, e) : 0.693147180559945309f * __builtin_amdgcn_logf(1.0f + e);
+            z[i] = fmaf(l, ibeta, fmaxf(z[i], 0.f));
             if (want) {
                 const float r = nm_d_rcp<F32>(1.0f + e);
                 d[i] = u >= 0.f ? r : e * r;
@@ -95,6 +97,19 @@ __device__ __forceinline__ void nm_d_act(int act, float beta, float ibeta, bool 
         const float c1 = act == NM_ACT_GELU_TANH ? 1.59576912160573071f : 1.0f;      // 2 sqrt(2 / pi)
         const float c3 = act == NM_ACT_GELU_TANH ? 0.044715f : 0.0f;
         const bool gate_only = act == NM_ACT_SIGMOID;
+        if constexpr (!F32) {            // 16 bits: one exponential of either sign; where it is infinite q is 0, and so is what it multiplies
+            const float k1 = -1.44269504088896341f * c1;
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                const float x = z[i], e = __builtin_amdgcn_exp2f(k1 * x * fmaf(c3, fminf(x * x, 1e8f), 1.0f)), q = __builtin_amdgcn_rcpf(1.0f + e);
+                if (want) {
+                    const float t = fminf(fmaxf(x, -1e4f), 1e4f), q1 = fminf(e, 3e38f) * q;      // (beyond, q or q1 is 0: no infinity times zero)
+                    d[i] = gate_only ? q * q1 : fmaf(t * q, q1 * (c1 * fmaf(3.0f * c3, t * t, 1.0f)), q);
+                }
+                z[i] = gate_only ? q : x * q;
+            }
+            return;
+        }
 #pragma unroll
         for (int i = 0; i < N; ++i) {
             const float t = fminf(fmaxf(z[i], -1e4f), 1e4f), t2 = t * t;             // (beyond, q or q1 is 0: no infinity times zero)

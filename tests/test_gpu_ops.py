@@ -217,6 +217,27 @@ def test_dense_activations_at_extremes(act):
         assert ((dx.double() - d).abs() <= 2e-6 * d.abs() + 1e-6).all()
 
 
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("act", ["softplus", "sigmoid", "silu", "gelu_tanh", "relu"])
+def test_dense_16_bit_activations_at_extremes(act, dtype):
+    t = TYPES[dtype]
+    top = 60000.0 if dtype == "fp16" else 2e38
+    z = torch.tensor([0.0, -0.0, 1e-3, -1e-3, 0.5, -0.5, 5.0, -5.0, 12.0, -12.0, 30.0, -30.0, 90.0, -90.0, 1e4, -1e4, top, -top], device="cuda").to(t)
+    special = torch.tensor([float("inf"), float("nan")], device="cuda").to(t)
+    for n in (1, 40):                                         # both row forms
+        x = torch.cat([z, special]).repeat_interleave(n)[:, None].contiguous().requires_grad_(True)
+        w = torch.ones(3, 1, device="cuda", dtype=t)
+        y = torch.cat([ops.dense(v, w, activation=act, beta=2.0) for v in x.split(8)]) if n == 1 else ops.dense(x, w, activation=act, beta=2.0)
+        dx = torch.autograd.grad(y[:, 0].sum(), x)[0]
+        m = z.numel() * n
+        h, d, _ = act64(act, x.detach().double()[:m], 2.0)
+        # relative: the result's rounding and 3e-6 of the evaluation (the argument's rounding, |u| < 20 where q is not 0 or 1 in 16 bits); softplus: 1e-7 absolute
+        # near 1 + e = 1, over beta; derivatives are kept with 11 bits at least and rounded once more as dx
+        assert ((y[:m, :1].double() - h).abs() <= (half_step(t) + 5e-6) * h.abs() + tiny(t) + 1e-7).all()
+        assert ((dx[:m].double() - d).abs() <= (half_step(t) + 2.0 ** -11 + 5e-6) * d.abs() + tiny(t) + 2.0 ** -24).all()
+        assert (y[m:m + n, 0] == (1.0 if act == "sigmoid" else float("inf"))).all() and y[m + n:].isnan().all()
+
+
 @pytest.mark.parametrize("dtype", TYPES)
 def test_dense_zero_sizes(dtype):
     t = TYPES[dtype]
