@@ -335,13 +335,13 @@ __device__ __forceinline__ void nm_d_store_cols(typename NmType<DT>::elem* row, 
 
 // accumulators of 16 RT rows x 32 NP columns -> bias (in LDS), activation, residual, stores.  A load waits for every store before it: a bias read from
 // global memory here, piece by piece, cost a 131072 x 256 layer 8 of 52 us.  So the residual (RES) of eight pieces is in flight before the first store, and
-// column blocks with one that stay resident have no more than eight pieces per wave.  The scheduling barriers keep the pieces apart, and the opaque column makes its tests, biases and
+// column blocks with one that stay resident have no more than eight pieces per wave (256 x 256 tiles: six ahead, eight would spill).  The scheduling barriers keep the pieces apart, and the opaque column makes its tests, biases and
 // addresses HERE: mixed together or hoisted out of a loop over row tiles they cost 100 registers and spills.
 template <int DT, bool PROD, bool RES, int RT, int NP>
 __device__ __forceinline__ void nm_d_epilogue(const NmDenseArgs& p, const nm_v4f (&acc)[RT][2 * NP], const float* bias, long long m0, int cb,
                                               int lane) {
     typedef typename NmType<DT>::elem T;
-    constexpr int DD = NmFactor<DT>::T, PIECES = RT * NP, AHEAD = PIECES < 8 ? PIECES : 8;
+    constexpr int DD = NmFactor<DT>::T, PIECES = RT * NP, AHEAD = RT == 8 ? 6 : PIECES < 8 ? PIECES : 8;
     const float ibeta = 1.0f / p.beta;
     const int cw = cb * (32 * NP) + (DT == NM_F32 ? 4 : 8) * (lane >> 4);
     NmOct<DT> rs[AHEAD];
@@ -557,7 +557,7 @@ __global__ __launch_bounds__(512, 2) void nm_dense_resident_kernel(NmDenseArgs p
     }
 }
 
-// Large 16-bit layers in W's own layout: 256 rows x 256 columns per workgroup of eight waves (128 x 64 each).  Both operands come in panels of 64
+// Large 16-bit layers, W as it lies: 256 rows x 256 columns per workgroup of eight waves (128 x 64 each).  Both operands come in panels of 64
 // contraction elements as whole 128-byte lines, eight lanes a line -- read straight into fragments, sixteen rows side by side, the rows of a
 // 16384 x 1024 -> 1024 layer kept the address units busy for 72 % of 93 us -- and go through LDS, in two buffers, with one barrier per panel and the
 // next panel in flight in registers.  The eight 16-byte pieces of an LDS row are exchanged by the row's number, so that the sixteen rows of a fragment
@@ -1098,8 +1098,6 @@ static inline long long nm_d_align(long long b) { return nm_d_up(b, 256) * 256; 
 
 struct NmDensePlan { bool resident, tile; int np, tiles, col_blocks, rt; long long steps, bytes; };
 
-#define NM_D_TILES 128   // tiles of 256 x 256 from which nm_dense_tile_kernel is taken
-
 // columns C, contraction Q, rows R: which kernel, and its column blocks of 32 np columns
 static NmDensePlan nm_d_plan(int dt, bool prod, bool res, bool trans, long long R, long long C, long long Q) {
     NmDensePlan p;
@@ -1110,7 +1108,13 @@ static NmDensePlan nm_d_plan(int dt, bool prod, bool res, bool trans, long long 
     if (res && fit == 8) fit = 4;                            // (the residual of eight pieces is in flight at once)
     while (fit > 0 && 2 * steps * pieces * fit > NM_D_RESIDENT) fit >>= 1;
     p.resident = fit > 0 && nm_d_up(C, 32 * fit) <= 4;
-    p.tile = !p.resident && dt != NM_F32 && !prod && !trans && nm_d_up(R, 256) * nm_d_up(C, 256) >= NM_D_TILES && 4 * C >= 3 * 256 * nm_d_up(C, 256);
+    // 256 x 256 tiles: one per CU and round, so what counts is the share of the rounds' 2^24 outputs that is there.  Measured in bf16 with GELU, us
+    // (tiles / otherwise).  Against streaming: share 1: 50 / 80 (16384 x 1024 -> 1024), 0.63: 90 / 120 (16384 x 1024 -> 1280), 0.38: 46 / 58, 0.25: 44 / 44
+    // (6144 and 4096 x 1024 -> 1024).  Against resident weights: share 1: 55 / 90 (65536 x 1024 -> 256), 27 / 30 (65536 x 256 -> 256), 48 / 46 (65536 x
+    // 256 -> 512), 0.59: 55 / 51 (65536 x 300 -> 300), 0.5: 50 / 49 (32768 x 1024 -> 256).
+    const double rounds = (double)nm_d_up(nm_d_up(R, 256) * nm_d_up(C, 256), 256), share = (double)R * (double)C / (rounds * 16777216.0);
+    p.tile = dt != NM_F32 && !prod && !trans && Q > 0 && R > 0 && share >= (p.resident ? 0.75 : 0.3);
+    if (p.tile) p.resident = false;
     p.np = p.resident ? fit : p.np > 4 ? 4 : p.np;
     // few rows: narrower column blocks until every wave has a tile (streaming: every CU a workgroup)
     while (p.np > 1 && (p.resident ? nm_d_up(R, 32) * nm_d_up(C, 32 * p.np) < 1024 : nm_d_up(R, 128) * nm_d_up(C, 32 * p.np) < 256)) p.np >>= 1;
