@@ -8,7 +8,8 @@ appearance heads, other hidden widths) and the gated linear recurrence along ray
 They stand beside the field's own layers (`NeuMesh`, fp32 tensors and fixed networks) and its own compositing (`volume_render`: rgb, depth,
 normals): tensors are fp32, fp16 or bf16 on a HIP device, sums and states are fp32, results are rounded once.  Calls run on the
 current stream of the tensors' device, do not synchronise, can be captured into a graph and give the same bits from run to run.  Their
-gradients are not differentiable a second time.
+gradients are not differentiable a second time.  A backward pass is captured with leaves of its own (`detach().requires_grad_()`): where an
+eager graph of the same leaves still lives, autograd makes the captured stream wait for that graph's, which ends the capture.
 """
 from __future__ import annotations
 

@@ -94,7 +94,7 @@ def dense_inputs(M, K, N, t, seed, residual=True, exact=False):
 
 SIZES = [(1, 1, 1), (1, 256, 256), (2, 300, 20), (3, 7, 5), (8, 64, 33), (9, 16, 16), (12, 3, 300), (31, 177, 131), (128, 8, 9), (129, 207, 256), (257, 256, 257),
          (300, 1, 300), (70, 300, 1), (640, 72, 40), (1000, 520, 130),
-         (8200, 264, 1030), (4200, 521, 2050)]
+         (8200, 264, 1030), (4200, 521, 2050), (50000, 3, 256)]
 
 
 @pytest.mark.parametrize("dtype", TYPES)
@@ -576,6 +576,48 @@ def test_feature_field_along_rays_end_to_end(dtype):
     assert (out.double().cpu() - want).abs().max() <= tol * want.abs().max()
     for a, b in zip(grads, wgrads):
         assert (a.double().cpu() - b).norm() <= tol * b.norm() + 1e-30
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+def test_dense_tiles_of_strided_rows(dtype):
+    """Enough rows and columns for 256 x 256 tiles: odd strides and offsets give the bits of contiguous tensors."""
+    t = TYPES[dtype]
+    gen = torch.Generator(device="cuda").manual_seed(3)
+    x = torch.randn(13000, 231, generator=gen, device="cuda").to(t)[:, 5:208]
+    w = torch.randn(1030, 301, generator=gen, device="cuda").to(t)[:, 3:206]
+    r = torch.randn(13000, 1101, generator=gen, device="cuda").to(t)[:, 7:1037]
+    b = torch.randn(1030, generator=gen, device="cuda")
+    y = ops.dense(x, w, b, r, activation="silu")
+    assert torch.equal(y, ops.dense(x.contiguous(), w.contiguous(), b, r.contiguous(), activation="silu"))
+    want, bound = dense_reference(x[-300:], w, b, r[-300:], "silu", 1.0)
+    close(y[-300:], want, bound, "last rows")
+
+
+def test_offsets_beyond_32_bits():
+    """More than 2^31 elements and 2^32 bytes: the far end against the same rows on their own."""
+    L, D = 8_500_000, 256
+    gen = torch.Generator(device="cuda").manual_seed(4)
+    x = torch.empty(L, D, device="cuda", dtype=torch.bfloat16).uniform_(-1, 1, generator=gen)
+
+    def near(a, b):                                           # two roundings of one value to 8 bits, sums in another order
+        return bool(((a.float() - b.float()).abs() <= 2.0 ** -7 * b.float().abs() + 1e-4).all())
+    w = torch.randn(D, D, generator=gen, device="cuda").to(torch.bfloat16) / 16
+    y = ops.dense(x, w, activation="relu")
+    assert near(y[-70000:], ops.dense(x[-70000:], w, activation="relu"))
+    del y
+    gate = torch.empty(1, L, 1, device="cuda").uniform_(0.2, 0.9, generator=gen)      # 3000 steps: nothing is left of what was before
+    v = x[None].requires_grad_(True)
+    states, last = ops.gated_scan(gate, v)
+    tail, end = ops.gated_scan(gate[:, -5000:], x[None, -5000:])
+    assert near(states[0, -2000:], tail[0, -2000:]) and near(last, end)
+    dx = torch.autograd.grad(states, v, torch.ones_like(states))[0]
+    u = x[None, -5000:].clone().requires_grad_(True)
+    du = torch.autograd.grad(ops.gated_scan(gate[:, -5000:], u)[0], u, torch.ones_like(u))[0]
+    assert near(dx[0, -5000:], du[0])
+    cu = torch.tensor([0, 10, L - 3000, L], device="cuda")
+    st, last = ops.gated_scan(gate[0], x, cu_seqlens=cu)
+    one, end = ops.gated_scan(gate[:, -3000:], x[None, -3000:])
+    assert near(st[-3000:], one[0]) and near(last[2:], end)
 
 
 def test_same_bits_again_and_on_other_streams():
