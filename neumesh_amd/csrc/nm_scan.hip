@@ -15,7 +15,8 @@
 //   - few long ones, or packed ones of any length: ranges are cut anywhere.  A first launch reduces every range to its map, reading it from its LAST
 //     sequence start on only; a small launch scans the maps; the main launch starts every range from its carried state.
 // The backward pass walks the tiles from the last to the first with the same decomposition of f, and recomputes h_{i-1} in fp32 from the
-// states that the forward pass kept at every tile's start: 4 bytes per channel and tile instead of a second read of rounded states.
+// states that the forward pass kept at every tile's start: 4 bytes per channel and tile instead of a second read of rounded states; sequences that fit a
+// tile keep none.  Sequences of one step (a state carried from call to call) have a kernel of their own, nm_scan_step_kernel.
 // States, maps and sums are fp32; outputs are rounded once.  Every sum has a fixed order.
 #include "nm_error.h"
 #include "nm_num.h"
@@ -398,7 +399,10 @@ template <int VEC, bool SHARED> struct NmSeg {
     static constexpr int B = VEC == 4 ? 4 : 8;
 };
 
-// MAP: only the range's map, from its last sequence start on
+// MAP: only the range's map, from its last sequence start on.
+// Measured, main launch: 4 x 16384 x 512 bf16 44 us (201 MB: 4.6 TB/s; maps 25 us, carries 9), 8192 packed sequences of 96 x 32 fp32 60 us (302 MB: 5.0 TB/s;
+// maps 20), 32768 x 127 x 3 fp32, last state only, 26 us (67 MB: 2.5 TB/s: two rounds of workgroups of one tile, a third of the time instructions and
+// the rest latency of loads, lane exchanges and barriers).
 template <int DX, int DG, int VEC, bool SHARED, bool MAP>
 __global__ __launch_bounds__(NM_S_THREADS) void nm_scan_forward_kernel(NmScanArgs p) {
     typedef typename NmType<DX>::elem TX;
@@ -552,7 +556,10 @@ __global__ __launch_bounds__(NM_S_THREADS) void nm_scan_forward_kernel(NmScanArg
     }
 }
 
-// MAP: only the range's map of the flow, up to its first sequence end
+// MAP: only the range's map of the flow, up to its first sequence end.
+// Measured, main launch: 8192 packed sequences of 96 x 32 fp32 with h0 118 us (503 MB: 4.3 TB/s; maps 23), 1 x 32768 x 256 bf16 27 us (84 MB: 3.0 TB/s), 2048 x
+// 127 x 32 bf16 with a shared gate 27 us (51 MB: 1.9 TB/s).  Bound by two or three workgroups per CU (180 .. 200 registers): a bound of three for
+// all of them spills and costs 35 us instead of 27 for the second.
 template <int DX, int DG, int VEC, bool SHARED, bool MAP>
 __global__ __launch_bounds__(NM_S_THREADS) void nm_scan_backward_kernel(NmScanArgs p) {
     typedef typename NmType<DX>::elem TX;
@@ -767,7 +774,7 @@ __global__ __launch_bounds__(NM_S_THREADS) void nm_scan_backward_kernel(NmScanAr
 }
 
 // maps of the ranges -> the state before every range (DIR = 1), or the flow after it (-1).  8 channels x 128 lanes in time, 16 ranges each: one round for
-// all the ranges of a launch (nm_s_plan makes some NM_S_FILL_PACKED at most, so that offsets stay far below 2^32), for what a round costs is its latency.
+// all the ranges of a launch (nm_s_plan makes some NM_S_FILL_PACKED at most, so that offsets stay far below 2^32), for what a round costs is its latency (9 us for 1537 ranges of 32 channels).
 #define NM_S_CARRY 1024
 template <int DIR>
 __global__ __launch_bounds__(NM_S_CARRY) void nm_scan_carry_kernel(const float* __restrict__ map_a, const float* __restrict__ map_h, const int* __restrict__ map_f, int n, int D,
