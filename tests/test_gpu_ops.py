@@ -593,6 +593,55 @@ def test_dense_tiles_of_strided_rows(dtype):
     close(y[-300:], want, bound, "last rows")
 
 
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+def test_dense_tiles_keep_non_finite_values_apart(dtype):
+    """... of rows in rows, of weights in columns; last pieces of odd contraction lengths included."""
+    t = TYPES[dtype]
+    gen = torch.Generator(device="cuda").manual_seed(6)
+    x, w = torch.randn(13000, 203, generator=gen, device="cuda").to(t), torch.randn(1030, 203, generator=gen, device="cuda").to(t)
+    clean = ops.dense(x, w)
+    assert clean.isfinite().all()
+    bad, wbad = x.clone(), w.clone()
+    bad[5], bad[300, 202], bad[12999, 196], bad[700, 0] = float("nan"), float("inf"), float("-inf"), float("inf")
+    rows = torch.tensor([5, 300, 700, 12999], device="cuda")
+    y = ops.dense(bad, w)
+    keep = torch.ones(13000, dtype=torch.bool, device="cuda").index_fill(0, rows, False)
+    assert torch.equal(y[keep], clean[keep]) and not y[rows].isfinite().any()
+    wbad[7, 200], wbad[1029, 0] = float("inf"), float("nan")
+    y = ops.dense(x, wbad)
+    cols = torch.ones(1030, dtype=torch.bool, device="cuda").index_fill(0, torch.tensor([7, 1029], device="cuda"), False)
+    assert torch.equal(y[:, cols], clean[:, cols]) and y[:, 1029].isnan().all()
+
+
+def test_captured_large_layers_and_scans_replay():
+    """The kernels of large sizes (tiles, split gradients, ranges with carried states) captured together, replayed on new data."""
+    t = torch.bfloat16
+    gen = torch.Generator(device="cuda").manual_seed(8)
+    x = torch.randn(13000, 200, generator=gen, device="cuda").to(t)
+    p = [torch.randn(1030, 200, generator=gen, device="cuda").to(t).mul_(0.07).requires_grad_(True), torch.randn(1030, generator=gen, device="cuda").requires_grad_(True)]
+    cu = torch.tensor([0, 0, 900, 901, 7000, 12990], device="cuda")
+    gate = torch.rand(13000, 1, generator=gen, device="cuda")
+    g, gs = torch.randn(5, 1030, generator=gen, device="cuda"), torch.randn(13000, 1030, generator=gen, device="cuda").to(t)
+
+    def step(p):
+        states, last = ops.gated_scan(gate, ops.dense(x, p[0], p[1], activation="silu"), cu_seqlens=cu, blend=True)
+        return [states, last] + list(torch.autograd.grad((states, last), p, (gs, g)))
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        step(p)
+    torch.cuda.current_stream().wait_stream(stream)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = step(p)
+    for i in range(3):
+        x.copy_(torch.randn(x.shape, generator=gen, device="cuda").to(t))
+        graph.replay()
+        want = step([v.detach().clone().requires_grad_(True) for v in p])
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(held, want)), i
+
+
 def test_offsets_beyond_32_bits():
     """More than 2^31 elements and 2^32 bytes: the far end against the same rows on their own."""
     L, D = 8_500_000, 256
