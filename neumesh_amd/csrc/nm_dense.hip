@@ -38,6 +38,7 @@ template <int DT> struct NmFactor { static constexpr int T = DT == NM_F32 ? (int
 
 #define NM_D_MAX_DIM (1 << 20)   // columns and contraction lengths fit 32-bit arithmetic with room
 #define NM_D_MAX_LD (1 << 24)    // 64 rows of any stride stay below 2^32 bytes
+#define NM_D_MAX_THREADS 0xffffffffLL    // of one launch
 
 // ------------------------------------------------------------------------------------------------ activations
 // Exponentials and reciprocals from the hardware's approximations; F32 (fp32 outputs) corrects them to the last place (library exponential and division:
@@ -1177,7 +1178,7 @@ static int nm_d_launch(const NmDensePlan& pl, NmDenseArgs a, hipStream_t stream)
         return 0;
     }
     const long long groups = nm_d_up(nm_d_up(a.R, pl.tile ? 256 : 64 * pl.rt), 8) * 8 * pl.col_blocks;
-    if (groups > 0x7fffffffLL) return nm_fail("nm_dense: %lld rows x %d columns exceed one launch", a.R, a.C);
+    if (groups * (pl.tile ? 512 : 256) > NM_D_MAX_THREADS) return nm_fail("nm_dense: %lld rows x %d columns exceed one launch", a.R, a.C);
     const dim3 grid((unsigned)groups), block(256);
     if (pl.tile) {
         if constexpr (!F && !PROD) hipLaunchKernelGGL((nm_dense_tile_kernel<DT>), grid, dim3(512), 0, stream, a);
@@ -1254,7 +1255,7 @@ static int nm_d_backward(const void* g, long long ldg, const void* deriv, const 
     const long long tiles = (long long)pl.n_tiles * pl.k_tiles;
     const long long groups = tiles * nm_d_up(pl.splits, 8) * 8;
     a.splits = pl.splits;
-    if (groups > 0x7fffffffLL) return nm_fail("nm_dense_backward: %d x %d weights exceed one launch", N, K);
+    if (groups * 256 > NM_D_MAX_THREADS) return nm_fail("nm_dense_backward: %d x %d weights exceed one launch", N, K);
     const dim3 grid((unsigned)groups), block(256);
     if (deriv) hipLaunchKernelGGL((nm_dense_grad_kernel<DT, true>), grid, block, 0, stream, a);
     else hipLaunchKernelGGL((nm_dense_grad_kernel<DT, false>), grid, block, 0, stream, a);

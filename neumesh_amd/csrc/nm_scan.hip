@@ -392,6 +392,7 @@ __device__ __forceinline__ void nm_s_forget(T (&v)[SEG]) {
 }
 
 #define NM_S_THREADS 256
+#define NM_S_MAX_GROUPS (0xffffffffLL / NM_S_THREADS)    // of one launch: its threads are counted in 32 bits
 // Steps of a thread.  Forward: as many as 32 .. 64 registers of operands allow (the scan's own instructions are per thread; with 4 steps they bound
 // short sequences at 2.4 TB/s).  Backward: three operands and the recomputed states.
 template <int VEC, bool SHARED> struct NmSeg {
@@ -833,12 +834,14 @@ __global__ __launch_bounds__(NM_S_CARRY) void nm_scan_carry_kernel(const float* 
     }
 }
 
-// packed sequences: the sequence of every row (-1: none), and the result of empty sequences (their state / their cotangent passes through)
+// packed sequences: the sequence of every row (-1: none), and the result of empty sequences (their state / their cotangent passes through).
+// (Launches have 2^31 threads at most, nm_s_threads: S x D may be more.)
 __global__ __launch_bounds__(256) void nm_scan_rows_kernel(const int* __restrict__ cu, long long S, long long L, int D, const float* __restrict__ src, float* __restrict__ dst,
                                                            int* __restrict__ seg) {
-    const long long t = (long long)blockIdx.x * 256 + threadIdx.x;
-    if (seg && t < L) seg[t] = nm_scan_sequence(cu, S, t);
-    if (dst && t < S * D) {
+    const long long t0 = (long long)blockIdx.x * 256 + threadIdx.x;
+    if (seg && t0 < L) seg[t0] = nm_scan_sequence(cu, S, t0);
+    if (!dst) return;
+    for (long long t = t0; t < S * D; t += (long long)gridDim.x * 256) {
         const long long s = t / D;
         if (cu[s + 1] <= cu[s]) dst[t] = src ? src[t] : 0.f;
     }
@@ -846,8 +849,7 @@ __global__ __launch_bounds__(256) void nm_scan_rows_kernel(const int* __restrict
 
 // what passes through a batch without a single step
 __global__ __launch_bounds__(256) void nm_scan_pass_kernel(const float* __restrict__ src, float* __restrict__ dst, long long n) {
-    const long long t = (long long)blockIdx.x * 256 + threadIdx.x;
-    if (t < n) dst[t] = src ? src[t] : 0.f;
+    for (long long t = (long long)blockIdx.x * 256 + threadIdx.x; t < n; t += (long long)gridDim.x * 256) dst[t] = src ? src[t] : 0.f;
 }
 
 // Sequences of one step, the form of a state carried from call to call: no order among the rows, so one thread per VEC channels, without tiles, scans and
@@ -893,6 +895,8 @@ __global__ __launch_bounds__(256) void nm_scan_gate_sum_kernel(const float* __re
 // ------------------------------------------------------------------------------------------------ plans and launches
 static inline long long nm_s_up(long long a, long long b) { return (a + b - 1) / b; }
 static inline size_t nm_s_align(size_t x) { return (x + 255) & ~(size_t)255; }
+// workgroups of 256 threads for n threads, 2^31 threads at most (a launch of 2^32 is refused by the runtime; L < 2^31)
+static inline dim3 nm_s_threads(long long n) { return dim3((unsigned)(n < 0x80000000LL ? nm_s_up(n, 256) : 0x800000LL)); }
 
 struct NmScanShape { int vec, cl_log2, blocks, tile; };      // of one direction: channels and channel lanes, tile in steps
 struct NmScanPlan {
@@ -1030,19 +1034,20 @@ int nm_scan_forward(const void* gate, int gate_dtype, int shared_gate, const voi
     if (D == 0 || (L == 0 && S == 0)) return 0;
     if ((L > 0 && (!gate || !x)) || (S > 0 && !last)) return nm_fail("nm_scan_forward: NULL argument");
     if (L == 0) {                        // every sequence is empty: its state passes through
-        hipLaunchKernelGGL(nm_scan_pass_kernel, dim3((unsigned)nm_s_up(S * D, 256)), dim3(256), 0, stream, h0, last, (long long)(S * D));
+        hipLaunchKernelGGL(nm_scan_pass_kernel, nm_s_threads(S * D), dim3(256), 0, stream, h0, last, (long long)(S * D));
         NM_LAUNCH_CHECK();
         return 0;
     }
     const NmScanPlan pl = nm_s_plan(L, S, (int)D, dtype, shared, packed);
     const NmScanShape& shape = pl.f;
     if ((size_t)(workspace_bytes < 0 ? 0 : workspace_bytes) < pl.bytes || (pl.bytes > 0 && !workspace)) return nm_fail("nm_scan_forward: workspace too small");
-    if (pl.chunks_f * shape.blocks > 0x7fffffffLL) return nm_fail("nm_scan_forward: %lld steps x %lld channels exceed one launch", (long long)L, (long long)D);
+    if (pl.chunks_f * shape.blocks > NM_S_MAX_GROUPS) return nm_fail("nm_scan_forward: %lld steps x %lld channels exceed one launch", (long long)L, (long long)D);
     char* ws = (char*)workspace;
     int* rows = packed ? keep ? (int*)keep : (int*)(ws + pl.off_seg) : nullptr;
     if (packed) {
         const long long n = L > S * D ? L : S * D;
-        hipLaunchKernelGGL(nm_scan_rows_kernel, dim3((unsigned)nm_s_up(n, 256)), dim3(256), 0, stream, cu_seqlens, (long long)S, (long long)L, (int)D, h0, last, rows);
+        hipLaunchKernelGGL(nm_scan_rows_kernel, nm_s_threads(n), dim3(256), 0, stream, cu_seqlens, (long long)S, (long long)L, (int)D, h0, last, rows);
+        NM_LAUNCH_CHECK();               // (the main launch indexes with these rows)
     }
     NmScanArgs a = {};
     nm_s_fill(a, pl, shape, gate, x, h0, cu_seqlens, L, S, D, reverse, blend, ws, rows);
@@ -1086,19 +1091,20 @@ int nm_scan_backward(const void* gate, int gate_dtype, int shared_gate, const vo
     if (L > 0 && (!gate || (dgate && (!x || (!keep && nm_scan_keep_elems(L, S, D, dtype, shared_gate, packed) > 0))))) return nm_fail("nm_scan_backward: NULL argument");
     if (L == 0) {
         if (!dh0) return 0;
-        hipLaunchKernelGGL(nm_scan_pass_kernel, dim3((unsigned)nm_s_up(S * D, 256)), dim3(256), 0, stream, g_last, dh0, (long long)(S * D));
+        hipLaunchKernelGGL(nm_scan_pass_kernel, nm_s_threads(S * D), dim3(256), 0, stream, g_last, dh0, (long long)(S * D));
         NM_LAUNCH_CHECK();
         return 0;
     }
     const NmScanPlan pl = nm_s_plan(L, S, (int)D, dtype, shared, packed);
     const NmScanShape& shape = pl.b;
     if ((size_t)(workspace_bytes < 0 ? 0 : workspace_bytes) < pl.bytes || (pl.bytes > 0 && !workspace)) return nm_fail("nm_scan_backward: workspace too small");
-    if (pl.chunks_b * shape.blocks > 0x7fffffffLL) return nm_fail("nm_scan_backward: %lld steps x %lld channels exceed one launch", (long long)L, (long long)D);
+    if (pl.chunks_b * shape.blocks > NM_S_MAX_GROUPS) return nm_fail("nm_scan_backward: %lld steps x %lld channels exceed one launch", (long long)L, (long long)D);
     char* ws = (char*)workspace;
     int* rows = packed ? keep ? (int*)const_cast<float*>(keep) : (int*)(ws + pl.off_seg) : nullptr;
     if (packed && (!keep || dh0)) {      // (the rows' sequences are kept from the forward pass)
         const long long n = keep ? S * D : L > S * D ? L : S * D;
-        hipLaunchKernelGGL(nm_scan_rows_kernel, dim3((unsigned)nm_s_up(n, 256)), dim3(256), 0, stream, cu_seqlens, (long long)S, (long long)L, (int)D, g_last, dh0, keep ? nullptr : rows);
+        hipLaunchKernelGGL(nm_scan_rows_kernel, nm_s_threads(n), dim3(256), 0, stream, cu_seqlens, (long long)S, (long long)L, (int)D, g_last, dh0, keep ? nullptr : rows);
+        NM_LAUNCH_CHECK();
     }
     NmScanArgs a = {};
     nm_s_fill(a, pl, shape, gate, x, h0, cu_seqlens, L, S, D, reverse, blend, ws, rows);

@@ -126,3 +126,16 @@ def test_packed_rows_and_ranges():
                     while last < c1 - 1 and seq[0] >= 0 and seq[last + 1 - c0] == seq[0]:
                         last += 1
                     assert (lo, hi) == (first, last)
+
+
+def test_launches_beyond_32_bits_of_threads_are_refused():
+    """A launch's threads are counted in 32 bits: more is an error of the call's own, before anything is launched (the pointers are never followed)."""
+    lib = _lib.load(require_device=False)
+    p = C.c_void_p(4096)
+    L, S, D = 1 << 30, 1 << 25, 2048                          # ranges of 32 steps x 8 blocks of channels: 2^28 workgroups
+    assert lib.nm_scan_forward(p, 0, 0, p, 0, None, None, L, S, D, 0, 0, p, p, None, p, 1 << 62, None) == 1
+    assert b"exceed one launch" in lib.nm_last_error()
+    assert lib.nm_scan_backward(p, 0, 0, p, 0, None, None, L, S, D, 0, 0, p, p, p, p, p, p, p, 1 << 62, None) == 1
+    assert b"exceed one launch" in lib.nm_last_error()
+    assert lib.nm_dense_forward(p, 1024, p, 1024, None, 2, None, 0, 1 << 31, 1024, 1024, 2, 0, 1.0, p, 1024, None, p, 1 << 62, None) == 1     # 256 x 256 tiles
+    assert b"exceed one launch" in lib.nm_last_error()
