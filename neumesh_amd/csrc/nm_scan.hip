@@ -882,7 +882,7 @@ __global__ __launch_bounds__(256) void nm_scan_step_kernel(NmScanArgs p, int sha
     nm_s_store<NM_F32, VEC>(p.last + e, h);
 }
 
-// shared gate over several channel blocks: sum of the blocks' parts, in order
+// shared gate over several channel blocks: sum of the blocks' parts, in order (no block: 0)
 template <int DG>
 __global__ __launch_bounds__(256) void nm_scan_gate_sum_kernel(const float* __restrict__ part, int blocks, long long L, typename NmType<DG>::elem* __restrict__ dgate) {
     const long long t = (long long)blockIdx.x * 256 + threadIdx.x;
@@ -1012,6 +1012,13 @@ static void nm_s_fill(NmScanArgs& a, const NmScanPlan& pl, const NmScanShape& sh
     }
 }
 
+static void nm_s_gate_sum(const float* part, int blocks, long long L, void* dgate, int gate_dtype, hipStream_t stream) {
+    const dim3 grid = nm_s_threads(L);
+    if (gate_dtype == NM_F32) hipLaunchKernelGGL(nm_scan_gate_sum_kernel<NM_F32>, grid, dim3(256), 0, stream, part, blocks, L, (float*)dgate);
+    else if (gate_dtype == NM_F16) hipLaunchKernelGGL(nm_scan_gate_sum_kernel<NM_F16>, grid, dim3(256), 0, stream, part, blocks, L, (_Float16*)dgate);
+    else hipLaunchKernelGGL(nm_scan_gate_sum_kernel<NM_BF16>, grid, dim3(256), 0, stream, part, blocks, L, (__bf16*)dgate);
+}
+
 extern "C" {
 
 int64_t nm_scan_workspace_bytes(int64_t L, int64_t S, int64_t D, int dtype, int shared_gate, int packed) {
@@ -1087,7 +1094,12 @@ int nm_scan_backward(const void* gate, int gate_dtype, int shared_gate, const vo
     hipStream_t stream = (hipStream_t)stream_;
     const bool packed = cu_seqlens != nullptr, shared = shared_gate != 0;
     if (nm_s_check("nm_scan_backward", L, S, D, dtype, gate_dtype, packed)) return 1;
-    if (D == 0 || (L == 0 && S == 0) || (!dgate && !dx && !dh0)) return 0;
+    if ((L == 0 && S == 0) || (!dgate && !dx && !dh0)) return 0;
+    if (D == 0) {                        // no channels: nothing but a shared gate's gradient, a sum over none of them
+        if (dgate && shared && L > 0) nm_s_gate_sum(nullptr, 0, L, dgate, gate_dtype, stream);
+        NM_LAUNCH_CHECK();
+        return 0;
+    }
     if (L > 0 && (!gate || (dgate && (!x || (!keep && nm_scan_keep_elems(L, S, D, dtype, shared_gate, packed) > 0))))) return nm_fail("nm_scan_backward: NULL argument");
     if (L == 0) {
         if (!dh0) return 0;
@@ -1119,12 +1131,7 @@ int nm_scan_backward(const void* gate, int gate_dtype, int shared_gate, const vo
         a.carry = carry;
     }
     NM_S_PICK(nm_scan_backward_kernel, false, false);
-    if (parts) {
-        const dim3 g2((unsigned)nm_s_up(L, 256));
-        if (gate_dtype == NM_F32) hipLaunchKernelGGL(nm_scan_gate_sum_kernel<NM_F32>, g2, dim3(256), 0, stream, a.dgate_part, shape.blocks, (long long)L, (float*)dgate);
-        else if (gate_dtype == NM_F16) hipLaunchKernelGGL(nm_scan_gate_sum_kernel<NM_F16>, g2, dim3(256), 0, stream, a.dgate_part, shape.blocks, (long long)L, (_Float16*)dgate);
-        else hipLaunchKernelGGL(nm_scan_gate_sum_kernel<NM_BF16>, g2, dim3(256), 0, stream, a.dgate_part, shape.blocks, (long long)L, (__bf16*)dgate);
-    }
+    if (parts) nm_s_gate_sum(a.dgate_part, shape.blocks, L, dgate, gate_dtype, stream);
     NM_LAUNCH_CHECK();
     return 0;
 }

@@ -30,3 +30,21 @@ def test_states_beyond_32_bits_of_empty_sequences():
     # no rows at all
     _, last = ops.gated_scan(gate.detach()[:0], x.detach()[:0], g, cu_seqlens=torch.zeros_like(cu))
     assert torch.equal(last, g)
+
+
+@pytest.mark.parametrize("types", [(torch.float32, torch.float32), (torch.bfloat16, torch.float32), (torch.bfloat16, torch.bfloat16), (torch.float16, torch.float16)])
+def test_gradient_of_a_shared_gate_over_no_channels(types):
+    """An empty sum: 0, whatever the memory of the result held before."""
+    for packed in (False, True):
+        lead = (300,) if packed else (3, 100)
+        gate = torch.rand(*lead, 1, device="cuda").to(types[1]).requires_grad_(True)
+        x = torch.rand(*lead, 0, device="cuda").to(types[0]).requires_grad_(True)
+        cu = torch.tensor([0, 100, 290], device="cuda") if packed else None
+        states, last = ops.gated_scan(gate, x, cu_seqlens=cu)
+        torch.full((300,), float("nan"), device="cuda", dtype=types[1])      # (freed at once: what the allocator hands out next)
+        dgate, dx = torch.autograd.grad((states, last), (gate, x), (torch.ones_like(states), torch.ones_like(last)))
+        assert dgate.shape == gate.shape and (dgate == 0).all() and dx.shape == x.shape
+    alpha = torch.rand(5, 60, device="cuda").requires_grad_(True)
+    out = ops.composite_features(alpha, torch.rand(5, 60, 0, device="cuda"))
+    torch.full((300,), float("nan"), device="cuda")
+    assert (torch.autograd.grad(out, alpha, torch.ones_like(out))[0] == 0).all()
