@@ -8,8 +8,9 @@ appearance heads, other hidden widths) and the gated linear recurrence along ray
 They stand beside the field's own layers (`NeuMesh`, fp32 tensors and fixed networks) and its own compositing (`volume_render`: rgb, depth,
 normals): tensors are fp32, fp16 or bf16 on a HIP device, sums and states are fp32, results are rounded once.  Calls run on the
 current stream of the tensors' device, do not synchronise, can be captured into a graph and give the same bits from run to run.  Their
-gradients are not differentiable a second time.  A backward pass is captured with leaves of its own (`detach().requires_grad_()`): where an
-eager graph of the same leaves still lives, autograd makes the captured stream wait for that graph's, which ends the capture.
+gradients are not differentiable a second time, and tangents of forward-mode differentiation are refused.  A backward pass is captured
+with leaves of its own (`detach().requires_grad_()`): where an eager graph of the same leaves still lives, autograd makes the captured
+stream wait for that graph's, which ends the capture.
 """
 from __future__ import annotations
 
@@ -18,6 +19,7 @@ import math
 from typing import Optional, Tuple
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 
@@ -71,6 +73,13 @@ def _once(who):
     through them would silently be taken as zero."""
     if torch.is_grad_enabled():
         raise RuntimeError(f"{who}: its gradient cannot be differentiated again (backward with create_graph=True)")
+
+
+def _no_tangents(who, *tensors):
+    """Forward-mode differentiation is not offered: a tangent would be dropped silently, since a dual tensor need not require grad.  (The level is -1
+    outside of every dual_level, the one thing that a call pays for.)"""
+    if forward_ad._current_level >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise RuntimeError(f"{who}: forward-mode derivatives are not supported (an input carries a tangent)")
 
 
 # ------------------------------------------------------------------------------------------------ dense layers
@@ -162,6 +171,7 @@ def dense(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] = 
     beta = float(beta)
     if activation == "softplus" and not (beta > 0.0 and math.isfinite(beta)):
         raise ValueError(f"dense: beta={beta} must be positive")
+    _no_tangents("dense", x, weight, bias, residual)
     _on_device("dense", dev)
     act = ACTIVATIONS[activation]
     if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or (bias is not None and bias.requires_grad) or (residual is not None and residual.requires_grad)):
@@ -249,6 +259,7 @@ def gated_scan(gate: torch.Tensor, x: torch.Tensor, h0: Optional[torch.Tensor] =
     S = cu_seqlens.shape[0] - 1 if packed else x.shape[0]
     if h0 is not None and tuple(h0.shape) != (S, D):
         raise ValueError(f"gated_scan: h0 has shape {tuple(h0.shape)}, expected {(S, D)}")
+    _no_tangents("gated_scan", gate, x, h0)
     _on_device("gated_scan", dev)
     h0 = None if h0 is None else h0.float().contiguous()
     cu = cu_seqlens.to(torch.int32).contiguous() if packed else None

@@ -139,3 +139,26 @@ def test_launches_beyond_32_bits_of_threads_are_refused():
     assert b"exceed one launch" in lib.nm_last_error()
     assert lib.nm_dense_forward(p, 1024, p, 1024, None, 2, None, 0, 1 << 31, 1024, 1024, 2, 0, 1.0, p, 1024, None, p, 1 << 62, None) == 1     # 256 x 256 tiles
     assert b"exceed one launch" in lib.nm_last_error()
+
+
+def test_tangents_are_refused():
+    """Forward-mode derivatives: an error, with and without inputs that require grad, in every differentiable argument; never a result without its tangent."""
+    from torch.autograd import forward_ad as fa
+    x, w, b, r = torch.randn(4, 6), torch.randn(5, 6), torch.randn(5), torch.randn(4, 5)
+    gate, v, h = torch.rand(2, 5, 3), torch.randn(2, 5, 3), torch.randn(2, 3)
+    alpha, feats, bg = torch.rand(2, 5), torch.randn(2, 5, 3), torch.randn(2, 3)
+    for fn, args in ((ops.dense, (x, w, b, r)), (ops.gated_scan, (gate, v, h)), (ops.composite_features, (alpha, feats, bg))):
+        for i in range(len(args)):
+            for leaf in (False, True):
+                with fa.dual_level():
+                    a = list(args)
+                    a[i - 1] = a[i - 1].clone().requires_grad_(leaf)
+                    a[i] = fa.make_dual(a[i], torch.ones_like(a[i]))
+                    with pytest.raises(RuntimeError, match="forward-mode derivatives are not supported"):
+                        fn(*a)
+                    with torch.no_grad(), pytest.raises(RuntimeError, match="forward-mode derivatives are not supported"):
+                        fn(*a)
+        with fa.dual_level(), pytest.raises(_lib.NeuMeshHipError, match="HIP device"):      # no input with a tangent: the call goes on
+            fn(*args)
+    with pytest.raises(RuntimeError, match="forward-mode derivatives are not supported"):
+        torch.func.jvp(lambda t: ops.dense(t, w), (x,), (x,))
