@@ -401,8 +401,8 @@ int nm_train_composite_backward(const float* sdf, const float* s, const float* d
  * pass needs; NULL = not wanted.  With
  * NM_ACT_NONE nothing is written and the backward pass takes NULL.
  * nm_dense_backward: g [M,N] cotangent of y -> dx [M,K] (lddx), dweight [N,K] contiguous, dbias [N] (NULL = not wanted; overwritten, not added to).  The
- * gradient of r is g itself.  The result does not change from run to run.  fp32: a non-finite operand makes the outputs it enters
- * NaN where IEEE arithmetic may give an infinity.
+ * gradient of r is g itself.  The result does not change from run to run.  fp32, and gradients with deriv: a non-finite operand makes the
+ * outputs it enters NaN where IEEE arithmetic may give an infinity.
  * workspace: nm_dense_workspace_bytes(.., backward) bytes, 16-byte aligned, of this call until its stream work is done. */
 enum { NM_F32 = 0, NM_F16 = 1, NM_BF16 = 2 };                 /* element types */
 enum { NM_ACT_NONE = 0, NM_ACT_RELU = 1, NM_ACT_SOFTPLUS = 2, NM_ACT_SIGMOID = 3, NM_ACT_SILU = 4, NM_ACT_GELU_TANH = 5 };

@@ -10,11 +10,14 @@
 //                        fixed order (the same bits from run to run)
 // nm_dense_few_kernel serves 1 .. 8 rows (a probe, a picked point).
 //
-// Arithmetic.  16-bit inputs: one product per pair on the f16 / bf16 pipe, fp32 accumulation, fp32 epilogue, one rounding at the end.  The
-// forward pass keeps act'(z) for the backward pass in 16 bits that are finer than the rows' own (NmFactor); dz = g act'(z) enters the products as TWO 16-bit pieces (value + residual): a single rounded piece put an error as
-// large as the output's own rounding on dx and dW.  fp32 inputs: every operand cut into three bf16 pieces (nm_gemm.h: exact), six
-// piece products, fp32 accumulation; act'(z) is kept in fp32.  An fp32 product with a non-finite operand is NaN where IEEE
-// arithmetic may give an infinity.
+// Arithmetic.  16-bit inputs: one product per pair on the f16 / bf16 pipe, fp32 accumulation, fp32 epilogue, one rounding at the end.  The forward pass
+// keeps act'(z) for the backward pass in 16 bits that are finer than the rows' own (NmFactor).  dz = g act'(z) enters the products as TWO bf16
+// pieces (value + residual: 16 bits, over fp32's whole range): a single rounded piece put an error as large as the output's own rounding on dx and
+// dW, and fp16 pieces lost what lies below 2^-13 (g of a mean over many outputs) and beyond 65504 (g near the maximum times act' = 1.13).
+// Beside fp16 rows the other operand is cut into two bf16 pieces as well, exactly, and three piece products are taken (10007 x 177 -> 131 forward and
+// backward 123 us, 126 with two products of fp16 pieces).  fp32 inputs: every operand cut into three bf16 pieces (nm_gemm.h: exact), six piece
+// products, fp32 accumulation; act'(z) is kept in fp32.  A product of several pieces with a non-finite operand is NaN where IEEE arithmetic may
+// give an infinity.
 #include "nm_error.h"
 #include "nm_num.h"
 
@@ -143,20 +146,26 @@ __device__ __forceinline__ void nm_d_cut8(const float (&f)[8], uint4 (&p)[3]) {
     for (int q = 0; q < 3; ++q)
         p[q] = make_uint4(nm_d_pair(b[q][0], b[q][1]), nm_d_pair(b[q][2], b[q][3]), nm_d_pair(b[q][4], b[q][5]), nm_d_pair(b[q][6], b[q][7]));
 }
-// value + residual in the 16-bit type (no residual of an infinity)
-template <int DT>
+// value + residual in bf16: 16 bits of any fp32 value, all of an fp16 one (no residual of an infinity)
 __device__ __forceinline__ void nm_d_two8(const float (&f)[8], uint4 (&p)[2]) {
-    typedef typename NmType<DT>::elem T;
-    T hi[8], lo[8];
+    __bf16 hi[8], lo[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-        hi[e] = (T)f[e];
+        hi[e] = (__bf16)f[e];
         const float b = (float)hi[e];
-        lo[e] = (T)(fabsf(b) < __builtin_inff() ? f[e] - b : 0.f);
+        lo[e] = (__bf16)(fabsf(b) < __builtin_inff() ? f[e] - b : 0.f);
     }
     __builtin_memcpy(&p[0], hi, 16);
     __builtin_memcpy(&p[1], lo, 16);
 }
+
+// Pieces of the operands of a product, and the 16-bit type that the matrix pipe sees.  PROD: one operand (the rows, or dz of the weight gradient) is g * act'(z).
+template <int DT, bool PROD> struct NmPieces {
+    static constexpr int PLAIN = DT == NM_F32 ? 3 : DT == NM_F16 && PROD ? 2 : 1;        // the other operand
+    static constexpr int ROWS = DT == NM_F32 ? 3 : PROD ? 2 : 1;
+    static constexpr int MF = DT == NM_F16 && !PROD ? (int)NM_F16 : (int)NM_BF16;
+};
+static inline int nm_d_pieces(int dt, bool prod) { return dt == NM_F32 ? 3 : dt == NM_F16 && prod ? 2 : 1; }      // (PLAIN)
 
 // one matrix instruction: V = nm_v16f: 32 x 32 outputs, 16 deep;  nm_v4f: 16 x 16 outputs, 32 deep
 template <int DT, typename V>
@@ -187,8 +196,12 @@ __device__ __forceinline__ V nm_d_products(const uint4 (&a)[PA], const uint4 (&b
         c = nm_d_mfma<DT>(a[0], b[1], c);
         c = nm_d_mfma<DT>(a[1], b[0], c);
         return nm_d_mfma<DT>(a[0], b[0], c);
+    } else if constexpr (PA == 2 && PB == 2) {               // dropped: a1 b1 < 2^-18 |a||b|, of either sign
+        c = nm_d_mfma<DT>(a[1], b[0], c);
+        c = nm_d_mfma<DT>(a[0], b[1], c);
+        return nm_d_mfma<DT>(a[0], b[0], c);
     } else {
-        static_assert(PA == 1 || PB == 1, "16-bit products: at most one operand in two pieces");
+        static_assert(PA == 1 || PB == 1, "two pieces against one");
 #pragma unroll
         for (int i = PA - 1; i >= 0; --i)
 #pragma unroll
@@ -212,11 +225,24 @@ __host__ __device__ __forceinline__ int nm_d_column(int tile, int i) {
 // repeats is zero on the packed side (and cleared on the rows' side, where it may be an infinity).  Q < 8: element by element from 0.
 __host__ __device__ __forceinline__ long long nm_d_window(long long q0, long long Q) { return Q < 8 || q0 + 8 <= Q ? q0 : Q - 8; }
 
-// pieces per weight element
-template <int DT> struct NmPlanes { static constexpr int W = DT == NM_F32 ? 3 : 1; };
+// eight weights in PW pieces -> their place in each plane
+template <int DT, int PW>
+__device__ __forceinline__ void nm_d_put_weights(const NmOct<DT>& o, uint4* d) {
+    if constexpr (PW == 1) {
+        *d = o.v[0];
+    } else {
+        float f[8];
+        uint4 x[PW];
+        nm_oct_to_float<DT>(o, f);
+        if constexpr (PW == 3) nm_d_cut8(f, x);
+        else nm_d_two8(f, x);
+#pragma unroll
+        for (int q = 0; q < PW; ++q) d[q * 64] = x[q];
+    }
+}
 
 // The streaming kernel's weights: dst [steps][tiles][plane][lane], zero beyond C and Q
-template <int DT>
+template <int DT, int PW>
 __global__ __launch_bounds__(256) void nm_dense_pack_kernel(const typename NmType<DT>::elem* __restrict__ w, long long ldw, int trans, int C, int Q, int tiles,
                                                             int steps, uint4* __restrict__ dst) {
     typedef typename NmType<DT>::elem T;
@@ -228,33 +254,20 @@ __global__ __launch_bounds__(256) void nm_dense_pack_kernel(const typename NmTyp
     if (step >= steps) return;
     const int c = nm_d_column<DT>(tile, lane & 15);
     const long long q0 = 32 * step + 8 * h, s0 = nm_d_window(q0, Q);
-    T e[8];
+    NmOct<DT> o = nm_oct_zero<DT>();
     if (!trans) {
-        NmOct<DT> o = nm_oct_zero<DT>();
         if (c < C) {
             const T* row = w + (long long)c * ldw;
             if (Q < 8) { if (q0 == 0) o = nm_oct_load_short<DT>(row, Q); }
             else o = nm_oct_clear_first<DT>(nm_oct_load<DT>(row + s0), (int)(q0 - s0 < 8 ? q0 - s0 : 8));
         }
-        __builtin_memcpy(e, &o, sizeof(o));
     } else {
+        T e[8];
 #pragma unroll
         for (int k = 0; k < 8; ++k) e[k] = c < C && s0 + k < Q && s0 + k >= q0 ? w[(s0 + k) * ldw + c] : (T)0.f;
+        __builtin_memcpy(&o, e, sizeof(o));
     }
-    uint4* d = dst + ((step * tiles + tile) * NmPlanes<DT>::W) * 64 + lane;
-    if constexpr (DT == NM_F32) {
-        float f[8];
-        uint4 p[3];
-#pragma unroll
-        for (int k = 0; k < 8; ++k) f[k] = e[k];
-        nm_d_cut8(f, p);
-#pragma unroll
-        for (int q = 0; q < 3; ++q) d[q * 64] = p[q];
-    } else {
-        uint4 p;
-        __builtin_memcpy(&p, e, 16);
-        *d = p;
-    }
+    nm_d_put_weights<DT, PW>(o, dst + ((step * tiles + tile) * PW) * 64 + lane);
 }
 
 // ------------------------------------------------------------------------------------------------ rows x weights
@@ -289,7 +302,7 @@ __device__ __forceinline__ void nm_d_operand(const NmOct<DT>& a, const NmOct<NmF
             for (int e = 0; e < 8; ++e) f[e] *= g[e];
         }
         if constexpr (DT == NM_F32) nm_d_cut8(f, x);
-        else nm_d_two8<DT>(f, x);
+        else nm_d_two8(f, x);
     }
 }
 
@@ -395,10 +408,9 @@ __device__ __forceinline__ float nm_d_bias(const NmDenseArgs& p, int c) {
 }
 
 // a weight block -> LDS in fragment order, [step][tile][plane][lane], by 512 threads; zero beyond C and Q
-template <int DT, int NP>
+template <int DT, int PW, int NP>
 __device__ __forceinline__ void nm_d_load_block(const NmDenseArgs& p, int cb, int steps, uint4* lds, int t) {
     typedef typename NmType<DT>::elem T;
-    constexpr int PW = NmPlanes<DT>::W;
     const T* w = (const T*)p.W;
     if (!p.trans) {                                          // a lane's eight contraction elements lie on end: one piece each
         const int n = steps * 2 * NP * 64;
@@ -408,18 +420,7 @@ __device__ __forceinline__ void nm_d_load_block(const NmDenseArgs& p, int cb, in
             const int c = cb * (32 * NP) + nm_d_column<DT>(tile, lane & 15), q0 = 32 * s + 8 * (lane >> 4);
             NmOct<DT> o = nm_d_fetch<DT>(w + (long long)(c < p.C ? c : p.C - 1) * p.ldw, q0, p.Q);
             const int sh = c >= p.C ? 8 : p.Q < 8 || q0 + 8 <= p.Q ? 0 : q0 + 8 - p.Q;
-            o = nm_oct_clear_first<DT>(o, sh);
-            uint4* d = lds + (i >> 6) * (PW * 64) + lane;
-            if constexpr (DT == NM_F32) {
-                float f[8];
-                uint4 x[3];
-                nm_oct_to_float<DT>(o, f);
-                nm_d_cut8(f, x);
-#pragma unroll
-                for (int q = 0; q < 3; ++q) d[q * 64] = x[q];
-            } else {
-                *d = o.v[0];
-            }
+            nm_d_put_weights<DT, PW>(nm_oct_clear_first<DT>(o, sh), lds + (i >> 6) * (PW * 64) + lane);
         }
         return;
     }
@@ -440,25 +441,24 @@ __device__ __forceinline__ void nm_d_load_block(const NmDenseArgs& p, int cb, in
             // tile and position of column 8 g + e of the block
             const int tile = DT == NM_F32 ? g >> 1 : 2 * (g >> 2) + (e >> 2), pos = DT == NM_F32 ? 8 * (g & 1) + e : 4 * (g & 3) + (e & 3);
             uint4* d = lds + ((qg >> 2) * (2 * NP) + tile) * (PW * 64) + 16 * (qg & 3) + pos;
+            NmOct<DT> o;
             if constexpr (DT == NM_F32) {
                 float f[8], a[8];
-                uint4 x[3];
 #pragma unroll
                 for (int k = 0; k < 8; ++k) {
                     nm_oct_to_float<DT>(v[k], a);
                     f[k] = a[e];
                 }
-                nm_d_cut8(f, x);
-#pragma unroll
-                for (int q = 0; q < 3; ++q) d[q * 64] = x[q];
+                __builtin_memcpy(&o, f, sizeof(o));
             } else {
                 const unsigned sel = (e & 1) ? 0x07060302u : 0x05040100u;
                 unsigned r[8];
 #pragma unroll
                 for (int k = 0; k < 8; ++k) r[k] = (e >> 1) == 0 ? v[k].v[0].x : (e >> 1) == 1 ? v[k].v[0].y : (e >> 1) == 2 ? v[k].v[0].z : v[k].v[0].w;
-                *d = make_uint4(__builtin_amdgcn_perm(r[1], r[0], sel), __builtin_amdgcn_perm(r[3], r[2], sel), __builtin_amdgcn_perm(r[5], r[4], sel),
-                                __builtin_amdgcn_perm(r[7], r[6], sel));
+                o.v[0] = make_uint4(__builtin_amdgcn_perm(r[1], r[0], sel), __builtin_amdgcn_perm(r[3], r[2], sel), __builtin_amdgcn_perm(r[5], r[4], sel),
+                                    __builtin_amdgcn_perm(r[7], r[6], sel));
             }
+            nm_d_put_weights<DT, PW>(o, d);
         }
     }
 }
@@ -474,7 +474,7 @@ __device__ __forceinline__ void nm_d_load_block(const NmDenseArgs& p, int cb, in
 template <int DT, bool PROD, int NP>
 __global__ __launch_bounds__(512, 2) void nm_dense_resident_kernel(NmDenseArgs p) {
     typedef typename NmType<DT>::elem T;
-    constexpr int PW = NmPlanes<DT>::W, PX = DT == NM_F32 ? 3 : PROD ? 2 : 1, DD = NmFactor<DT>::T;
+    constexpr int PW = NmPieces<DT, PROD>::PLAIN, PX = NmPieces<DT, PROD>::ROWS, MF = NmPieces<DT, PROD>::MF, DD = NmFactor<DT>::T;
     constexpr int RING = DT == NM_F32 || (PROD && NP == 8) ? 2 : 4;
     __shared__ uint4 lds[NM_D_RESIDENT * 64];
     __shared__ float bias[32 * NP];
@@ -513,7 +513,7 @@ __global__ __launch_bounds__(512, 2) void nm_dense_resident_kernel(NmDenseArgs p
         for (int u = 0; u < RING; ++u)
             if (u < steps) fetch(u, xa[u], xd[u]);
     }
-    nm_d_load_block<DT, NP>(p, cb, steps, lds, t);
+    nm_d_load_block<DT, PW, NP>(p, cb, steps, lds, t);
     if (!PROD && p.bias && t < 32 * NP) bias[t] = nm_d_bias<DT>(p, cb * (32 * NP) + t);
     __syncthreads();
     for (; tile < tiles; tile += slots * 8) {
@@ -553,7 +553,7 @@ __global__ __launch_bounds__(512, 2) void nm_dense_resident_kernel(NmDenseArgs p
 #pragma unroll
                     for (int q = 0; q < PW; ++q) w[q] = lds[((s * (2 * NP) + n) * PW + q) * 64 + lane];
 #pragma unroll
-                    for (int r = 0; r < 2; ++r) acc[r][n] = nm_d_products<DT>(w, x[r], acc[r][n]);
+                    for (int r = 0; r < 2; ++r) acc[r][n] = nm_d_products<MF>(w, x[r], acc[r][n]);
                 }
             }
         }
@@ -652,7 +652,7 @@ __global__ __launch_bounds__(512, 2) void nm_dense_tile_kernel(NmDenseArgs p) {
 template <int DT, bool PROD, int RT, int NP, int PS>
 __global__ __launch_bounds__(256, 2) void nm_dense_stream_kernel(NmDenseArgs p) {
     typedef typename NmType<DT>::elem T;
-    constexpr int PW = NmPlanes<DT>::W, PX = DT == NM_F32 ? 3 : PROD ? 2 : 1, DD = NmFactor<DT>::T;
+    constexpr int PW = NmPieces<DT, PROD>::PLAIN, PX = NmPieces<DT, PROD>::ROWS, MF = NmPieces<DT, PROD>::MF, DD = NmFactor<DT>::T;
     constexpr int STEP = 2 * NP * PW * 64, PANEL = PS * STEP, WV = PANEL / 256;      // uint4
     static_assert(PANEL % 256 == 0, "a panel is whole 16-byte pieces per thread");
     __shared__ uint4 lds[2][PANEL];
@@ -728,7 +728,7 @@ __global__ __launch_bounds__(256, 2) void nm_dense_stream_kernel(NmDenseArgs p) 
 #pragma unroll
                 for (int q = 0; q < PW; ++q) w[q] = lds[buf][((s * (2 * NP) + n) * PW + q) * 64 + lane];
 #pragma unroll
-                for (int r = 0; r < RT; ++r) acc[r][n] = nm_d_products<DT>(w, x[r], acc[r][n]);
+                for (int r = 0; r < RT; ++r) acc[r][n] = nm_d_products<MF>(w, x[r], acc[r][n]);
             }
         }
     };
@@ -917,7 +917,7 @@ __global__ __launch_bounds__(256, 2) void nm_dense_grad_kernel(NmDenseGradArgs p
     typedef typename NmType<DT>::elem T;
     constexpr int DD = NmFactor<DT>::T, CG = NmGroup<DT>::C;
     typedef typename NmType<DD>::elem TD;
-    constexpr int PZ = DT == NM_F32 ? 3 : PROD ? 2 : 1, PX = DT == NM_F32 ? 3 : 1;
+    constexpr int PZ = NmPieces<DT, PROD>::ROWS, PX = NmPieces<DT, PROD>::PLAIN, MF = NmPieces<DT, PROD>::MF;
     constexpr int LANES = 128 / CG;                          // lanes side by side
     constexpr int ROWS = 8 * 4 * (64 / LANES), STEPS = ROWS / 16;
     __shared__ uint4 lds[(PZ + PX) * STEPS * 256];           // [plane][step][tile 4][lane 64], dz then x
@@ -978,13 +978,22 @@ __global__ __launch_bounds__(256, 2) void nm_dense_grad_kernel(NmDenseGradArgs p
             } else {
                 if constexpr (PROD) {
                     uint4 c[2];
-                    nm_d_two8<DT>(f, c);
+                    nm_d_two8(f, c);
                     put(lds, c[0], e);
                     put(lds + STEPS * 256, c[1], e);
                 } else {
                     put(lds, nm_d_column16(vg, e), e);
                 }
-                put(lds + LZ, nm_d_column16(vx, e), e);
+                if constexpr (PX == 2) {
+                    uint4 c[2];
+#pragma unroll
+                    for (int r = 0; r < 8; ++r) f[r] = nm_d_element<DT>(vx[r], e);
+                    nm_d_two8(f, c);
+                    put(lds + LZ, c[0], e);
+                    put(lds + LZ + STEPS * 256, c[1], e);
+                } else {
+                    put(lds + LZ, nm_d_column16(vx, e), e);
+                }
             }
         }
     };
@@ -1009,7 +1018,7 @@ __global__ __launch_bounds__(256, 2) void nm_dense_grad_kernel(NmDenseGradArgs p
 #pragma unroll
             for (int i = 0; i < 2; ++i)
 #pragma unroll
-                for (int j = 0; j < 2; ++j) acc[i][j] = nm_d_products<DT>(z[i], x[j], acc[i][j]);
+                for (int j = 0; j < 2; ++j) acc[i][j] = nm_d_products<MF>(z[i], x[j], acc[i][j]);
         }
         __syncthreads();
     }
@@ -1111,7 +1120,7 @@ struct NmDensePlan { bool resident, tile; int np, tiles, col_blocks, rt; long lo
 // columns C, contraction Q, rows R: which kernel, and its column blocks of 32 np columns
 static NmDensePlan nm_d_plan(int dt, bool prod, bool res, bool trans, long long R, long long C, long long Q) {
     NmDensePlan p;
-    const int pieces = dt == NM_F32 ? 3 : 1;
+    const int pieces = nm_d_pieces(dt, prod);
     const long long steps = nm_d_up(Q, 32);
     p.np = C > 128 ? 8 : C > 64 ? 4 : C > 32 ? 2 : 1;
     int fit = pieces == 3 && p.np == 8 ? 4 : p.np;           // (three pieces of sixteen tiles leave no registers)
@@ -1195,10 +1204,10 @@ static int nm_d_launch(const NmDensePlan& pl, NmDenseArgs a, hipStream_t stream)
     return 0;
 }
 
-template <int DT>
+template <int DT, bool PROD>
 static int nm_d_pack(const NmDensePlan& pl, const NmDenseArgs& a, char* ws, hipStream_t stream) {
     if (pl.resident || pl.tile || pl.steps == 0) return 0;
-    hipLaunchKernelGGL((nm_dense_pack_kernel<DT>), dim3((unsigned)nm_d_up(pl.steps * pl.tiles * 64, 256)), dim3(256), 0, stream, (const typename NmType<DT>::elem*)a.W,
+    hipLaunchKernelGGL((nm_dense_pack_kernel<DT, NmPieces<DT, PROD>::PLAIN>), dim3((unsigned)nm_d_up(pl.steps * pl.tiles * 64, 256)), dim3(256), 0, stream, (const typename NmType<DT>::elem*)a.W,
                        a.ldw, a.trans, a.C, a.Q, pl.tiles, (int)pl.steps, (uint4*)ws);
     NM_LAUNCH_CHECK();
     return 0;
@@ -1226,7 +1235,7 @@ static int nm_d_forward(const void* x, long long ldx, const void* w, long long l
     NmDenseArgs a = {};
     a.A = x; a.lda = ldx; a.W = w; a.ldw = ldw; a.P = (const uint4*)ws; a.bias = bias; a.bias_f32 = bias_dt == NM_F32;
     a.res = res; a.ldr = ldr; a.Y = y; a.ldy = ldy; a.DV = deriv; a.R = M; a.Q = K; a.C = N; a.act = act; a.beta = beta;
-    if (nm_d_pack<DT>(pl, a, ws, stream)) return 1;
+    if (nm_d_pack<DT, false>(pl, a, ws, stream)) return 1;
     return nm_d_launch<DT, false>(pl, a, stream);
 }
 
@@ -1238,7 +1247,7 @@ static int nm_d_backward(const void* g, long long ldg, const void* deriv, const 
         const NmDensePlan pl = nm_d_plan(DT, deriv != nullptr, false, true, M, K, N);
         NmDenseArgs a = {};
         a.A = g; a.lda = ldg; a.D = deriv; a.W = w; a.ldw = ldw; a.trans = 1; a.P = (const uint4*)ws; a.Y = dx; a.ldy = lddx; a.R = M; a.Q = N; a.C = K; a.act = NM_ACT_NONE; a.beta = 1.f;
-        if (nm_d_pack<DT>(pl, a, ws, stream)) return 1;
+        if (deriv ? nm_d_pack<DT, true>(pl, a, ws, stream) : nm_d_pack<DT, false>(pl, a, ws, stream)) return 1;
         if (deriv ? nm_d_launch<DT, true>(pl, a, stream) : nm_d_launch<DT, false>(pl, a, stream)) return 1;
         ws += pl.bytes;
     }
@@ -1289,7 +1298,8 @@ int64_t nm_dense_workspace_bytes(int64_t M, int64_t K, int64_t N, int dtype, int
     }
     // (the bias gradient alone is a plan of its own: one block of columns, more splits)
     const long long both = nm_d_grad_plan(M, N, K).bytes, bias = nm_d_grad_plan(M, N, 1).bytes;
-    return nm_d_plan(dtype, false, false, true, M, K, N).bytes + (both > bias ? both : bias);
+    const long long plain = nm_d_plan(dtype, false, false, true, M, K, N).bytes, prod = nm_d_plan(dtype, true, false, true, M, K, N).bytes;      // (deriv given or not)
+    return (plain > prod ? plain : prod) + (both > bias ? both : bias);
 }
 
 int nm_dense_forward(const void* x, int64_t ldx, const void* weight, int64_t ldw, const void* bias, int bias_dtype, const void* residual, int64_t ldr, int64_t M,

@@ -156,7 +156,8 @@ def dense(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] = 
     bias may be fp32 beside 16-bit rows).  activation: one of ACTIVATIONS; softplus is log(1 + exp(beta z)) / beta (100 as in the
     geometry network), GELU its tanh form.  Differentiable in all four tensors.  Rows may be strided (a column slice of a wider tensor); other
     layouts are copied.  One row to many: up to 8 rows go through a form that reads the weights once and in place.
-    fp32 products are as accurate as an fp32 matrix product; a non-finite operand makes the outputs it enters NaN there."""
+    fp32 products are as accurate as an fp32 matrix product; a non-finite operand makes the outputs it enters NaN there, and so in gradients
+    beside an activation."""
     if activation not in ACTIVATIONS:
         raise ValueError(f"dense: activation={activation!r}, expected one of {sorted(ACTIVATIONS)}")
     if not isinstance(x, torch.Tensor) or not isinstance(weight, torch.Tensor) or weight.dim() != 2 or x.dim() < 1 or x.shape[-1] != weight.shape[1]:

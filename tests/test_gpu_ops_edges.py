@@ -48,3 +48,109 @@ def test_gradient_of_a_shared_gate_over_no_channels(types):
     out = ops.composite_features(alpha, torch.rand(5, 60, 0, device="cuda"))
     torch.full((300,), float("nan"), device="cuda")
     assert (torch.autograd.grad(out, alpha, torch.ones_like(out))[0] == 0).all()
+
+
+# ------------------------------------------------------------------------------------------------ gradients of dense over the ranges of their types
+def derivative(act, z, beta):
+    """act'(z) in 64 bits, the size of its terms (what its evaluation's relative errors act on), |act''| at most over a small neighbourhood of z, and |u| of the exponential exp(-|u|)."""
+    if act == "softplus":
+        d = torch.sigmoid(beta * z)
+        return d, d, beta * d, beta * z.abs()
+    c1, c3 = (2 * (2 / torch.pi) ** 0.5, 0.044715) if act == "gelu_tanh" else (1.0, 0.0)
+    u, du = c1 * (z + c3 * z ** 3), c1 * (1 + 3 * c3 * z * z)
+    q, q1 = torch.sigmoid(u), torch.sigmoid(-u)
+    if act == "sigmoid":
+        return q * q1, q * q1, q * q1, u.abs()
+    size = q + z.abs() * q * q1 * du
+    # (q + z q q1 u')' = 2 q q1 u' + z q q1 (u'^2 (1 - 2 q) + u'')
+    return q + z * q * q1 * du, size, q * q1 * (2 * du + z.abs() * (du * du + 6 * c1 * c3 * z.abs())), u.abs()
+
+
+def gradient_bounds(x, w, b, act, beta, g, keep):
+    """64-bit dx, dW, db and elementwise bounds.  Nothing absolute stands in them but the last rounding of each result: act' is kept to `keep` of itself, dz = g act' enters
+    the products with 16 bits at least (fp32: in three exact pieces), sums are fp32."""
+    t = x.dtype
+    u32 = 2.0 ** -23                                          # one operation of a matrix instruction may truncate
+    half, tiny = torch.finfo(t).eps / 2, torch.finfo(t).smallest_normal * torch.finfo(t).eps / 2
+    x, w, b, g = (v.detach().double().cpu() for v in (x, w, b, g))
+    K, N, M = x.shape[1], w.shape[0], x.shape[0]
+    extra = 2.0 ** -21 if t == torch.float32 else 0.0        # piece products that are dropped
+    z = x @ w.t() + b
+    ez = ((K + 2) * u32 + extra) * (x.abs() @ w.abs().t() + b.abs())
+    d, size, curve, u = derivative(act, z, beta)
+    # the exponential's argument is rounded three times, exponential and reciprocal are off by 1e-6 in all
+    ed = curve * 1.01 * ez + (2e-6 + 4 * 2.0 ** -24 * u) * size + keep * d.abs()
+    dz = g * d
+    edz = g.abs() * ed + (0.0 if t == torch.float32 else 2.0 ** -16) * dz.abs() + u32 * dz.abs()
+
+    def out(v, e):
+        return v, e + half * (v.abs() + e) + tiny
+    return (out(dz @ w, edz @ w.abs() + ((N + 2) * u32 + extra) * (dz.abs() @ w.abs())),
+            out(dz.t() @ x, edz.t() @ x.abs() + ((M + 2) * u32 + extra) * (dz.abs().t() @ x.abs())),
+            out(dz.sum(0), edz.sum(0) + (M + 2) * u32 * dz.abs().sum(0)))
+
+
+def check_gradients(x, w, b, act, beta, g, keep, what):
+    v = [p.detach().clone().requires_grad_(True) for p in (x, w, b)]
+    got = torch.autograd.grad(ops.dense(*v, activation=act, beta=beta), v, g)
+    for name, p, (want, bound) in zip(("d_x", "d_weight", "d_bias"), got, gradient_bounds(x, w, b, act, beta, g, keep)):
+        off = (p.double().cpu() - want).abs()
+        assert (off <= bound).all(), f"{what} {name}: {int((~(off <= bound)).sum())} of {off.numel()} off, worst {float((off / bound).nan_to_num(1e9).max()):.3g} x the bound"
+        tiny = torch.finfo(p.dtype).smallest_normal * torch.finfo(p.dtype).eps
+        assert (want.abs() > 4 * bound).float().mean() > 0.5 or want.abs().max() < 64 * tiny, f"{what} {name}: the bound says nothing"
+
+
+# few rows; resident weights; streamed weights and a gradient without a split; many rows and a split gradient
+GRAD_SIZES = [(5, 24, 40), (300, 130, 70), (1500, 520, 700), (70000, 40, 24)]
+SCALES = {"fp16": (2.0 ** -24, 2.0 ** -21, 2.0 ** -17, 2.0 ** -12, 1.0), "bf16": (1e-30, 1e-12, 1e25), "fp32": (1e-25, 1e-6, 1e25)}
+TYPES = {"fp32": torch.float32, "fp16": torch.float16, "bf16": torch.bfloat16}
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("size", GRAD_SIZES, ids=lambda s: "x".join(map(str, s)))
+def test_dense_gradients_of_small_and_large_cotangents(size, dtype):
+    """Cotangents over the range of their type: those of a mean over many outputs (fp16: down to its smallest number) as exact as those of size one."""
+    (M, K, N), t = size, TYPES[dtype]
+    gen = torch.Generator().manual_seed(M + K)
+    for i, scale in enumerate(SCALES[dtype]):
+        # all of one sign, so that the sums keep what their terms have; z within a few units of 0
+        x, w = 0.5 + torch.rand(M, K, generator=gen), (0.5 + torch.rand(N, K, generator=gen)) / K
+        b, g = torch.randn(N, generator=gen) * 0.3 - 0.5, (1 + torch.rand(M, N, generator=gen)) * scale
+        x, w, b, g = (v.to(t).cuda() for v in (x, w, b, g))
+        check_gradients(x, w, b, ("sigmoid", "silu", "softplus", "gelu_tanh", "sigmoid")[i], 1.0, g, 2.0 ** -11, f"{scale:g}")
+
+
+@pytest.mark.parametrize("size", GRAD_SIZES, ids=lambda s: "x".join(map(str, s)))
+def test_dense_fp16_cotangents_near_the_maximum(size):
+    """g act' beyond fp16's range (act' up to 1.13) inside, finite results outside."""
+    M, K, N = size
+    gen = torch.Generator().manual_seed(M)
+    for act, z in (("gelu_tanh", 1.4), ("silu", 2.4)):
+        x, w = 2.0 ** -14 * (1 + torch.rand(M, K, generator=gen)), 2.0 ** -12 * (1 + torch.rand(N, K, generator=gen))
+        b, g = z + 0.1 * torch.rand(N, generator=gen), 61000 + 4000 * torch.rand(M, N, generator=gen)
+        if M > 10000:                                         # (dW within fp16: most rows without a cotangent)
+            g[torch.rand(M, 1, generator=gen).expand(M, N) < 0.95] = 0
+        x, w, g = (v.half().cuda() for v in (x, w, g))
+        b = b.cuda()
+        v = [p.clone().requires_grad_(True) for p in (x, w, b)]
+        dx, dw, db = torch.autograd.grad(ops.dense(*v, activation=act), v, g)
+        dz = g.double() * derivative(act, x.double() @ w.double().t() + b.double(), 1.0)[0]
+        assert dz.max() > 65504 and dx.isfinite().all() and dw.isfinite().all() and db.isfinite().all()
+        for name, p, (want, bound) in zip(("d_x", "d_weight"), (dx, dw), gradient_bounds(x, w, b, act, 1.0, g, 2.0 ** -11)):
+            off = (p.double().cpu() - want).abs()
+            assert (off <= bound).all(), f"{act} {name}: worst {float((off / bound).max()):.3g} x the bound"
+
+
+def test_dense_fp16_infinities_in_the_cotangent_stay_in_their_rows():
+    x, w = torch.randn(200, 41, device="cuda").half(), torch.randn(19, 41, device="cuda").half()
+    g = torch.randn(200, 19, device="cuda").half()
+    bad = g.clone()
+    bad[3, 4], bad[100, 18] = float("inf"), float("nan")
+    grads = []
+    for c in (g, bad):
+        v = [p.clone().requires_grad_(True) for p in (x, w)]
+        grads.append(torch.autograd.grad(ops.dense(*v, activation="silu"), v, c))
+    rows = [i for i in range(200) if i not in (3, 100)]
+    cols = [i for i in range(19) if i not in (4, 18)]
+    assert torch.equal(grads[0][0][rows], grads[1][0][rows]) and not grads[1][0][[3, 100]].isfinite().any()
+    assert torch.equal(grads[0][1][cols], grads[1][1][cols]) and not grads[1][1][[4, 18]].isfinite().any()
