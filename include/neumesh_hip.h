@@ -39,7 +39,7 @@
 extern "C" {
 #endif
 
-#define NM_ABI_VERSION 12
+#define NM_ABI_VERSION 13
 #define NM_MAX_K 32
 
 typedef struct nm_grid_s* nm_grid_t;    /* spatial index over the mesh vertices */
@@ -397,9 +397,8 @@ int nm_train_composite_backward(const float* sdf, const float* s, const float* d
  * of one element type (the bias: that type or fp32), last axis contiguous, any element alignment.  K, N <= 2^20, strides <= 2^24; zero sizes are allowed
  * (K = 0: y = act(b) + r).  Products accumulate in fp32 and are rounded once, at the end.
  * act: softplus is log(1 + exp(beta z)) / beta (beta > 0; other activations ignore it), GELU in its tanh form.
- * deriv [M,N] contiguous, 2 bytes per element beside 16-bit rows, 4 beside fp32 rows: act'(z) in a form of the library's own, what the backward
- * pass needs; NULL = not wanted.  With
- * NM_ACT_NONE nothing is written and the backward pass takes NULL.
+ * deriv: M N elements of 3 bytes beside 16-bit rows, of 4 beside fp32 rows (2-byte / 4-byte aligned): act'(z) in a form of the library's own, what the
+ * backward pass needs; NULL = not wanted.  With NM_ACT_NONE nothing is written and the backward pass takes NULL.
  * nm_dense_backward: g [M,N] cotangent of y -> dx [M,K] (lddx), dweight [N,K] contiguous, dbias [N] (NULL = not wanted; overwritten, not added to).  The
  * gradient of r is g itself.  The result does not change from run to run.  fp32, and gradients with deriv: a non-finite operand makes the
  * outputs it enters NaN where IEEE arithmetic may give an infinity.

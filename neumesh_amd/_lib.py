@@ -11,7 +11,7 @@ import os
 
 from . import build as _build
 
-ABI_VERSION = 12
+ABI_VERSION = 13
 MAX_K = 32
 
 

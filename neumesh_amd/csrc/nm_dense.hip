@@ -11,37 +11,91 @@
 // nm_dense_few_kernel serves 1 .. 8 rows (a probe, a picked point).
 //
 // Arithmetic.  16-bit inputs: one product per pair on the f16 / bf16 pipe, fp32 accumulation, fp32 epilogue, one rounding at the end.  The forward pass
-// keeps act'(z) for the backward pass in 16 bits that are finer than the rows' own (NmFactor).  dz = g act'(z) enters the products as TWO bf16
+// keeps act'(z) for the backward pass (NmFactor).  dz = g act'(z) enters the products as TWO bf16
 // pieces (value + residual: 16 bits, over fp32's whole range): a single rounded piece put an error as large as the output's own rounding on dx and
 // dW, and fp16 pieces lost what lies below 2^-13 (g of a mean over many outputs) and beyond 65504 (g near the maximum times act' = 1.13).
 // Beside fp16 rows the other operand is cut into two bf16 pieces as well, exactly, and three piece products are taken (10007 x 177 -> 131 forward and
 // backward 123 us, 126 with two products of fp16 pieces).  fp32 inputs: every operand cut into three bf16 pieces (nm_gemm.h: exact), six piece
-// products, fp32 accumulation; act'(z) is kept in fp32.  A product of several pieces with a non-finite operand is NaN where IEEE arithmetic may
+// products, fp32 accumulation.  A product of several pieces with a non-finite operand is NaN where IEEE arithmetic may
 // give an infinity.
 #include "nm_error.h"
 #include "nm_num.h"
 
-// act'(z) in 16 bits, values in (-2, 2).  Beside bf16 rows (8 bits): fp16 (11 bits).  Beside fp16 rows: fp16 with one bit of exponent traded for one of
-// mantissa -- 4 bits of exponent, 1.0 = 2^0 at the top of the range, 12 significant bits down to 2^-14, steps of 2^-25 below; all ones is NaN --
-// so that keeping act' does not cost what rounding the result costs.
-enum { NM_ACT16 = 3 };
-template <> struct NmType<NM_ACT16> { typedef unsigned short elem; };
-template <>
-__device__ __forceinline__ float nm_to_float<NM_ACT16>(unsigned short b) {
-    const unsigned m = b & 0x7fffu;
-    const unsigned f = __float_as_uint(__uint_as_float(m << 12) * 0x1p112f) | ((unsigned)(b & 0x8000u) << 16);
-    return m == 0x7fffu ? __builtin_nanf("") : __uint_as_float(f);
-}
-template <>
-__device__ __forceinline__ unsigned short nm_from_float<NM_ACT16>(float d) {
-    const unsigned m = (__float_as_uint(fabsf(d) * 0x1p-112f) + 0x800u) >> 12;
-    return (unsigned short)(d != d ? 0x7fffu : m | ((__float_as_uint(d) >> 16) & 0x8000u));
-}
-template <int DT> struct NmFactor { static constexpr int T = DT == NM_F32 ? (int)NM_F32 : DT == NM_F16 ? (int)NM_ACT16 : (int)NM_F16; };
+#include <utility>
 
 #define NM_D_MAX_DIM (1 << 20)   // columns and contraction lengths fit 32-bit arithmetic with room
 #define NM_D_MAX_LD (1 << 24)    // 64 rows of any stride stay below 2^32 bytes
 #define NM_D_MAX_THREADS 0xffffffffLL    // of one launch
+
+// ------------------------------------------------------------------------------------------------ kept derivatives
+// act'(z) of [R, C] outputs, contiguous, from the forward to the backward pass.  Beside fp32 rows: fp32.  Beside 16-bit rows: the upper 24 bits of the
+// fp32 value, rounded: 16 significant bits, as many as dz has in the products, and fp32's exponent, so that a unit deep in the tail of its activation keeps
+// its gradient (fp16 had steps of 2^-24: sigmoid' 3 % off at -15 and 0 at -18).  Two planes: upper halves [R, C], 16 bits each, then the third
+// bytes [R, C].  Three bytes and not four because the buffer is written once and read twice, in layers that are bound by memory.
+template <int DT> struct NmFactor {                          // a row (or any place) of the planes
+    const char* hi; const char* lo;
+    static constexpr int E = DT == NM_F32 ? 4 : 2;           // bytes per element of the first plane
+    __device__ __forceinline__ NmFactor at(long long i) const { return {hi + i * E, DT == NM_F32 ? nullptr : lo + i}; }
+};
+template <int DT> struct NmFactorOct { uint4 hi[DT == NM_F32 ? 2 : 1]; uint2 lo; };       // eight of them
+
+// the planes that start at `base`, n elements
+template <int DT>
+__host__ __device__ __forceinline__ NmFactor<DT> nm_d_planes(const void* base, long long n) { return {(const char*)base, DT == NM_F32 || !base ? nullptr : (const char*)base + 2 * n}; }
+
+// upper half (h = 0, 1) of a word of the first plane and byte k of a word of the second -> the value
+template <int H, int K>
+__device__ __forceinline__ float nm_d_join(unsigned hi, unsigned lo) {
+    return __uint_as_float(__builtin_amdgcn_perm(hi, lo, (unsigned)(5 + 2 * H) << 24 | (unsigned)(4 + 2 * H) << 16 | (unsigned)K << 8 | 0x0cu));
+}
+__device__ __forceinline__ unsigned nm_d_round24(float d) { return d != d ? 0x7fc00000u : __float_as_uint(d) + 0x80u; }
+
+template <int DT>
+__device__ __forceinline__ void nm_d_factors(const NmFactorOct<DT>& o, float (&f)[8]) {
+    if constexpr (DT == NM_F32) {
+        __builtin_memcpy(f, &o, 32);
+    } else {
+        unsigned w[4];
+        __builtin_memcpy(w, &o, 16);
+        f[0] = nm_d_join<0, 0>(w[0], o.lo.x); f[1] = nm_d_join<1, 1>(w[0], o.lo.x); f[2] = nm_d_join<0, 2>(w[1], o.lo.x); f[3] = nm_d_join<1, 3>(w[1], o.lo.x);
+        f[4] = nm_d_join<0, 0>(w[2], o.lo.y); f[5] = nm_d_join<1, 1>(w[2], o.lo.y); f[6] = nm_d_join<0, 2>(w[3], o.lo.y); f[7] = nm_d_join<1, 3>(w[3], o.lo.y);
+    }
+}
+// eight from place q of a row of Q on, by the rule of nm_d_fetch: rows of eight or more in one whole load that ends at Q at the latest
+template <int DT>
+__device__ __forceinline__ NmFactorOct<DT> nm_d_fetch_factors(const NmFactor<DT>& row, int q, int Q) {
+    NmFactorOct<DT> o;
+    if (Q >= 8) {                                            // (uniform)
+        const NmFactor<DT> from = row.at(q + 8 <= Q ? q : Q - 8);
+        __builtin_memcpy(&o.hi, from.hi, sizeof(o.hi));
+        if constexpr (DT != NM_F32) __builtin_memcpy(&o.lo, from.lo, 8);
+        return o;
+    }
+    const int n = q == 0 ? Q : 0;
+    __builtin_memset(&o, 0, sizeof(o));
+    if constexpr (DT == NM_F32) {
+        const NmOct<NM_F32> v = nm_oct_load_short<NM_F32>((const float*)row.hi, n);
+        __builtin_memcpy(&o.hi, &v, sizeof(v));
+    } else {
+        o.hi[0] = nm_oct_load_short<NM_F16>((const _Float16*)row.hi, n).v[0];
+#pragma unroll 1
+        for (int i = 0; i < n; ++i) {
+            const unsigned b = (unsigned char)row.lo[i];
+            o.lo.x |= i < 4 ? b << (8 * i) : 0u;
+            o.lo.y |= i < 4 ? 0u : b << (8 * (i - 4));
+        }
+    }
+    return o;
+}
+// its first `sh` cleared (upper halves are enough: what is left is below 2^-133, and goes with an operand that is cleared)
+template <int DT>
+__device__ __forceinline__ NmFactorOct<DT> nm_d_clear_factors(NmFactorOct<DT> o, int sh) {
+    NmOct<DT> h;
+    __builtin_memcpy(&h, &o.hi, sizeof(h));
+    h = nm_oct_clear_first<DT>(h, sh);
+    __builtin_memcpy(&o.hi, &h, sizeof(h));
+    return o;
+}
 
 // ------------------------------------------------------------------------------------------------ activations
 // Exponentials and reciprocals from the hardware's approximations; F32 (fp32 outputs) corrects them to the last place (library exponential and division:
@@ -196,7 +250,7 @@ __device__ __forceinline__ V nm_d_products(const uint4 (&a)[PA], const uint4 (&b
         c = nm_d_mfma<DT>(a[0], b[1], c);
         c = nm_d_mfma<DT>(a[1], b[0], c);
         return nm_d_mfma<DT>(a[0], b[0], c);
-    } else if constexpr (PA == 2 && PB == 2) {               // dropped: a1 b1 < 2^-18 |a||b|, of either sign
+    } else if constexpr (PA == 2 && PB == 2) {               // dropped: a1 b1 <= 2^-16 |a||b|, of either sign
         c = nm_d_mfma<DT>(a[1], b[0], c);
         c = nm_d_mfma<DT>(a[0], b[1], c);
         return nm_d_mfma<DT>(a[0], b[0], c);
@@ -273,14 +327,14 @@ __global__ __launch_bounds__(256) void nm_dense_pack_kernel(const typename NmTyp
 // ------------------------------------------------------------------------------------------------ rows x weights
 struct NmDenseArgs {
     const void* A; long long lda;        // rows [R, Q]
-    const void* D;                       // PROD: factor of every element of A (NmFactor), contiguous [R, Q]
+    const void* D;                       // PROD: factor of every element of A (kept derivatives), contiguous [R, Q]
     const void* W; long long ldw;        // column operand as it is: [C, Q], or (trans) [Q, C]
     const uint4* P; int tiles;           // ... in fragment order (streaming kernel)
     const void* bias;                    // [C] or NULL
     int trans, bias_f32;
     const void* res; long long ldr;      // added after the activation, [R, C] or NULL
     void* Y; long long ldy;              // [R, C]
-    void* DV;                            // act'(z) (NmFactor), contiguous [R, C], or NULL
+    void* DV;                            // act'(z) (kept derivatives), contiguous [R, C], or NULL
     long long R;
     int Q, C, act;
     float beta;
@@ -289,7 +343,7 @@ struct NmDenseArgs {
 
 // a piece of a row (times its factor) -> fragments
 template <int DT, bool PROD, int PX>
-__device__ __forceinline__ void nm_d_operand(const NmOct<DT>& a, const NmOct<NmFactor<DT>::T>& d, uint4 (&x)[PX]) {
+__device__ __forceinline__ void nm_d_operand(const NmOct<DT>& a, const NmFactorOct<DT>& d, uint4 (&x)[PX]) {
     if constexpr (DT != NM_F32 && !PROD) {
         x[0] = a.v[0];
     } else {
@@ -297,7 +351,7 @@ __device__ __forceinline__ void nm_d_operand(const NmOct<DT>& a, const NmOct<NmF
         nm_oct_to_float<DT>(a, f);
         if constexpr (PROD) {
             float g[8];
-            nm_oct_to_float<NmFactor<DT>::T>(d, g);
+            nm_d_factors<DT>(d, g);
 #pragma unroll
             for (int e = 0; e < 8; ++e) f[e] *= g[e];
         }
@@ -348,6 +402,45 @@ __device__ __forceinline__ void nm_d_store_cols(typename NmType<DT>::elem* row, 
     }
 }
 
+// ... of kept derivatives
+template <int DT>
+__device__ __forceinline__ void nm_d_store_factors(void* base, long long R, int C, long long m, const float (&f)[8], int c) {
+    if constexpr (DT == NM_F32) {
+        nm_d_store_cols<DT>((float*)base + m * C, f, c, C);
+    } else {
+        if (c >= C) return;
+        const NmFactor<DT> at = nm_d_planes<DT>(base, R * C).at(m * C + c);
+        char *hi = const_cast<char*>(at.hi), *lo = const_cast<char*>(at.lo);
+        unsigned u[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) u[i] = nm_d_round24(f[i]);
+        uint4 h = make_uint4(nm_d_pair(u[0], u[1]), nm_d_pair(u[2], u[3]), nm_d_pair(u[4], u[5]), nm_d_pair(u[6], u[7]));
+        uint2 l;
+        l.x = __builtin_amdgcn_perm(u[1], u[0], 0x0c0c0501u) | __builtin_amdgcn_perm(u[3], u[2], 0x05010c0cu);
+        l.y = __builtin_amdgcn_perm(u[5], u[4], 0x0c0c0501u) | __builtin_amdgcn_perm(u[7], u[6], 0x05010c0cu);
+        if (c + 8 <= C) {
+            __builtin_memcpy(hi, &h, 16);
+            __builtin_memcpy(lo, &l, 8);
+            return;
+        }
+#pragma unroll 1
+        for (int i = 0; i < C - c; ++i) {
+            const unsigned short e = (unsigned short)h.x;
+            __builtin_memcpy(hi + 2 * i, &e, 2);
+            lo[i] = (char)l.x;
+            h.x = h.x >> 16 | h.y << 16;
+            h.y = h.y >> 16 | h.z << 16;
+            h.z = h.z >> 16 | h.w << 16;
+            h.w >>= 16;
+            l.x = l.x >> 8 | l.y << 24;
+            l.y >>= 8;
+        }
+    }
+}
+
+template <typename F, int... K>
+__device__ __forceinline__ void nm_d_each(F f, std::integer_sequence<int, K...>) { (f(std::integral_constant<int, K>{}), ...); }
+
 // accumulators of 16 RT rows x 32 NP columns -> bias (in LDS), activation, residual, stores.  A load waits for every store before it: a bias read from
 // global memory here, piece by piece, cost a 131072 x 256 layer 8 of 52 us.  So the residual (RES) of eight pieces is in flight before the first store, and
 // column blocks with one that stay resident have no more than eight pieces per wave (256 x 256 tiles: six ahead, eight would spill).  The scheduling barriers keep the pieces apart, and the opaque column makes its tests, biases and
@@ -356,7 +449,7 @@ template <int DT, bool PROD, bool RES, int RT, int NP>
 __device__ __forceinline__ void nm_d_epilogue(const NmDenseArgs& p, const nm_v4f (&acc)[RT][2 * NP], const float* bias, long long m0, int cb,
                                               int lane) {
     typedef typename NmType<DT>::elem T;
-    constexpr int DD = NmFactor<DT>::T, PIECES = RT * NP, AHEAD = RT == 8 ? 6 : PIECES < 8 ? PIECES : 8;
+    constexpr int PIECES = RT * NP, AHEAD = RT == 8 ? 6 : PIECES < 8 ? PIECES : 8;
     const float ibeta = 1.0f / p.beta;
     const int cw = cb * (32 * NP) + (DT == NM_F32 ? 4 : 8) * (lane >> 4);
     NmOct<DT> rs[AHEAD];
@@ -371,10 +464,10 @@ __device__ __forceinline__ void nm_d_epilogue(const NmDenseArgs& p, const nm_v4f
     };
 #pragma unroll
     for (int k = 0; k < AHEAD; ++k) fetch(k);
-#pragma unroll
-    for (int k = 0; k < PIECES; ++k) {
+    // (written out by a template: `#pragma unroll` gives up on pieces of this size, which leaves the accumulators in scratch memory)
+    nm_d_each([&](auto piece) __attribute__((always_inline)) {
         __builtin_amdgcn_sched_barrier(0);
-        const int r = k / NP, n = k % NP;
+        constexpr int k = decltype(piece)::value, r = k / NP, n = k % NP;
         const long long m = row_of(k);
         int c = cw + 32 * n;
         asm volatile("" : "+v"(c));
@@ -390,16 +483,16 @@ __device__ __forceinline__ void nm_d_epilogue(const NmDenseArgs& p, const nm_v4f
             fetch(k + AHEAD);
         }
         if constexpr (!PROD) nm_d_act<DT == NM_F32>(p.act, p.beta, ibeta, p.DV != nullptr, z, dv);
-        if (m >= p.R) continue;
+        if (m >= p.R) return;
         if constexpr (!PROD) {
-            if (p.DV) nm_d_store_cols<DD>((typename NmType<DD>::elem*)p.DV + m * p.C, dv, c, p.C);
+            if (p.DV) nm_d_store_factors<DT>(p.DV, p.R, p.C, m, dv, c);
             if (RES && p.res) {
 #pragma unroll
                 for (int i = 0; i < 8; ++i) z[i] += q[i];
             }
         }
         nm_d_store_cols<DT>((T*)p.Y + m * p.ldy, z, c, p.C);
-    }
+    }, std::make_integer_sequence<int, PIECES>{});
 }
 
 template <int DT>
@@ -474,7 +567,7 @@ __device__ __forceinline__ void nm_d_load_block(const NmDenseArgs& p, int cb, in
 template <int DT, bool PROD, int NP>
 __global__ __launch_bounds__(512, 2) void nm_dense_resident_kernel(NmDenseArgs p) {
     typedef typename NmType<DT>::elem T;
-    constexpr int PW = NmPieces<DT, PROD>::PLAIN, PX = NmPieces<DT, PROD>::ROWS, MF = NmPieces<DT, PROD>::MF, DD = NmFactor<DT>::T;
+    constexpr int PW = NmPieces<DT, PROD>::PLAIN, PX = NmPieces<DT, PROD>::ROWS, MF = NmPieces<DT, PROD>::MF;
     constexpr int RING = DT == NM_F32 || (PROD && NP == 8) ? 2 : 4;
     __shared__ uint4 lds[NM_D_RESIDENT * 64];
     __shared__ float bias[32 * NP];
@@ -487,23 +580,24 @@ __global__ __launch_bounds__(512, 2) void nm_dense_resident_kernel(NmDenseArgs p
     const int steps = (p.Q + 31) / 32;
     const long long tiles = (p.R + 31) / 32;
     const T* arow[2];
-    const typename NmType<DD>::elem* drow[2];
+    const NmFactor<DT> planes = nm_d_planes<DT>(p.D, p.R * p.Q);
+    NmFactor<DT> drow[2];
     auto rows_of = [&](long long tile) {
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
             long long m = tile * 32 + 16 * r + li;
             m = m < p.R ? m : p.R - 1;
             arow[r] = (const T*)p.A + m * p.lda;
-            drow[r] = PROD ? (const typename NmType<DD>::elem*)p.D + m * p.Q : nullptr;
+            if constexpr (PROD) drow[r] = planes.at(m * p.Q);
         }
     };
     NmOct<DT> xa[RING][2];
-    NmOct<DD> xd[RING][2];
-    auto fetch = [&](int s, NmOct<DT> (&a)[2], NmOct<DD> (&d)[2]) {
+    NmFactorOct<DT> xd[RING][2];
+    auto fetch = [&](int s, NmOct<DT> (&a)[2], NmFactorOct<DT> (&d)[2]) {
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
             a[r] = nm_d_fetch<DT>(arow[r], 32 * s + 8 * h, p.Q);
-            if constexpr (PROD) d[r] = nm_d_fetch<DD>(drow[r], 32 * s + 8 * h, p.Q);
+            if constexpr (PROD) d[r] = nm_d_fetch_factors<DT>(drow[r], 32 * s + 8 * h, p.Q);
         }
     };
     long long tile = slot * 8 + wave;
@@ -533,11 +627,11 @@ __global__ __launch_bounds__(512, 2) void nm_dense_resident_kernel(NmDenseArgs p
 #pragma unroll
                 for (int r = 0; r < 2; ++r) {
                     NmOct<DT> a = xa[u][r];
-                    NmOct<DD> d = xd[u][r];
+                    NmFactorOct<DT> d = xd[u][r];
                     if (32 * s + 32 > p.Q && p.Q >= 8) {     // what the last whole load repeated
                         const int q = 32 * s + 8 * h, sh = q + 8 <= p.Q ? 0 : q + 8 - p.Q;
                         a = nm_oct_clear_first<DT>(a, sh);
-                        if constexpr (PROD) d = nm_oct_clear_first<DD>(d, sh);
+                        if constexpr (PROD) d = nm_d_clear_factors<DT>(d, sh);
                     }
                     nm_d_operand<DT, PROD>(a, d, x[r]);
                 }
@@ -652,7 +746,7 @@ __global__ __launch_bounds__(512, 2) void nm_dense_tile_kernel(NmDenseArgs p) {
 template <int DT, bool PROD, int RT, int NP, int PS>
 __global__ __launch_bounds__(256, 2) void nm_dense_stream_kernel(NmDenseArgs p) {
     typedef typename NmType<DT>::elem T;
-    constexpr int PW = NmPieces<DT, PROD>::PLAIN, PX = NmPieces<DT, PROD>::ROWS, MF = NmPieces<DT, PROD>::MF, DD = NmFactor<DT>::T;
+    constexpr int PW = NmPieces<DT, PROD>::PLAIN, PX = NmPieces<DT, PROD>::ROWS, MF = NmPieces<DT, PROD>::MF;
     constexpr int STEP = 2 * NP * PW * 64, PANEL = PS * STEP, WV = PANEL / 256;      // uint4
     static_assert(PANEL % 256 == 0, "a panel is whole 16-byte pieces per thread");
     __shared__ uint4 lds[2][PANEL];
@@ -665,13 +759,14 @@ __global__ __launch_bounds__(256, 2) void nm_dense_stream_kernel(NmDenseArgs p) 
     if (rb * (64 * RT) >= p.R) return;
     const int steps = (p.Q + 31) / 32, panels = (steps + PS - 1) / PS;
     const T* arow[RT];
-    const typename NmType<DD>::elem* drow[RT];
+    const NmFactor<DT> planes = nm_d_planes<DT>(p.D, p.R * p.Q);
+    NmFactor<DT> drow[RT];
 #pragma unroll
     for (int r = 0; r < RT; ++r) {
         long long m = m0 + 16 * r + li;
         m = m < p.R ? m : p.R - 1;
         arow[r] = (const T*)p.A + m * p.lda;
-        drow[r] = PROD ? (const typename NmType<DD>::elem*)p.D + m * p.Q : nullptr;
+        if constexpr (PROD) drow[r] = planes.at(m * p.Q);
     }
     nm_v4f acc[RT][2 * NP];
 #pragma unroll
@@ -681,7 +776,7 @@ __global__ __launch_bounds__(256, 2) void nm_dense_stream_kernel(NmDenseArgs p) 
 
     uint4 wv[WV];
     NmOct<DT> xa[PS][RT];
-    NmOct<DD> xd[PS][RT];
+    NmFactorOct<DT> xd[PS][RT];
     auto load_w = [&](int panel) {
 #pragma unroll
         for (int i = 0; i < WV; ++i) {
@@ -693,17 +788,17 @@ __global__ __launch_bounds__(256, 2) void nm_dense_stream_kernel(NmDenseArgs p) 
 #pragma unroll
         for (int i = 0; i < WV; ++i) lds[buf][i * 256 + t] = wv[i];
     };
-    auto load_x = [&](int panel, NmOct<DT> (&a)[PS][RT], NmOct<DD> (&d)[PS][RT]) {
+    auto load_x = [&](int panel, NmOct<DT> (&a)[PS][RT], NmFactorOct<DT> (&d)[PS][RT]) {
 #pragma unroll
         for (int s = 0; s < PS; ++s)
 #pragma unroll
             for (int r = 0; r < RT; ++r) {
                 a[s][r] = nm_d_fetch<DT>(arow[r], (panel * PS + s) * 32 + 8 * h, p.Q);
-                if constexpr (PROD) d[s][r] = nm_d_fetch<DD>(drow[r], (panel * PS + s) * 32 + 8 * h, p.Q);
+                if constexpr (PROD) d[s][r] = nm_d_fetch_factors<DT>(drow[r], (panel * PS + s) * 32 + 8 * h, p.Q);
             }
     };
     // the last panel: clear what a whole load repeated or brought beyond the row
-    auto trim = [&](int panel, NmOct<DT> (&a)[PS][RT], NmOct<DD> (&d)[PS][RT]) {
+    auto trim = [&](int panel, NmOct<DT> (&a)[PS][RT], NmFactorOct<DT> (&d)[PS][RT]) {
         if ((panel + 1) * (32 * PS) <= p.Q || p.Q < 8) return;
 #pragma unroll
         for (int s = 0; s < PS; ++s) {
@@ -711,11 +806,11 @@ __global__ __launch_bounds__(256, 2) void nm_dense_stream_kernel(NmDenseArgs p) 
 #pragma unroll
             for (int r = 0; r < RT; ++r) {
                 a[s][r] = nm_oct_clear_first<DT>(a[s][r], sh);
-                if constexpr (PROD) d[s][r] = nm_oct_clear_first<DD>(d[s][r], sh);
+                if constexpr (PROD) d[s][r] = nm_d_clear_factors<DT>(d[s][r], sh);
             }
         }
     };
-    auto compute = [&](int buf, const NmOct<DT> (&a)[PS][RT], const NmOct<DD> (&d)[PS][RT]) {
+    auto compute = [&](int buf, const NmOct<DT> (&a)[PS][RT], const NmFactorOct<DT> (&d)[PS][RT]) {
 #pragma unroll
         for (int s = 0; s < PS; ++s) {
             __builtin_amdgcn_sched_barrier(0);               // (one step's pieces at a time)
@@ -743,7 +838,7 @@ __global__ __launch_bounds__(256, 2) void nm_dense_stream_kernel(NmDenseArgs p) 
     for (int k = 0; k < panels; ++k) {
         // (a wave that is a panel ahead fills the OTHER buffer; nobody is two panels ahead: one barrier per panel)
         NmOct<DT> na[PS][RT];
-        NmOct<DD> nd[PS][RT];
+        NmFactorOct<DT> nd[PS][RT];
         if (k + 1 < panels) {
             load_w(k + 1);
             load_x(k + 1, na, nd);
@@ -804,8 +899,14 @@ __global__ __launch_bounds__(256) void nm_dense_few_kernel(const typename NmType
     float h = hv[0];
     if (res) h += (float)res[sub * ldr + n];
     y[sub * ldy + n] = (T)h;
-    if (dv) {
-        ((typename NmType<NmFactor<DT>::T>::elem*)dv)[(long long)sub * N + n] = nm_from_float<NmFactor<DT>::T>(d[0]);
+    if (!dv) return;
+    const long long at = (long long)sub * N + n;
+    if constexpr (DT == NM_F32) {
+        ((float*)dv)[at] = d[0];
+    } else {
+        const unsigned u = nm_d_round24(d[0]);
+        ((unsigned short*)dv)[at] = (unsigned short)(u >> 16);
+        ((unsigned char*)dv)[2LL * M * N + at] = (unsigned char)(u >> 8);
     }
 }
 
@@ -818,7 +919,7 @@ __global__ __launch_bounds__(256) void nm_dense_few_kernel(const typename NmType
 // SIMDs.  The next block's rows are in flight while this one is multiplied.
 // Measured: 256 x 256 weights, 131072 rows bf16 60 us (201 MB: 3.3 TB/s), 65536 rows fp32 61 us (51.5 G as six products: 840 TFLOP/s).
 struct NmDenseGradArgs {
-    const void* G; long long ldg; const void* D;   // dz = G * D (D contiguous [R, N], NmFactor, or NULL)
+    const void* G; long long ldg; const void* D;   // dz = G * D (D contiguous [R, N], kept derivatives, or NULL)
     const void* X; long long ldx;
     long long R;
     int N, K, n_tiles, k_tiles, splits;
@@ -841,50 +942,46 @@ __host__ __device__ __forceinline__ void nm_d_place(int t, int i, int& group, in
 template <int DT>
 __host__ __device__ __forceinline__ int nm_d_group(int c, int n) { return n < NmGroup<DT>::C ? 0 : c + NmGroup<DT>::C <= n ? c : n - NmGroup<DT>::C; }
 
-// 8 bytes of elements at any element-aligned address
-template <int DT> struct NmPiece { typename NmType<DT>::elem e[8 / sizeof(typename NmType<DT>::elem)]; };
-template <int DT>
-__device__ __forceinline__ uint2 nm_d_load8(const typename NmType<DT>::elem* p) {
-    uint2 v;
-    __builtin_memcpy(&v, p, 8);
-    return v;
-}
-// The thread's eight rows 8 rg .. of a block of `rows` <= full rows at row `base`, columns col .. (ncol: of the array).  An address is a uniform base and a
+// The thread's eight rows 8 rg .. of a block of `rows` <= full rows at row `base`, a piece V of columns col .. (ncol: of the array).  An address is a uniform base and a
 // 32-bit offset of the lane (strides are below 2^24): 24 addresses of 64 bits per lane cost more registers than the data.  All three forms are
 // straight code without branches per lane; rows beyond the block read its last row and are cleared.
-template <int DT>
-__device__ __forceinline__ void nm_d_load_rows(const typename NmType<DT>::elem* src, long long ld, int ncol, int col, long long base, int rows, int full, int rg,
-                                               uint2 (&v)[8]) {
-    typedef typename NmType<DT>::elem T;
-    constexpr unsigned E = sizeof(T);
+template <typename T, typename V>
+__device__ __forceinline__ void nm_d_load_rows(const T* src, long long ld, int ncol, int col, long long base, int rows, int full, int rg, V (&v)[8]) {
+    constexpr unsigned E = sizeof(T), G = sizeof(V) / E;
     const char* at = (const char*)(src + base * ld);
-    if (ncol >= (int)(8 / E) && rows == full) {              // (uniform)
+    if (ncol >= (int)G && rows == full) {                    // (uniform)
         const unsigned off = (unsigned)(rg * 8 * (unsigned)ld + col) * E;
 #pragma unroll
-        for (int r = 0; r < 8; ++r) v[r] = nm_d_load8<DT>((const T*)(at + r * ld * E + off));
+        for (int r = 0; r < 8; ++r) __builtin_memcpy(&v[r], (const T*)(at + r * ld * E + off), sizeof(V));
         return;
     }
 #pragma unroll
     for (int r = 0; r < 8; ++r) {
         const int m = rg * 8 + r < rows ? rg * 8 + r : rows - 1;
         const unsigned off = ((unsigned)m * (unsigned)ld + col) * E;
-        v[r] = make_uint2(0, 0);
-        if (ncol >= (int)(8 / E)) {
-            v[r] = nm_d_load8<DT>((const T*)(at + off));
+        v[r] = V{};
+        if (ncol >= (int)G) {
+            __builtin_memcpy(&v[r], (const T*)(at + off), sizeof(V));
         } else if (ncol > 0) {                               // fewer columns than a group: one by one, the last one again
-            NmPiece<DT> x;
+            T x[G];
 #pragma unroll
-            for (int e = 0; e < (int)(8 / E); ++e) x.e[e] = *(const T*)(at + off + (e < ncol ? e : ncol - 1) * E);
-            __builtin_memcpy(&v[r], &x, 8);
+            for (int e = 0; e < (int)G; ++e) x[e] = *(const T*)(at + off + (e < ncol ? e : ncol - 1) * E);
+            __builtin_memcpy(&v[r], x, sizeof(V));
         }
-        if (rg * 8 + r >= rows) v[r] = make_uint2(0, 0);
+        if (rg * 8 + r >= rows) v[r] = V{};
     }
 }
 template <int DT>
 __device__ __forceinline__ float nm_d_element(const uint2& v, int e) {
-    NmPiece<DT> x;
-    __builtin_memcpy(&x, &v, 8);
-    return nm_to_float<DT>(x.e[e]);
+    typename NmType<DT>::elem x[8 / sizeof(typename NmType<DT>::elem)];
+    __builtin_memcpy(x, &v, 8);
+    return nm_to_float<DT>(x[e]);
+}
+// column e of a piece of kept derivatives
+template <int DT>
+__device__ __forceinline__ float nm_d_factor(const uint2& hi, unsigned lo, int e) {
+    if constexpr (DT == NM_F32) return __uint_as_float(e ? hi.y : hi.x);
+    else return e == 0 ? nm_d_join<0, 0>(hi.x, lo) : e == 1 ? nm_d_join<1, 1>(hi.x, lo) : e == 2 ? nm_d_join<0, 2>(hi.y, lo) : nm_d_join<1, 3>(hi.y, lo);
 }
 // 16-bit elements: column e of eight rows
 __device__ __forceinline__ uint4 nm_d_column16(const uint2 (&r)[8], int e) {
@@ -915,8 +1012,8 @@ __device__ __forceinline__ void nm_d_put_grad(typename NmType<DT>::elem* dw, int
 template <int DT, bool PROD>
 __global__ __launch_bounds__(256, 2) void nm_dense_grad_kernel(NmDenseGradArgs p) {
     typedef typename NmType<DT>::elem T;
-    constexpr int DD = NmFactor<DT>::T, CG = NmGroup<DT>::C;
-    typedef typename NmType<DD>::elem TD;
+    typedef typename std::conditional<DT == NM_F32, float, unsigned short>::type TD;
+    constexpr int CG = NmGroup<DT>::C;
     constexpr int PZ = NmPieces<DT, PROD>::ROWS, PX = NmPieces<DT, PROD>::PLAIN, MF = NmPieces<DT, PROD>::MF;
     constexpr int LANES = 128 / CG;                          // lanes side by side
     constexpr int ROWS = 8 * 4 * (64 / LANES), STEPS = ROWS / 16;
@@ -942,12 +1039,15 @@ __global__ __launch_bounds__(256, 2) void nm_dense_grad_kernel(NmDenseGradArgs p
 #pragma unroll
             for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.f;
 
+    const NmFactor<DT> planes = nm_d_planes<DT>(p.D, p.R * p.N);
     uint2 vg[8], vd[8], vx[8];
+    unsigned vl[8];
     auto load = [&](long long base) {
         const int rows = r1 - base < ROWS ? (int)(r1 - base) : ROWS;
-        nm_d_load_rows<DT>((const T*)p.G, p.ldg, p.N, coln, base, rows, ROWS, rg, vg);
-        if constexpr (PROD) nm_d_load_rows<DD>((const TD*)p.D, p.N, p.N, coln, base, rows, ROWS, rg, vd);
-        nm_d_load_rows<DT>((const T*)p.X, p.ldx, p.K, colk, base, rows, ROWS, rg, vx);
+        nm_d_load_rows((const T*)p.G, p.ldg, p.N, coln, base, rows, ROWS, rg, vg);
+        if constexpr (PROD) nm_d_load_rows((const TD*)planes.hi, p.N, p.N, coln, base, rows, ROWS, rg, vd);
+        if constexpr (PROD && DT != NM_F32) nm_d_load_rows((const unsigned char*)planes.lo, p.N, p.N, coln, base, rows, ROWS, rg, vl);
+        nm_d_load_rows((const T*)p.X, p.ldx, p.K, colk, base, rows, ROWS, rg, vx);
     };
     // a fragment of this thread -> LDS: its column e, rows 8 rg ..
     auto put = [&](uint4* base, const uint4& c, int e) {
@@ -962,7 +1062,7 @@ __global__ __launch_bounds__(256, 2) void nm_dense_grad_kernel(NmDenseGradArgs p
 #pragma unroll
             for (int r = 0; r < 8; ++r) {
                 f[r] = nm_d_element<DT>(vg[r], e);
-                if constexpr (PROD) f[r] *= nm_d_element<DD>(vd[r], e);
+                if constexpr (PROD) f[r] *= nm_d_factor<DT>(vd[r], vl[r], e);
                 if (want_bias) bsum[e] += f[r];
             }
             if constexpr (DT == NM_F32) {

@@ -105,7 +105,7 @@ def _dense_forward(x, weight, bias, residual, act: int, beta: float, want_deriv:
     y = torch.empty((*x.shape[:-1], N), dtype=x.dtype, device=dev)
     r2, ldr = (None, 0) if residual is None else _rows(residual, N)
     b = None if bias is None else bias.contiguous()
-    deriv = torch.empty((M, N), dtype=torch.float32 if dt == _lib.DTYPE_F32 else torch.float16, device=dev) if want_deriv and act else None
+    deriv = torch.empty((M * N * (4 if dt == _lib.DTYPE_F32 else 3),), dtype=torch.uint8, device=dev) if want_deriv and act else None
     nbytes = lib.nm_dense_workspace_bytes(M, K, N, dt, 0)
     ws = torch.empty((nbytes,), dtype=torch.uint8, device=dev) if nbytes > 0 else None
     with _on(dev):

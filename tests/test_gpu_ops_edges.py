@@ -74,12 +74,12 @@ def gradient_bounds(x, w, b, act, beta, g, keep):
     half, tiny = torch.finfo(t).eps / 2, torch.finfo(t).smallest_normal * torch.finfo(t).eps / 2
     x, w, b, g = (v.detach().double().cpu() for v in (x, w, b, g))
     K, N, M = x.shape[1], w.shape[0], x.shape[0]
-    extra = 2.0 ** -21 if t == torch.float32 else 0.0        # piece products that are dropped
+    extra = {torch.float32: 2.0 ** -21, torch.float16: 2.0 ** -16, torch.bfloat16: 0.0}[t]        # piece products that are dropped, of each product at most
     z = x @ w.t() + b
-    ez = ((K + 2) * u32 + extra) * (x.abs() @ w.abs().t() + b.abs())
+    ez = ((K + 2) * u32 + (extra if t == torch.float32 else 0.0)) * (x.abs() @ w.abs().t() + b.abs())
     d, size, curve, u = derivative(act, z, beta)
-    # the exponential's argument is rounded three times, exponential and reciprocal are off by 1e-6 in all
-    ed = curve * 1.01 * ez + (2e-6 + 4 * 2.0 ** -24 * u) * size + keep * d.abs()
+    # the exponential's argument: five roundings and three rounded constants at most; exponential and reciprocal are off by 1e-6 in all
+    ed = curve * 1.01 * ez + (2e-6 + 8 * 2.0 ** -24 * u) * size + keep * d.abs()
     dz = g * d
     edz = g.abs() * ed + (0.0 if t == torch.float32 else 2.0 ** -16) * dz.abs() + u32 * dz.abs()
 
@@ -154,3 +154,20 @@ def test_dense_fp16_infinities_in_the_cotangent_stay_in_their_rows():
     cols = [i for i in range(19) if i not in (4, 18)]
     assert torch.equal(grads[0][0][rows], grads[1][0][rows]) and not grads[1][0][[3, 100]].isfinite().any()
     assert torch.equal(grads[0][1][cols], grads[1][1][cols]) and not grads[1][1][[4, 18]].isfinite().any()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("size", GRAD_SIZES, ids=lambda s: "x".join(map(str, s)))
+def test_dense_gradients_in_the_tails_of_activations(size, dtype):
+    """Units far below 0 on every row: their small derivatives are kept as exactly as large ones (half a step of 16 significant bits, 24 beside fp32), not to an absolute step."""
+    (M, K, N), t = size, TYPES[dtype]
+    gen = torch.Generator().manual_seed(M + N)
+    cases = [("sigmoid", -15.0, 1.0), ("sigmoid", -18.0, 1.0), ("silu", -17.0, 1.0), ("gelu_tanh", -4.6, 1.0), ("softplus", -0.45, 50.0 if dtype == "fp16" else 100.0)]
+    if dtype != "fp16":
+        cases += [("sigmoid", -60.0, 1.0), ("softplus", -0.7, 100.0), ("gelu_tanh", -8.0, 1.0)]
+    for act, shift, beta in cases:
+        x, w = 0.5 + torch.rand(M, K, generator=gen), (0.5 + torch.rand(N, K, generator=gen)) / (8 * K)
+        b, g = shift - 0.1 * torch.rand(N, generator=gen), (1 + torch.rand(M, N, generator=gen)) * 2.0 ** (12 if dtype == "fp16" else 0)
+        x, w, b, g = (v.to(t).cuda() for v in (x, w, b, g))
+        assert (x.double() @ w.double().t() + b.double()).max() < 0.6 * shift
+        check_gradients(x, w, b.float(), act, beta, g, 2.0 ** -24 if dtype == "fp32" else 2.0 ** -16, f"{act} at {shift}")
