@@ -96,7 +96,7 @@ def _rows(t, n: int):
 
 
 def _dense_forward(x, weight, bias, residual, act: int, beta: float, want_deriv: bool):
-    """-> (y, what the backward pass needs besides tensors: sizes and strides; rows of x, rows of the weight, act'(z))"""
+    """-> (y, sizes and element type; rows of x, rows of the weight, act'(z))"""
     lib = _lib.load()
     N, K = weight.shape
     x2, ldx = _rows(x, K)
@@ -111,7 +111,7 @@ def _dense_forward(x, weight, bias, residual, act: int, beta: float, want_deriv:
     with _on(dev):
         _lib.check(lib.nm_dense_forward(x2.data_ptr(), ldx, w2.data_ptr(), ldw, _ptr(b), dt if b is None else _DTYPES[b.dtype], _ptr(r2), ldr, M, K, N, dt, act, beta,
                                         y.data_ptr(), N, _ptr(deriv), _ptr(ws), nbytes, _stream(dev)), "nm_dense_forward")
-    return y, (M, K, N, ldx, ldw, dt), x2, w2, deriv
+    return y, (M, K, N, dt), x2, w2, deriv
 
 
 class _Dense(torch.autograd.Function):
@@ -125,15 +125,18 @@ class _Dense(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, g):
-        # (runs on the engine's own thread, where every Python line costs twice: sizes and strides come from the forward pass)
+        # (runs on the engine's own thread, where every Python line costs twice: sizes come from the forward pass.  Strides do not: hooks on saved tensors, which
+        # move them to the host and back, keep values and sizes only.)
         _once("dense")
         need_x, need_w, need_b, need_r = ctx.needs_input_grad[:4]
         dx = dw = db = None
         if need_x or need_w or need_b:
             lib, dev, empty = _lib.load(), g.device, torch.empty
             x2, w2 = ctx.saved_tensors
-            M, K, N, ldx, ldw, dt = ctx.sizes
+            M, K, N, dt = ctx.sizes
             g2, ldg = (g, N) if g.is_contiguous() else _rows(g, N)
+            x2, ldx = (None, K) if x2 is None else _rows(x2, K)
+            w2, ldw = (None, K) if w2 is None else _rows(w2, K)
             if need_x:
                 dx = empty(ctx.x_shape, dtype=ctx.weight_dtype, device=dev)
             if need_w:
@@ -216,7 +219,7 @@ class _GatedScan(torch.autograd.Function):
     def backward(ctx, g_states, g_last):
         _once("gated_scan")
         lib = _lib.load()
-        gate, x, h0, cu = ctx.saved_tensors
+        gate, x, h0, cu = (None if t is None else t.contiguous() for t in ctx.saved_tensors)      # (hooks on saved tensors keep values and sizes only)
         dev, dt = x.device, _DTYPES[x.dtype]
         L, S, D = _scan_sizes(x, cu)
         packed, shared = int(cu is not None), int(gate.shape[-1] != D)

@@ -171,3 +171,41 @@ def test_dense_gradients_in_the_tails_of_activations(size, dtype):
         x, w, b, g = (v.to(t).cuda() for v in (x, w, b, g))
         assert (x.double() @ w.double().t() + b.double()).max() < 0.6 * shift
         check_gradients(x, w, b.float(), act, beta, g, 2.0 ** -24 if dtype == "fp32" else 2.0 ** -16, f"{act} at {shift}")
+
+
+# ------------------------------------------------------------------------------------------------ what a forward pass keeps for the backward pass
+def both_ways(make, wrap):
+    """Gradients of make() -> (outputs, leaves, cotangents), plainly and with the forward pass inside wrap()."""
+    out, leaves, cots = make()
+    want = torch.autograd.grad(out, leaves, cots)
+    with wrap():
+        out, leaves, cots = make()
+    got = torch.autograd.grad(out, leaves, cots)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def dense_slices():
+    """Rows that are slices of wider tensors, on both sides."""
+    gen = torch.Generator(device="cuda").manual_seed(2)
+    x = torch.randn(300, 401, generator=gen, device="cuda").half()[:, 5:182].detach().requires_grad_(True)
+    w = torch.randn(70, 300, generator=gen, device="cuda").half()[:, 3:180].detach().requires_grad_(True)
+    return ops.dense(x, w, activation="silu"), (x, w), torch.randn(300, 70, generator=gen, device="cuda").half()
+
+
+def packed_scan():
+    gen = torch.Generator(device="cuda").manual_seed(3)
+    gate = torch.rand(40, 800, generator=gen, device="cuda").t().detach().requires_grad_(True)     # columns first
+    x, h0 = torch.randn(800, 50, generator=gen, device="cuda")[:, 4:44].detach().requires_grad_(True), torch.randn(3, 40, generator=gen, device="cuda").requires_grad_(True)
+    states, last = ops.gated_scan(gate, x, h0, cu_seqlens=torch.tensor([0, 1, 500, 790], device="cuda"))
+    return (states, last), (gate, x, h0), (torch.randn(800, 40, generator=gen, device="cuda"), torch.randn(3, 40, generator=gen, device="cuda"))
+
+
+@pytest.mark.parametrize("make", [dense_slices, packed_scan])
+def test_saved_tensors_may_come_back_with_other_strides(make):
+    """Hooks that keep saved tensors on the host give them back contiguous; others give them back spread out."""
+    both_ways(make, torch.autograd.graph.save_on_cpu)
+
+    def spread(t):
+        wide = torch.empty((*t.shape[:-1], 2 * t.shape[-1] + 3), dtype=t.dtype, device=t.device)
+        return wide[..., 1:1 + 2 * t.shape[-1]:2].copy_(t) if t.dim() > 1 else t
+    both_ways(make, lambda: torch.autograd.graph.saved_tensors_hooks(lambda t: t, spread))
