@@ -118,8 +118,8 @@ class _Dense(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, residual, act, beta):
         need = ctx.needs_input_grad
-        y, ctx.sizes, x2, w2, ctx.deriv = _dense_forward(x, weight, bias, residual, act, beta, need[0] or need[1] or need[2])
-        ctx.save_for_backward(x2 if need[1] else None, w2 if need[0] else None)
+        y, ctx.sizes, x2, w2, deriv = _dense_forward(x, weight, bias, residual, act, beta, need[0] or need[1] or need[2])
+        ctx.save_for_backward(x2 if need[1] else None, w2 if need[0] else None, deriv)      # (released with the graph, and seen by hooks on saved tensors)
         ctx.x_shape, ctx.weight_dtype, ctx.bias_dtype = x.shape, weight.dtype, None if bias is None else bias.dtype
         return y
 
@@ -132,7 +132,7 @@ class _Dense(torch.autograd.Function):
         dx = dw = db = None
         if need_x or need_w or need_b:
             lib, dev, empty = _lib.load(), g.device, torch.empty
-            x2, w2 = ctx.saved_tensors
+            x2, w2, deriv = ctx.saved_tensors
             M, K, N, dt = ctx.sizes
             g2, ldg = (g, N) if g.is_contiguous() else _rows(g, N)
             x2, ldx = (None, K) if x2 is None else _rows(x2, K)
@@ -146,7 +146,7 @@ class _Dense(torch.autograd.Function):
             nbytes = lib.nm_dense_workspace_bytes(M, K, N, dt, 1)
             ws = empty((nbytes,), dtype=torch.uint8, device=dev) if nbytes > 0 else None
             with _on(dev):
-                _lib.check(lib.nm_dense_backward(g2.data_ptr(), ldg, _ptr(ctx.deriv), _ptr(x2), ldx, _ptr(w2), ldw, M, K, N, dt, _ptr(dx), K, _ptr(dw), _ptr(db),
+                _lib.check(lib.nm_dense_backward(g2.data_ptr(), ldg, _ptr(deriv), _ptr(x2), ldx, _ptr(w2), ldw, M, K, N, dt, _ptr(dx), K, _ptr(dw), _ptr(db),
                                                  dt if db is None else _DTYPES[db.dtype], _ptr(ws), nbytes, _stream(dev)), "nm_dense_backward")
         return dx, dw, db, (g if need_r else None), None, None
 
@@ -210,8 +210,8 @@ class _GatedScan(torch.autograd.Function):
     @staticmethod
     def forward(ctx, gate, x, h0, cu, reverse, blend, need_states):
         ctx.set_materialize_grads(False)
-        states, last, ctx.keep = _scan_forward(gate, x, h0, cu, reverse, blend, need_states, ctx.needs_input_grad[0] or cu is not None)
-        ctx.save_for_backward(gate, x, h0, cu)
+        states, last, keep = _scan_forward(gate, x, h0, cu, reverse, blend, need_states, ctx.needs_input_grad[0] or cu is not None)
+        ctx.save_for_backward(gate, x, h0, cu, keep)
         ctx.reverse, ctx.blend = reverse, blend
         return states, last
 
@@ -219,7 +219,7 @@ class _GatedScan(torch.autograd.Function):
     def backward(ctx, g_states, g_last):
         _once("gated_scan")
         lib = _lib.load()
-        gate, x, h0, cu = (None if t is None else t.contiguous() for t in ctx.saved_tensors)      # (hooks on saved tensors keep values and sizes only)
+        gate, x, h0, cu, keep = (None if t is None else t.contiguous() for t in ctx.saved_tensors)      # (hooks on saved tensors keep values and sizes only)
         dev, dt = x.device, _DTYPES[x.dtype]
         L, S, D = _scan_sizes(x, cu)
         packed, shared = int(cu is not None), int(gate.shape[-1] != D)
@@ -233,7 +233,7 @@ class _GatedScan(torch.autograd.Function):
         ws = torch.empty((nbytes,), dtype=torch.uint8, device=dev) if nbytes > 0 else None
         with _on(dev):
             _lib.check(lib.nm_scan_backward(gate.data_ptr(), _DTYPES[gate.dtype], shared, x.data_ptr(), dt, _ptr(h0), _ptr(cu), L, S, D,
-                                            int(ctx.reverse), int(ctx.blend), _ptr(ctx.keep), _ptr(g_states), _ptr(g_last), _ptr(dgate), _ptr(dx), _ptr(dh0),
+                                            int(ctx.reverse), int(ctx.blend), _ptr(keep), _ptr(g_states), _ptr(g_last), _ptr(dgate), _ptr(dx), _ptr(dh0),
                                             _ptr(ws), nbytes, _stream(dev)), "nm_scan_backward")
         return dgate, dx, dh0, None, None, None, None
 

@@ -2,6 +2,7 @@
 Tolerances are elementwise bounds from the arithmetic, as in test_gpu_ops.py."""
 import pytest
 import torch
+import torch.utils.checkpoint
 
 from neumesh_amd import ops
 
@@ -209,3 +210,37 @@ def test_saved_tensors_may_come_back_with_other_strides(make):
         wide = torch.empty((*t.shape[:-1], 2 * t.shape[-1] + 3), dtype=t.dtype, device=t.device)
         return wide[..., 1:1 + 2 * t.shape[-1]:2].copy_(t) if t.dim() > 1 else t
     both_ways(make, lambda: torch.autograd.graph.saved_tensors_hooks(lambda t: t, spread))
+
+
+@pytest.mark.parametrize("make", [dense_slices, packed_scan])
+def test_kept_tensors_are_saved_variables(make):
+    """What the forward pass keeps beside its inputs (act'(z), states) is released by the backward pass while the outputs live, passes through hooks on saved
+    tensors, and is made again under checkpointing."""
+    _, leaves, cots = make()
+    sizes = []
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: (sizes.append(t.numel() * t.element_size()), t)[1], lambda t: t):
+        make()
+    if make is dense_slices:
+        assert sizes[-1] == 300 * 70 * 3                      # act'(z)
+    else:
+        assert sizes[-1] > 800 * 4                            # the sequences of the rows, and states
+    leaves = [v.detach().requires_grad_(True) for v in leaves]
+
+    def run(*v):
+        return ops.dense(*v, activation="silu") if make is dense_slices else ops.gated_scan(*v, cu_seqlens=torch.tensor([0, 1, 500, 790], device="cuda"))
+    want = torch.autograd.grad(run(*leaves), leaves, cots)
+    got = torch.autograd.grad(torch.utils.checkpoint.checkpoint(run, *leaves, use_reentrant=False), leaves, cots)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_memory_falls_after_backward_while_outputs_live():
+    x, w = torch.randn(20000, 64, device="cuda", requires_grad=True), torch.randn(256, 64, device="cuda", requires_grad=True)
+    gate, v = torch.rand(1, 40000, 64, device="cuda", requires_grad=True), torch.randn(1, 40000, 64, device="cuda", requires_grad=True)
+    for run, leaves, kept in ((lambda: ops.dense(x, w, activation="silu"), (x, w), 20000 * 256 * 4), (lambda: ops.gated_scan(gate, v)[0], (gate, v), 40000 // 64 * 64 * 4)):
+        y = run()
+        before = torch.cuda.memory_allocated()
+        grads = torch.autograd.grad(y, leaves, torch.ones_like(y))
+        del grads
+        assert torch.cuda.memory_allocated() <= before - kept and y.grad_fn is not None
+        with pytest.raises(RuntimeError, match="backward through the graph a second time"):
+            torch.autograd.grad(y, leaves, torch.ones_like(y))
