@@ -396,7 +396,7 @@ int nm_train_composite_backward(const float* sdf, const float* s, const float* d
  * y = act(x W^T + b) + r and its gradient, for rows of any width: x [M,K] (row stride ldx), W [N,K] (ldw), b [N], r [M,N] (ldr), y [M,N] (ldy), all
  * of one element type (the bias: that type or fp32), last axis contiguous, any element alignment.  K, N <= 2^20, strides <= 2^24; zero sizes are allowed
  * (K = 0: y = act(b) + r).  Products accumulate in fp32 and are rounded once, at the end.
- * act: softplus is log(1 + exp(beta z)) / beta (beta > 0; other activations ignore it), GELU in its tanh form.
+ * act: softplus is log(1 + exp(beta z)) / beta (beta in [2^-126, 2^126]; other activations ignore it), GELU in its tanh form.
  * deriv: M N elements of 3 bytes beside 16-bit rows, of 4 beside fp32 rows (2-byte / 4-byte aligned): act'(z) in a form of the library's own, what the
  * backward pass needs; NULL = not wanted.  With NM_ACT_NONE nothing is written and the backward pass takes NULL.
  * nm_dense_backward: g [M,N] cotangent of y -> dx [M,K] (lddx), dweight [N,K] contiguous, dbias [N] (NULL = not wanted; overwritten, not added to).  The

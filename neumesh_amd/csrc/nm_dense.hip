@@ -1408,7 +1408,7 @@ int nm_dense_forward(const void* x, int64_t ldx, const void* weight, int64_t ldw
     hipStream_t stream = (hipStream_t)stream_;
     if (nm_d_check("nm_dense_forward", M, K, N, dtype, bias_dtype)) return 1;
     if (act < NM_ACT_NONE || act > NM_ACT_GELU_TANH) return nm_fail("nm_dense_forward: unknown activation %d", act);
-    if (act == NM_ACT_SOFTPLUS && !(beta > 0.f)) return nm_fail("nm_dense_forward: softplus needs beta > 0");
+    if (act == NM_ACT_SOFTPLUS && !(beta >= 0x1p-126f && beta <= 0x1p126f)) return nm_fail("nm_dense_forward: softplus needs beta in [2^-126, 2^126]");
     if (M == 0 || N == 0) return 0;
     if ((K > 0 && (!x || !weight)) || !y) return nm_fail("nm_dense_forward: NULL argument");
     if (ldx > NM_D_MAX_LD || ldw > NM_D_MAX_LD || ldy > NM_D_MAX_LD || ldr > NM_D_MAX_LD) return nm_fail("nm_dense_forward: row stride beyond 2^24");

@@ -156,8 +156,8 @@ def dense(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] = 
     """act(x weight^T + bias) + residual.
 
     x [..., K], weight [N, K] (as nn.Linear stores it), bias [N], residual [..., N] -> [..., N], all of one element type (fp32, fp16, bf16; the
-    bias may be fp32 beside 16-bit rows).  activation: one of ACTIVATIONS; softplus is log(1 + exp(beta z)) / beta (100 as in the
-    geometry network), GELU its tanh form.  Differentiable in all four tensors.  Rows may be strided (a column slice of a wider tensor); other
+    bias may be fp32 beside 16-bit rows).  activation: one of ACTIVATIONS; softplus is log(1 + exp(beta z)) / beta, beta in
+    [2^-126, 2^126] (100 as in the geometry network), GELU its tanh form.  Differentiable in all four tensors.  Rows may be strided (a column slice of a wider tensor); other
     layouts are copied.  One row to many: up to 8 rows go through a form that reads the weights once and in place.
     fp32 products are as accurate as an fp32 matrix product; a non-finite operand makes the outputs it enters NaN there, and so in gradients
     beside an activation."""
@@ -173,8 +173,8 @@ def dense(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] = 
     if residual is not None and tuple(residual.shape) != (*x.shape[:-1], N):
         raise ValueError(f"dense: residual has shape {tuple(residual.shape)}, expected {(*x.shape[:-1], N)}")
     beta = float(beta)
-    if activation == "softplus" and not (beta > 0.0 and math.isfinite(beta)):
-        raise ValueError(f"dense: beta={beta} must be positive")
+    if activation == "softplus" and not 2.0 ** -126 <= beta <= 2.0 ** 126:      # (beta and 1 / beta are normal fp32 numbers)
+        raise ValueError(f"dense: beta={beta} must be in [2^-126, 2^126]")
     _no_tangents("dense", x, weight, bias, residual)
     _on_device("dense", dev)
     act = ACTIVATIONS[activation]

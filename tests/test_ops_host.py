@@ -162,3 +162,16 @@ def test_tangents_are_refused():
             fn(*args)
     with pytest.raises(RuntimeError, match="forward-mode derivatives are not supported"):
         torch.func.jvp(lambda t: ops.dense(t, w), (x,), (x,))
+
+
+def test_softplus_refuses_what_fp32_does_not_hold():
+    """beta goes to the kernels in fp32, with its reciprocal: 1e39 would arrive as an infinity, 1e-46 as 0."""
+    x, w = torch.randn(4, 6), torch.randn(5, 6)
+    for beta in (1e39, 1e-46, 1e-40, 2.0 ** 127, -1.0, float("inf")):
+        with pytest.raises(ValueError, match="beta"):
+            ops.dense(x, w, activation="softplus", beta=beta)
+        with pytest.raises(_lib.NeuMeshHipError, match="HIP device"):
+            ops.dense(x, w, activation="silu", beta=beta)     # (ignored by the others)
+    lib, p = _lib.load(require_device=False), C.c_void_p(4096)
+    for beta in (float("inf"), 1e-40, 1.5e38):
+        assert lib.nm_dense_forward(p, 8, p, 8, None, 0, None, 0, 20, 8, 4, 0, 2, beta, p, 4, None, p, 1 << 30, None) == 1 and b"beta" in lib.nm_last_error()
