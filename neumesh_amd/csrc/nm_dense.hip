@@ -182,23 +182,21 @@ __device__ __forceinline__ void nm_d_act(int act, float beta, float ibeta, bool 
 }
 
 // ------------------------------------------------------------------------------------------------ operand pieces
-// fp32 -> three bf16 pieces by truncation, a = p0 + p1 + p2 exactly
-__device__ __forceinline__ void nm_d_cut(float a, unsigned& b0, unsigned& b1, unsigned& b2) {
-    b0 = __float_as_uint(a) & 0xffff0000u;
-    const float r = a - __uint_as_float(b0);
-    b1 = __float_as_uint(r) & 0xffff0000u;
-    b2 = __float_as_uint(r - __uint_as_float(b1));
-}
 __device__ __forceinline__ unsigned nm_d_pair(unsigned lo, unsigned hi) { return __builtin_amdgcn_perm(hi, lo, 0x07060302u); }   // upper halves
 
-// eight values -> fragments (16 bytes: eight 16-bit pieces per plane)
+// eight fp32 values -> fragments (16 bytes: eight 16-bit pieces per plane): three bf16 pieces each, a = p0 + p1 + p2 exactly.  The first two are rounded to
+// nearest, so that |p1| <= 2^-8 and |p2| <= 2^-17 of a's power of two, of either sign (cut off instead, pieces have the sign of a and are twice as
+// large: the piece products that are left out were up to 2^-21 of every product, all in one direction).  What would round to an infinity takes the largest bf16.
 __device__ __forceinline__ void nm_d_cut8(const float (&f)[8], uint4 (&p)[3]) {
-    unsigned b[3][8];
+    __bf16 b[3][8];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) nm_d_cut(f[e], b[0][e], b[1][e], b[2][e]);
-#pragma unroll
-    for (int q = 0; q < 3; ++q)
-        p[q] = make_uint4(nm_d_pair(b[q][0], b[q][1]), nm_d_pair(b[q][2], b[q][3]), nm_d_pair(b[q][4], b[q][5]), nm_d_pair(b[q][6], b[q][7]));
+    for (int e = 0; e < 8; ++e) {
+        b[0][e] = (__bf16)__builtin_amdgcn_fmed3f(f[e], -0x1.fep127f, 0x1.fep127f);
+        const float r = f[e] - (float)b[0][e];
+        b[1][e] = (__bf16)r;
+        b[2][e] = (__bf16)(r - (float)b[1][e]);
+    }
+    __builtin_memcpy(p, b, sizeof(b));
 }
 // value + residual in bf16: 16 bits of any fp32 value, all of an fp16 one (no residual of an infinity)
 __device__ __forceinline__ void nm_d_two8(const float (&f)[8], uint4 (&p)[2]) {
@@ -243,7 +241,7 @@ __device__ __forceinline__ V nm_d_mfma(const uint4& a, const uint4& b, V c) {
 // all piece products of one pair of fragments, small terms first.  Planes: PA of a, PB of b.
 template <int DT, int PA, int PB, typename V>
 __device__ __forceinline__ V nm_d_products(const uint4 (&a)[PA], const uint4 (&b)[PB], V c) {
-    if constexpr (PA == 3 && PB == 3) {      // dropped: a1 b2 + a2 b1 + a2 b2 < 2^-21 |a||b|
+    if constexpr (PA == 3 && PB == 3) {      // dropped: a1 b2 + a2 b1 + a2 b2 < 2^-23 |a||b|, of either sign
         c = nm_d_mfma<DT>(a[1], b[1], c);
         c = nm_d_mfma<DT>(a[0], b[2], c);
         c = nm_d_mfma<DT>(a[2], b[0], c);

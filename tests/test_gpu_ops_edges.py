@@ -244,3 +244,29 @@ def test_memory_falls_after_backward_while_outputs_live():
         assert torch.cuda.memory_allocated() <= before - kept and y.grad_fn is not None
         with pytest.raises(RuntimeError, match="backward through the graph a second time"):
             torch.autograd.grad(y, leaves, torch.ones_like(y))
+
+
+@pytest.mark.parametrize("rows", [4, 40, 20000])              # few rows, streamed or resident weights, a split gradient
+def test_fp32_products_are_fp32_products(rows):
+    """Layers of one and a few inputs, where nothing hides what a product loses: operands whose bits below the first eight are all ones, and the largest numbers there
+    are.  Piece products of 2^-23 of a product are left out at most, and its largest one is added with an error of one unit in the last place."""
+    def near(got, a, b):
+        a, b, got = a.detach().double().cpu(), b.detach().double().cpu(), got.detach().double().cpu()
+        terms = ((a != 0).double() @ (b != 0).double()).clamp(min=1)
+        return ((got - a @ b).abs() <= (2.0 ** -23 + (2 * terms - 1) * 2.0 ** -23 + 2.0 ** -26) * (a.abs() @ b.abs())).all()
+    for K in (1, 3):
+        gen = torch.Generator().manual_seed(K)
+        ones = torch.tensor([1.0 + 2.0 ** -7 - 2.0 ** -23, 1.0 + 2.0 ** -8 - 2.0 ** -23, 2.0 - 2.0 ** -23, 1.0 + 2.0 ** -6 - 2.0 ** -14])
+
+        def some(*shape):
+            return ones[torch.randint(0, 4, shape, generator=gen)]
+        x, w = some(rows, K) * 2.0 ** torch.randint(-40, 40, (rows, 1), generator=gen), some(24, K) * 2.0 ** torch.randint(-20, 20, (24, 1), generator=gen)
+        g = (some(rows, 24) * torch.nn.functional.one_hot(torch.arange(rows) % 24, 24)).cuda()      # one term in every sum of dx
+        x, w = x.cuda().requires_grad_(True), w.cuda().requires_grad_(True)
+        y = ops.dense(x, w)
+        dx, dw = torch.autograd.grad(y, (x, w), g)
+        assert near(y, x, w.t()) and near(dx, g, w) and near(dw, g.t(), x), K
+    top = torch.full((rows, 8), 3.4e38).cuda()                # (sums in any order stay finite)
+    w = torch.tensor([[0.1, -0.1] * 4, [2.0 ** -4] * 8, [2.0 ** -126] * 8]).cuda()
+    y = ops.dense(top, w)
+    assert y.isfinite().all() and near(y, top, w.t())
