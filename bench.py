@@ -488,6 +488,15 @@ def order_config(cfg: dict) -> dict:
     return head
 
 
+LINE_MAX = 16000    # bytes of the JSON line: readers that keep the end of a program's output lose the start of a longer one (a line of 21.7 KB was)
+
+
+def short_rows(extra):
+    """The rows after the headline as they go into a line that would be too long: names without their explanations, rates and times alone."""
+    return {name.split(" (")[0]: {k: v for k, v in row.items() if k in ("value", "unit", "error") or k.startswith("ms_per_")} if isinstance(row, dict) else row
+            for name, row in extra.items()}
+
+
 def line_guard(out, extra, budget_s):
     """(emit, timer) for the ONE line of the contract.  emit(note=None) prints `out` (+ `extra` as out["extra"]) exactly once; timer is an
     unstarted threading.Timer that, when it fires after budget_s seconds, emits the line with the rows finished so far and ends the process
@@ -505,6 +514,9 @@ def line_guard(out, extra, budget_s):
                 if note:
                     snap["_watchdog"] = note
                 line = json.dumps(dict(out, extra=snap) if snap else out, default=str)
+                if len(line) > LINE_MAX:        # everything on stderr, the rows' figures on the line
+                    print("all rows: " + line, file=sys.stderr, flush=True)
+                    line = json.dumps(dict(out, extra=short_rows(snap)), default=str)
                 break
             except RuntimeError:
                 time.sleep(0.01)

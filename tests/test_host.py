@@ -483,3 +483,20 @@ def test_trained_checkpoint_is_the_one_the_fixture_was_rendered_from():
     assert np.abs(g[:, 0] / np.linalg.norm(v, axis=1) - 1.0).max() > 0.05          # trained: g is no longer |v|
     untrained = common.scene_state(common.scene_mesh(140000))
     assert float(np.abs(st["color_features"] - untrained["color_features"]).mean()) > 1e-3
+
+
+def test_bench_line_stays_short_enough_to_be_read():
+    """The ONE line of the contract: rows whose explanations would make it longer than LINE_MAX are shortened to their figures, and printed whole on stderr."""
+    import json
+    code = ("import sys; sys.path.insert(0, %r); import bench\n"
+            "extra = {'row_%%d (%%s)' %% (i, 'why ' * 200): {'value': float(i), 'unit': 'rays/s', 'ms_per_frame': 2.0, 'points': {'a': 1.0}} for i in range(30)}\n"
+            "emit, timer = bench.line_guard({'metric': 'm', 'value': 1.0, 'config': {'model': 'x'}}, extra, 60.0)\n"
+            "assert emit()\n") % ROOT
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=120)
+    assert r.returncode == 0, r.stderr[-500:]
+    lines = r.stdout.splitlines()
+    d = json.loads(lines[0])
+    assert len(lines) == 1 and len(lines[0]) <= 16000 and d["value"] == 1.0 and d["config"] == {"model": "x"}
+    assert len(d["extra"]) == 30 and d["extra"]["row_7"] == {"value": 7.0, "unit": "rays/s", "ms_per_frame": 2.0}
+    whole = [l for l in r.stderr.splitlines() if l.startswith("all rows: ")]
+    assert len(whole) == 1 and len(json.loads(whole[0][len("all rows: "):])["extra"]) == 30
