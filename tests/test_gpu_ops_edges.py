@@ -270,3 +270,52 @@ def test_fp32_products_are_fp32_products(rows):
     w = torch.tensor([[0.1, -0.1] * 4, [2.0 ** -4] * 8, [2.0 ** -126] * 8]).cuda()
     y = ops.dense(top, w)
     assert y.isfinite().all() and near(y, top, w.t())
+
+
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+def test_kept_derivatives_of_rows_of_any_width(dtype):
+    """The gradient of an fp32 bias is a sum of kept derivatives that nothing rounds again: 16 significant bits of each, whatever the width of the rows."""
+    t = TYPES[dtype]
+    gen = torch.Generator().manual_seed(5)
+    for N in (1, 2, 3, 5, 7, 8, 9, 13, 31, 33, 57, 129, 250, 517):
+        for M in (1, 7, 9, 50, 700):                          # few rows, narrow and wide blocks of columns
+            x, w, b = (torch.randn(*s, generator=gen) for s in ((M, 3), (N, 3), (N,)))
+            x, w, b = x.to(t).cuda(), w.to(t).cuda(), (b - 3).cuda().requires_grad_(True)
+            for act in ("sigmoid", "gelu_tanh"):
+                db = torch.autograd.grad(ops.dense(x, w, b, activation=act), b, torch.ones(M, N, dtype=t, device="cuda"))[0]
+                z = x.double() @ w.double().t() + b.double()
+                d, size, curve, u = derivative(act, z, 1.0)
+                bound = ((2.0 ** -16 + M * 2.0 ** -23) * d.abs() + (2e-6 + 8 * 2.0 ** -24 * u) * size + curve * 1.01 * 5 * 2.0 ** -23 * (x.double().abs() @ w.double().abs().t() + b.abs())).sum(0)
+                assert ((db - d.sum(0)).abs() <= bound).all(), (N, M, act)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_nan_inputs_keep_to_their_rows_in_gradients(dtype):
+    t = TYPES[dtype]
+    gen = torch.Generator(device="cuda").manual_seed(7)
+    for M, K, N in ((6, 20, 37), (150, 41, 19), (400, 700, 600)):
+        x, w, g = (torch.randn(*s, generator=gen, device="cuda").to(t) for s in ((M, K), (N, K), (M, N)))
+        bad = x.clone()
+        bad[3, K - 1] = float("nan")
+        grads = []
+        for v in (x, bad):
+            leaves = [p.clone().requires_grad_(True) for p in (v, w)]
+            grads.append(torch.autograd.grad(ops.dense(*leaves, activation="silu"), leaves, g))
+        rows = [i for i in range(M) if i != 3]
+        assert torch.equal(grads[0][0][rows], grads[1][0][rows]) and grads[1][0][3].isnan().all() and grads[1][1].isnan().all()
+
+
+def test_training_layer_beyond_32_bits():
+    """More than 2^32 bytes of kept derivatives: gradients of the far end against the same rows on their own."""
+    M, D = 8_500_000, 256
+    gen = torch.Generator(device="cuda").manual_seed(4)
+    x = torch.empty(M, D, device="cuda", dtype=torch.bfloat16).uniform_(-1, 1, generator=gen).requires_grad_(True)
+    w, b = (torch.randn(D, D, generator=gen, device="cuda") / 16).bfloat16(), torch.zeros(D, device="cuda", requires_grad=True)
+    g = torch.zeros(M, D, device="cuda", dtype=torch.bfloat16)
+    g[-70000:].uniform_(-1, 1, generator=gen)
+    dx, db = torch.autograd.grad(ops.dense(x, w, b, activation="silu"), (x, b), g)
+    assert (dx[:-70000] == 0).all()
+    u, c = x.detach()[-70000:].clone().requires_grad_(True), torch.zeros(D, device="cuda", requires_grad=True)
+    du, dc = torch.autograd.grad(ops.dense(u, w, c, activation="silu"), (u, c), g[-70000:])
+    # sums of 70000 terms of size one in two orders; rounding of one value to 8 bits twice
+    assert ((dx[-70000:].float() - du.float()).abs() <= 2.0 ** -7 * du.float().abs() + 1e-5).all() and (db - dc).abs().max() <= 70000 * 2.0 ** -22
