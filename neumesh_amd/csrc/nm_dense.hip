@@ -443,7 +443,7 @@ __device__ __forceinline__ void nm_d_each(F f, std::integer_sequence<int, K...>)
 // global memory here, piece by piece, cost a 131072 x 256 layer 8 of 52 us.  So the residual (RES) of eight pieces is in flight before the first store, and
 // column blocks with one that stay resident have no more than eight pieces per wave (256 x 256 tiles: six ahead, eight would spill).  The scheduling barriers keep the pieces apart, and the opaque column makes its tests, biases and
 // addresses HERE: mixed together or hoisted out of a loop over row tiles they cost 100 registers and spills.
-template <int DT, bool PROD, bool RES, int RT, int NP>
+template <int DT, bool PROD, bool RES, int RT, int NP, bool KEEP = !PROD>
 __device__ __forceinline__ void nm_d_epilogue(const NmDenseArgs& p, const nm_v4f (&acc)[RT][2 * NP], const float* bias, long long m0, int cb,
                                               int lane) {
     typedef typename NmType<DT>::elem T;
@@ -480,10 +480,10 @@ __device__ __forceinline__ void nm_d_epilogue(const NmDenseArgs& p, const nm_v4f
             nm_oct_to_float<DT>(rs[k % AHEAD], q);
             fetch(k + AHEAD);
         }
-        if constexpr (!PROD) nm_d_act<DT == NM_F32>(p.act, p.beta, ibeta, p.DV != nullptr, z, dv);
+        if constexpr (!PROD) nm_d_act<DT == NM_F32>(p.act, p.beta, ibeta, KEEP && p.DV, z, dv);
         if (m >= p.R) return;
         if constexpr (!PROD) {
-            if (p.DV) nm_d_store_factors<DT>(p.DV, p.R, p.C, m, dv, c);
+            if (KEEP && p.DV) nm_d_store_factors<DT>(p.DV, p.R, p.C, m, dv, c);
             if (RES && p.res) {
 #pragma unroll
                 for (int i = 0; i < 8; ++i) z[i] += q[i];
@@ -662,7 +662,7 @@ __global__ __launch_bounds__(512, 2) void nm_dense_resident_kernel(NmDenseArgs p
 // (60.8 MB: 2.3 TB/s).  131072 x 256 -> 256 with softplus, residual and kept derivative takes 93 us: 47 for the layer, and 15 for the residual, 15
 // for the derivative and 19 for the activation, one after the other, since the one workgroup of a CU has all its waves in the same phase.  Results
 // and residual through LDS, in whole lines, changed nothing (61.8 us instead of 60.9 for the first layer).
-template <int DT>
+template <int DT, bool KEEP>
 __global__ __launch_bounds__(512, 2) void nm_dense_tile_kernel(NmDenseArgs p) {
     typedef typename NmType<DT>::elem T;
     __shared__ uint4 lds[2][2][256 * 8];                     // [buffer][rows, columns][row][piece]
@@ -735,7 +735,7 @@ __global__ __launch_bounds__(512, 2) void nm_dense_tile_kernel(NmDenseArgs p) {
         if (k + 1 < panels) store(k + 1);
         __syncthreads();
     }
-    nm_d_epilogue<DT, false, true, 8, 2>(p, acc, bias + wc * 64, rb * 256 + wr * 128, cb * 4 + wc, lane);
+    nm_d_epilogue<DT, false, true, 8, 2, KEEP>(p, acc, bias + wc * 64, rb * 256 + wr * 128, cb * 4 + wc, lane);
 }
 
 // Otherwise: one workgroup: 4 waves, 64 RT rows x 32 NP columns, both sides streamed.  The rows as above; the column operand is shared by the four waves
@@ -1288,7 +1288,10 @@ static int nm_d_launch(const NmDensePlan& pl, NmDenseArgs a, hipStream_t stream)
     if (groups * (pl.tile ? 512 : 256) > NM_D_MAX_THREADS) return nm_fail("nm_dense: %lld rows x %d columns exceed one launch", a.R, a.C);
     const dim3 grid((unsigned)groups), block(256);
     if (pl.tile) {
-        if constexpr (!F && !PROD) hipLaunchKernelGGL((nm_dense_tile_kernel<DT>), grid, dim3(512), 0, stream, a);
+        if constexpr (!F && !PROD) {
+            if (a.DV) hipLaunchKernelGGL((nm_dense_tile_kernel<DT, true>), grid, dim3(512), 0, stream, a);
+            else hipLaunchKernelGGL((nm_dense_tile_kernel<DT, false>), grid, dim3(512), 0, stream, a);
+        }
     } else if (pl.rt == 4) {
         if constexpr (!F && !PROD) hipLaunchKernelGGL((nm_dense_stream_kernel<DT, PROD, 4, 4, 2>), grid, block, 0, stream, a);
     } else {
