@@ -416,7 +416,7 @@ int nm_dense_backward(const void* g, int64_t ldg, const void* deriv, const void*
 /* ----------------------------------------------------------------------------- gated linear recurrence
  * Along S sequences of rows, in row order or (reverse) from the last row to the first, for every channel:
  *   plain: h_i = gate_i h_{i-1} + x_i        blend: h_i = (1 - gate_i) h_{i-1} + gate_i x_i     (alpha compositing: gate = opacity, reverse = far to near)
- * x, states [L,D] and gate [L,D] (shared_gate: [L], one for all channels), contiguous, any element alignment; the gate is of x's element type or fp32.
+ * (L, S < 2^31, D <= 2^20)  x, states [L,D] and gate [L,D] (shared_gate: [L], one for all channels), contiguous, any element alignment; the gate is of x's element type or fp32.
  * |gate| <= 1 (blend: 0 <= gate <= 1) is expected: products of the factors over a sequence must stay finite.
  * cu_seqlens == NULL: S sequences of L / S rows.  Otherwise DEVICE int32 [S+1], ascending: sequence s is rows cu[s] .. cu[s+1]-1; rows
  * outside belong to none (their states and gradients are 0).  What an ill-formed cu_seqlens gives is unspecified but stays within the buffers.

@@ -558,8 +558,9 @@ __device__ __forceinline__ void nm_d_load_block(const NmDenseArgs& p, int cb, in
 // it once, and its eight waves then walk over tiles of 32 rows, each for itself, without another barrier.  A wave owns whole rows: their elements
 // go from global memory straight into fragments (a lane's 8 consecutive elements of one row ARE a fragment), RING steps ahead of their use
 // and across the end of a tile: the next tile's rows are in flight while this one's results are stored.
-// Measured: 65536 x 256 -> 256 fp32 with softplus 78 us and its dx 86 us (51.5 G multiply-adds and adds each as six bf16 products: 660 and 600 TFLOP/s; bound by
-// cutting the rows into pieces once per column block, and by the products); dx of 131072 x 256 -> 256 bf16 53 us (201 MB: 3.8 TB/s).
+// Measured (counters: profiles/ops_counters.txt): 65536 x 256 -> 256 fp32 with softplus 83 us (51.5 G multiplications and additions as six bf16 products: 620 TFLOP/s;
+// the rows are cut into pieces once per column block, the vector unit is busy 56 % of the time, the matrix pipe 27 %) and its dx 90 us (570 TFLOP/s; address units busy
+// 73 %); dx of 131072 x 256 -> 256 bf16 65 us (234 MB with the kept derivatives: 3.6 TB/s, address units 62 %).
 #define NM_D_RESIDENT 144
 
 template <int DT, bool PROD, int NP>
@@ -654,14 +655,14 @@ __global__ __launch_bounds__(512, 2) void nm_dense_resident_kernel(NmDenseArgs p
 }
 
 // Large 16-bit layers, W as it lies: 256 rows x 256 columns per workgroup of eight waves (128 x 64 each).  Both operands come in panels of 64
-// contraction elements as whole 128-byte lines, eight lanes a line -- read straight into fragments, sixteen rows side by side, the rows of a
-// 16384 x 1024 -> 1024 layer kept the address units busy for 72 % of 93 us -- and go through LDS, in two buffers, with one barrier per panel and the
-// next panel in flight in registers.  The eight 16-byte pieces of an LDS row are exchanged by the row's number, so that the sixteen rows of a fragment
+// contraction elements as whole 128-byte lines, eight lanes a line -- the kernel above reads rows straight into fragments, sixteen rows side by side, which keeps
+// the address units busy for 62 .. 73 % of its time, this one for 22 .. 28 % -- and go through LDS, in two buffers, with one barrier per panel and
+// the next panel in flight in registers.  The eight 16-byte pieces of an LDS row are exchanged by the row's number, so that the sixteen rows of a fragment
 // lie in different banks.
-// Measured: 16384 x 1024 -> 1024 bf16 with GELU and residual 56 us, 44 without both (34.4 GFLOP: 610 and 780 TFLOP/s); 65536 x 207 -> 256 with ReLU 27 us
-// (60.8 MB: 2.3 TB/s).  131072 x 256 -> 256 with softplus, residual and kept derivative takes 93 us: 47 for the layer, and 15 for the residual, 15
-// for the derivative and 19 for the activation, one after the other, since the one workgroup of a CU has all its waves in the same phase.  Results
-// and residual through LDS, in whole lines, changed nothing (61.8 us instead of 60.9 for the first layer).
+// Measured: 16384 x 1024 -> 1024 bf16 with GELU and residual 55 us (34.4 GFLOP: 630 TFLOP/s); 65536 x 207 -> 256 with ReLU 24 us (60.8 MB: 2.5 TB/s); 131072 x
+// 256 -> 256 with softplus, residual and kept derivatives 105 us (302 MB: 2.9 TB/s).  Waves wait 43 .. 58 % of their time: load, product, activation and store add
+// up, since the one workgroup of a CU has all its waves in the same phase.  Results and residual through LDS, in whole lines, changed nothing.
+// KEEP: with kept derivatives.  One kernel for both has 81 KB of instructions, and calls without derivatives paid for them (the second layer: 28.6 us a call instead of 21.5).
 template <int DT, bool KEEP>
 __global__ __launch_bounds__(512, 2) void nm_dense_tile_kernel(NmDenseArgs p) {
     typedef typename NmType<DT>::elem T;
@@ -740,7 +741,7 @@ __global__ __launch_bounds__(512, 2) void nm_dense_tile_kernel(NmDenseArgs p) {
 
 // Otherwise: one workgroup: 4 waves, 64 RT rows x 32 NP columns, both sides streamed.  The rows as above; the column operand is shared by the four waves
 // through LDS, PS steps at a time in two buffers, one barrier per panel, both sides' next panel in flight in registers meanwhile.
-// Measured: 4096 x 1024 -> 1024 bf16 with GELU 44 us, 16384 x 520 -> 300 24 us; bound by the address units, which see sixteen rows side by side.
+// Measured: 4096 x 1024 -> 1024 bf16 with GELU 43 us, 16384 x 520 -> 300 25 us; bound by latency: one workgroup of four waves per CU, waiting 63 % of their time.
 template <int DT, bool PROD, int RT, int NP, int PS>
 __global__ __launch_bounds__(256, 2) void nm_dense_stream_kernel(NmDenseArgs p) {
     typedef typename NmType<DT>::elem T;
@@ -915,7 +916,7 @@ __global__ __launch_bounds__(256) void nm_dense_few_kernel(const typename NmType
 // columns, eight consecutive rows -- a fragment -- and writes it to LDS in the order in which the waves read fragments.  Every wave brings its share of
 // dz (from g and act'(z), in two pieces or three) AND of x: the conversions, which cost as much as the products, are spread over the four
 // SIMDs.  The next block's rows are in flight while this one is multiplied.
-// Measured: 256 x 256 weights, 131072 rows bf16 60 us (201 MB: 3.3 TB/s), 65536 rows fp32 61 us (51.5 G as six products: 840 TFLOP/s).
+// Measured: 256 x 256 weights, 131072 rows bf16 68 us (234 MB with the kept derivatives: 3.5 TB/s), 65536 rows fp32 65 us (51.5 G as six products: 790 TFLOP/s).
 struct NmDenseGradArgs {
     const void* G; long long ldg; const void* D;   // dz = G * D (D contiguous [R, N], kept derivatives, or NULL)
     const void* X; long long ldx;
@@ -1226,9 +1227,9 @@ static NmDensePlan nm_d_plan(int dt, bool prod, bool res, bool trans, long long 
     while (fit > 0 && 2 * steps * pieces * fit > NM_D_RESIDENT) fit >>= 1;
     p.resident = fit > 0 && nm_d_up(C, 32 * fit) <= 4;
     // 256 x 256 tiles: one per CU and round, so what counts is the share of the rounds' 2^24 outputs that is there.  Measured in bf16 with GELU, us
-    // (tiles / otherwise).  Against streaming: share 1: 50 / 80 (16384 x 1024 -> 1024), 0.63: 90 / 120 (16384 x 1024 -> 1280), 0.38: 46 / 58, 0.25: 44 / 44
-    // (6144 and 4096 x 1024 -> 1024).  Against resident weights: share 1: 55 / 90 (65536 x 1024 -> 256), 27 / 30 (65536 x 256 -> 256), 48 / 46 (65536 x
-    // 256 -> 512), 0.59: 55 / 51 (65536 x 300 -> 300), 0.5: 50 / 49 (32768 x 1024 -> 256).
+    // (tiles / otherwise).  Against streaming: share 1: 50 / 85 (16384 x 1024 -> 1024), 0.63: 86 / 131 (16384 x 1024 -> 1280), 0.38: 43 / 56, 0.25: 42 / 43
+    // (6144 and 4096 x 1024 -> 1024).  Against resident weights: share 1: 51 / 81 (65536 x 1024 -> 256), 25 / 31 (65536 x 256 -> 256), 44 / 47 (65536 x
+    // 256 -> 512), 0.59: 51 / 50 (65536 x 300 -> 300), 0.5: 43 / 45 (32768 x 1024 -> 256).
     const double rounds = (double)nm_d_up(nm_d_up(R, 256) * nm_d_up(C, 256), 256), share = (double)R * (double)C / (rounds * 16777216.0);
     p.tile = dt != NM_F32 && !prod && !trans && Q > 0 && R > 0 && share >= (p.resident ? 0.75 : 0.3);
     if (p.tile) p.resident = false;

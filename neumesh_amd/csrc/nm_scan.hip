@@ -402,7 +402,7 @@ template <int VEC, bool SHARED> struct NmSeg {
 
 // MAP: only the range's map, from its last sequence start on.
 // Measured, main launch: 4 x 16384 x 512 bf16 44 us (201 MB: 4.6 TB/s; maps 25 us, carries 9), 8192 packed sequences of 96 x 32 fp32 60 us (302 MB: 5.0 TB/s;
-// maps 20), 32768 x 127 x 3 fp32, last state only, 26 us (67 MB: 2.5 TB/s: two rounds of workgroups of one tile, a third of the time instructions and
+// maps 20), 32768 x 127 x 3 fp32, last state only, 26 us (67 MB: 2.5 TB/s: two rounds of workgroups of one tile, 38 % of the time instructions and
 // the rest latency of loads, lane exchanges and barriers).
 template <int DX, int DG, int VEC, bool SHARED, bool MAP>
 __global__ __launch_bounds__(NM_S_THREADS) void nm_scan_forward_kernel(NmScanArgs p) {
@@ -559,7 +559,7 @@ __global__ __launch_bounds__(NM_S_THREADS) void nm_scan_forward_kernel(NmScanArg
 
 // MAP: only the range's map of the flow, up to its first sequence end.
 // Measured, main launch: 8192 packed sequences of 96 x 32 fp32 with h0 118 us (503 MB: 4.3 TB/s; maps 23), 1 x 32768 x 256 bf16 27 us (84 MB: 3.0 TB/s), 2048 x
-// 127 x 32 bf16 with a shared gate 27 us (51 MB: 1.9 TB/s).  Bound by two or three workgroups per CU (180 .. 200 registers): a bound of three for
+// 127 x 32 bf16 with a shared gate 27 us (51 MB: 1.9 TB/s).  Bound by two or three workgroups per CU (163 .. 193 registers): a bound of three for
 // all of them spills and costs 35 us instead of 27 for the second.
 template <int DX, int DG, int VEC, bool SHARED, bool MAP>
 __global__ __launch_bounds__(NM_S_THREADS) void nm_scan_backward_kernel(NmScanArgs p) {

@@ -156,9 +156,10 @@ def dense(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] = 
     """act(x weight^T + bias) + residual.
 
     x [..., K], weight [N, K] (as nn.Linear stores it), bias [N], residual [..., N] -> [..., N], all of one element type (fp32, fp16, bf16; the
-    bias may be fp32 beside 16-bit rows).  activation: one of ACTIVATIONS; softplus is log(1 + exp(beta z)) / beta, beta in
-    [2^-126, 2^126] (100 as in the geometry network), GELU its tanh form.  Differentiable in all four tensors.  Rows may be strided (a column slice of a wider tensor); other
-    layouts are copied.  One row to many: up to 8 rows go through a form that reads the weights once and in place.
+    bias may be fp32 beside 16-bit rows); K, N <= 2^20.  activation: one of ACTIVATIONS; softplus is log(1 + exp(beta z)) / beta, beta in
+    [2^-126, 2^126] (100 as in the geometry network), GELU its tanh form.  Differentiable in all four tensors: act'(z) is kept for the backward
+    pass (3 bytes per output beside 16-bit rows, 4 beside fp32).  Rows may be strided (a column slice of a wider tensor); other layouts are copied.
+    One row to many: up to 8 rows go through a form that reads the weights once and in place.
     fp32 products are as accurate as an fp32 matrix product; a non-finite operand makes the outputs it enters NaN there, and so in gradients
     beside an activation."""
     if activation not in ACTIVATIONS:
@@ -247,7 +248,8 @@ def gated_scan(gate: torch.Tensor, x: torch.Tensor, h0: Optional[torch.Tensor] =
     cu_seqlens[s] .. cu_seqlens[s+1] - 1, rows outside belong to none (states and gradients 0).
     gate: as x, or [..., 1]: one for all channels of a row; of x's element type or fp32.  |gate| <= 1 (blend: 0 <= gate <= 1).
     h0 [B,D] / [S,D]: the state before each sequence (None = 0).  states as x (None with need_states=False: nothing is written), last [B,D] / [S,D]
-    fp32: the state behind each sequence, h0 of the next call where a sequence goes on.  Differentiable in gate, x and h0."""
+    fp32: the state behind each sequence, h0 of the next call where a sequence goes on.  Differentiable in gate, x and h0.  Less than 2^31 rows and
+    sequences, at most 2^20 channels."""
     if not isinstance(x, torch.Tensor) or not isinstance(gate, torch.Tensor):
         raise ValueError("gated_scan: gate and x must be tensors")
     packed = cu_seqlens is not None
@@ -276,9 +278,10 @@ def gated_scan(gate: torch.Tensor, x: torch.Tensor, h0: Optional[torch.Tensor] =
 def composite_features(alpha: torch.Tensor, features: torch.Tensor, background: Optional[torch.Tensor] = None, *, cu_seqlens: Optional[torch.Tensor] = None) -> torch.Tensor:
     """Alpha compositing of any number of channels along rays: sum_i T_i alpha_i features_i + T_N background, T_i = prod_{j<i} (1 - alpha_j).
 
-    alpha [R,N] and features [R,N,C] ordered near to far (as volume_render's `alpha` and the samples are), or packed alpha [L] and
+    alpha [R,N] and features [R,N,C] ordered near to far, as volume_render's detailed `alpha` and its samples are, or packed alpha [L] and
     features [L,C] with cu_seqlens [R+1] for rays with different numbers of samples.  alpha in [0,1], of the features' type or fp32; background [R,C].
-    -> [R,C] fp32, differentiable in all three."""
+    -> [R,C] fp32, differentiable in all three.  (volume_render's own `alpha` carries no gradient unless it composites with NEUMESH_COMPOSITE=torch: to
+    train the geometry through these features, take alpha from the sdf with torch, as renderer.sdf_to_alpha does.)"""
     if not isinstance(alpha, torch.Tensor) or not isinstance(features, torch.Tensor) or alpha.shape != features.shape[:-1]:
         raise ValueError(f"composite_features: alpha {tuple(getattr(alpha, 'shape', ()))} must have the shape of features {tuple(getattr(features, 'shape', ()))} without channels")
     return gated_scan(alpha.unsqueeze(-1), features, background, cu_seqlens=cu_seqlens, reverse=True, blend=True, need_states=False)[1]
