@@ -319,3 +319,50 @@ def test_training_layer_beyond_32_bits():
     du, dc = torch.autograd.grad(ops.dense(u, w, c, activation="silu"), (u, c), g[-70000:])
     # sums of 70000 terms of size one in two orders; rounding of one value to 8 bits twice
     assert ((dx[-70000:].float() - du.float()).abs() <= 2.0 ** -7 * du.float().abs() + 1e-5).all() and (db - dc).abs().max() <= 70000 * 2.0 ** -22
+
+
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+def test_widest_layers_and_scans(dtype):
+    """2^20 inputs, outputs and channels: the last ones of each as exact as the first."""
+    t, W = TYPES[dtype], 1 << 20
+    gen = torch.Generator(device="cuda").manual_seed(9)
+
+    def rand(*s):
+        return torch.rand(s, generator=gen, device="cuda").to(t)
+    half = torch.finfo(t).eps / 2
+    for M, K, N in ((3, W, 2), (20, W, 3), (3, 2, W), (20, 5, W)):
+        x, w, g = rand(M, K).requires_grad_(True), rand(N, K).requires_grad_(True), rand(M, N)
+        y = ops.dense(x, w)
+        dx, dw = torch.autograd.grad(y, (x, w), g)
+        x64, w64, g64 = x.detach().double(), w.detach().double(), g.double()
+        for got, want, terms in ((y, x64 @ w64.t(), K), (dx, g64 @ w64, N), (dw, g64.t() @ x64, M)):
+            # terms of one sign: every matrix instruction (16 terms at least) may truncate a unit in the last place of the sum so far, and so may each of its pieces
+            assert ((got.double() - want).abs() <= (half + (terms / 16 * 6 + 8) * 2.0 ** -23) * want.abs()).all(), (M, K, N)
+    for T, packed in ((1, False), (5, False), (9, True)):
+        gate, x = (rand(2, T, 1) if not packed else rand(T, 1)).requires_grad_(True), (rand(2, T, W) if not packed else rand(T, W)).requires_grad_(True)
+        cu = torch.tensor([0, 4, 8], device="cuda") if packed else None
+        states, last = ops.gated_scan(gate, x, cu_seqlens=cu)
+        dgate, dx = torch.autograd.grad(last, (gate, x), torch.ones_like(last))
+        rows = [range(0, 4), range(4, 8)] if packed else [range(T)] * 2
+        for s in range(2):
+            a, v = (gate if packed else gate[s]).detach().double(), (x if packed else x[s]).detach().double()
+            h = [torch.zeros(W, dtype=torch.float64, device="cuda")]
+            for i in rows[s]:
+                h.append(a[i] * h[-1] + v[i])
+            f = torch.ones(W, dtype=torch.float64, device="cuda")
+            assert ((last[s].double() - h[-1]).abs() <= 16 * 2.0 ** -23 * h[-1]).all()
+            for k, i in reversed(list(enumerate(rows[s]))):
+                got_x, got_a = (dx if packed else dx[s])[i].double(), (dgate if packed else dgate[s])[i].double()
+                assert ((got_x - f).abs() <= (half + 16 * 2.0 ** -23) * f).all()
+                want = (f * h[k]).sum()
+                assert abs(got_a - want) <= (half + 2.6e-4) * want     # (2^20 terms in 4096 blocks of 256, then the blocks in order: 4096 + 20 roundings of 2^-24)
+                f = f * a[i]
+        if packed:
+            assert (states[8:] == 0).all() and (dx[8:] == 0).all() and (dgate[8:] == 0).all()
+
+
+def test_backward_twice_through_one_graph():
+    for make in (dense_slices, packed_scan):
+        out, leaves, cots = make()
+        first = torch.autograd.grad(out, leaves, cots, retain_graph=True)
+        assert all(torch.equal(a, b) for a, b in zip(first, torch.autograd.grad(out, leaves, cots)))
