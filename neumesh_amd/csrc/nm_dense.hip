@@ -11,13 +11,12 @@
 // nm_dense_few_kernel serves 1 .. 8 rows (a probe, a picked point).
 //
 // Arithmetic.  16-bit inputs: one product per pair on the f16 / bf16 pipe, fp32 accumulation, fp32 epilogue, one rounding at the end.  The forward pass
-// keeps act'(z) for the backward pass (NmFactor).  dz = g act'(z) enters the products as TWO bf16
-// pieces (value + residual: 16 bits, over fp32's whole range): a single rounded piece put an error as large as the output's own rounding on dx and
-// dW, and fp16 pieces lost what lies below 2^-13 (g of a mean over many outputs) and beyond 65504 (g near the maximum times act' = 1.13).
-// Beside fp16 rows the other operand is cut into two bf16 pieces as well, exactly, and three piece products are taken (10007 x 177 -> 131 forward and
-// backward 123 us, 126 with two products of fp16 pieces).  fp32 inputs: every operand cut into three bf16 pieces (nm_gemm.h: exact), six piece
-// products, fp32 accumulation.  A product of several pieces with a non-finite operand is NaN where IEEE arithmetic may
-// give an infinity.
+// keeps act'(z) for the backward pass (NmFactor).  dz = g act'(z) enters the products as TWO bf16 pieces (value + residual: 16 bits over fp32's whole
+// range, an error of 1/32 (fp16) and 1/256 (bf16) of the result's own rounding): a single rounded piece put an error as large as that rounding on dx and
+// dW, and fp16 pieces lost what lies below 2^-13 (g of a mean over many outputs) and beyond 65504 (g near the maximum times act' = 1.13).  Beside fp16
+// rows the other operand is cut into two bf16 pieces as well, exactly, and three piece products are taken (10007 x 177 -> 131 forward and backward 123 us,
+// 126 with two products of fp16 pieces).  fp32 inputs: every operand cut into three bf16 pieces (nm_d_cut8), six piece products, fp32 accumulation.  A
+// product of several pieces with a non-finite operand is NaN where IEEE arithmetic may give an infinity.
 #include "nm_error.h"
 #include "nm_num.h"
 
